@@ -346,6 +346,69 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
                             int history_capacity, void* stream);
 
 /*
+ * Low-rank adapters of many requests beside shared projections (1..3 of equal k_in, as b200rwkv_gemm_u8 takes them):
+ *   out_i[r][:] = y_i[r][:] + scale_i[id] * (x_i[r][:] A_i[id]^T) B_i[id]^T,   id = ids[r / tokens_per_stream]
+ * for rows r of streams with an adapter; an id outside [0, n_adapters) means none, and out_i[r] = y_i[r].
+ *   banks     a device [n_adapters][rank][k_in], b device [n_adapters][n_out][rank] of `dtype` (B200RWKV_F32 / _BF16 / _F16),
+ *             16-byte aligned; scale device f32 [n_adapters], NULL for 1.  rank a multiple of 4 up to 256, k_in of 8
+ *   x, y, out device [streams * tokens_per_stream][k_in] and [...][n_out_i] of row_dtype (f32, or the weights' type), x
+ *             16-byte aligned; out_i may be y_i and overlaps nothing else.  Rows <= 65535
+ *   ids       device int64 [streams], read on the device (a captured call follows them)
+ *   workspace b200rwkv_adapt_rows_workspace_bytes(...) (0: a size that is not taken, or no device), 256-byte aligned; nothing
+ *             is kept in it between calls
+ * Sums are f32 over exact products of 16-bit pieces, h = x A^T stays f32, and out is rounded once.  Sums go over fixed parts
+ * in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
+ * adapter.  Two launches on `stream`, no allocation, capturable.  No counterpart in the reference.
+ */
+typedef struct b200rwkv_adapters {
+  const void *a, *b;
+  const float* scale;
+  int32_t n_out;
+} b200rwkv_adapters;
+size_t b200rwkv_adapt_rows_workspace_bytes(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype,
+                                           int streams, int tokens_per_stream);
+int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, const void* const* x,
+                        const void* const* y, void* const* out, int row_dtype, const int64_t* ids, int streams, int tokens_per_stream,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Verification of drafted tokens.  Per stream, step t = 0, 1, ... (up to its number of drafted tokens): token d is accepted
+ * where u[t] * q_t(d) / Q_t < p_t(d) / P_t, with the target's weights p_t of sum P_t and the draft's q_t of sum Q_t.  At the
+ * first refusal one token is drawn from max(0, p_t/P_t - q_t/Q_t) (from p_t where that is empty); with all accepted, from the
+ * target's next row.  Draws are inverse CDF in index order with u[drafts]: the first token of positive weight at which the
+ * running sum reaches u times the whole.  So the tokens are distributed as the target's own would be.
+ *   target    device f32, row t of stream s at target + s * target_stream_stride + t * target_row_stride, drafts + 1 rows of
+ *             n weights (as probs_out of b200rwkv_sample_typical: any sum; what is not above zero counts as zero; finite)
+ *   draft     the same with `drafts` rows, or NULL: the draft is sure of its tokens (q_t(d) = 1), as one looked up in a text is
+ *   tokens    device int64 [streams][drafts]; one outside [0, n) is refused
+ *   u         device f32 [streams][drafts + 1], uniform in [0,1)
+ *   lengths   device int64 [streams], drafted tokens of each stream (clamped to [0, drafts]), or NULL: all
+ *   out       device int64 [streams][drafts + 1]: the accepted tokens, the drawn one, -1 behind it; the drawn one is -1 where
+ *             its row has no weight above zero
+ *   accepted  device int64 [streams]
+ *   workspace b200rwkv_verify_drafts_workspace_bytes(streams, drafts, n) (0: a size that is not taken), 8-byte aligned; nothing is kept in it
+ * All sums and comparisons are fp64.  drafts <= 64, n <= 524288, streams <= 65535.  A stream's result does not depend on the
+ * others.  Two launches, no allocation, capturable.  No counterpart in the reference.
+ */
+size_t b200rwkv_verify_drafts_workspace_bytes(int streams, int drafts, int n);
+int b200rwkv_verify_drafts(const float* target, int64_t target_stream_stride, int64_t target_row_stride, const float* draft,
+                           int64_t draft_stream_stride, int64_t draft_row_stride, const int64_t* tokens, const float* u,
+                           const int64_t* lengths, int streams, int drafts, int n, int64_t* out, int64_t* accepted, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
+ * The recurrent state after the first counts[s] of a step's `tokens` tokens, all blocks in one launch (a step whose later
+ * tokens were refused).  state and out device f32 [streams][layers][5][channels] (rows as in b200rwkv_forward_rows; out may be
+ * state); counts device int64 [streams], clamped to [0, tokens], 0 leaves the state as it is; trace device f32
+ * [layers][4][streams][tokens][channels]: the residual stream in front of ln1 and of ln2, key and value of every token; params
+ * device f32 [layers][5][channels]: ln1 weight and bias, ln2 weight and bias, w = -exp(time_decay).  Row 0 / 1 become the layer
+ * norm of the last accepted token's rows, rows 2..4 take counts[s] WKV steps (agnosticRwkv.py:68-103).  channels a multiple of 4;
+ * all buffers 16-byte aligned.  One launch, no allocation, capturable.
+ */
+int b200rwkv_advance_state(const float* state, float* out, const int64_t* counts, const float* trace, const float* params, int streams,
+                           int layers, int tokens, int channels, void* stream);
+
+/*
  * Unquantised weights: the TORCH-mode matrix-vector product of the reference
  * (agnostic/backends/torch.py:162-164, `x.to(W.dtype).matmul(W).to(x.dtype)`).
  *   y[o] = round_T( sum_j round_T(x[j]) * W[o][j] ),  T = the weights' type, fp32 accumulation

@@ -22,6 +22,8 @@ EXPORTS = (
     "b200rwkv_decode_workspace_bytes", "b200rwkv_decode_step", "b200rwkv_decode_step_traced", "b200rwkv_decode_step_stage",
     "b200rwkv_gemm_plan", "b200rwkv_gemm_workspace_bytes", "b200rwkv_gemm_u8", "b200rwkv_rows_workspace_bytes", "b200rwkv_forward_rows", "b200rwkv_forward_rows_stage", "b200rwkv_argmax",
     "b200rwkv_sample_typical", "b200rwkv_gemv_dense",
+    "b200rwkv_adapt_rows_workspace_bytes", "b200rwkv_adapt_rows", "b200rwkv_verify_drafts_workspace_bytes", "b200rwkv_verify_drafts",
+    "b200rwkv_advance_state",
     "b200rwkv_dense_workspace_bytes", "b200rwkv_dense_step", "b200rwkv_dense_rows_workspace_bytes", "b200rwkv_dense_forward_rows",
     "b200rwkv_dense_step_layers", "b200rwkv_dense_forward_rows_layers", "b200rwkv_wait_selftest", "b200rwkv_debug_expire_waits",
     "b200rwkv_step_plan_bytes", "b200rwkv_step_plan_init", "b200rwkv_decode_step_persistent", "b200rwkv_step_geometry",
@@ -46,6 +48,10 @@ class Model(C.Structure):
                 ("emb", C.c_void_p), ("ln0_w", C.c_void_p), ("ln0_b", C.c_void_p),
                 ("ln_out_w", C.c_void_p), ("ln_out_b", C.c_void_p), ("head", Matrix),
                 ("layers", C.POINTER(Layer))]
+
+
+class Adapters(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("n_out", C.c_int32)]
 
 
 class DenseLayer(C.Structure):
@@ -137,6 +143,18 @@ def lib() -> C.CDLL:
     L.b200rwkv_sample_typical.restype = C.c_int
     L.b200rwkv_sample_typical.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_float, C.c_float, C.c_void_p,
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
+    L.b200rwkv_adapt_rows_workspace_bytes.restype = C.c_size_t
+    L.b200rwkv_adapt_rows_workspace_bytes.argtypes = [C.c_int, C.POINTER(Adapters)] + [C.c_int] * 6
+    L.b200rwkv_adapt_rows.restype = C.c_int
+    L.b200rwkv_adapt_rows.argtypes = ([C.c_int, C.POINTER(Adapters)] + [C.c_int] * 4 + [C.POINTER(C.c_void_p)] * 3 +
+                                      [C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p])
+    L.b200rwkv_verify_drafts_workspace_bytes.restype = C.c_size_t
+    L.b200rwkv_verify_drafts_workspace_bytes.argtypes = [C.c_int] * 3
+    L.b200rwkv_verify_drafts.restype = C.c_int
+    L.b200rwkv_verify_drafts.argtypes = ([C.c_void_p, C.c_int64, C.c_int64] * 2 + [C.c_void_p] * 3 + [C.c_int] * 3 +
+                                         [C.c_void_p] * 3 + [C.c_size_t, C.c_void_p])
+    L.b200rwkv_advance_state.restype = C.c_int
+    L.b200rwkv_advance_state.argtypes = [C.c_void_p] * 5 + [C.c_int] * 4 + [C.c_void_p]
     L.b200rwkv_gemv_dense.restype = C.c_int
     L.b200rwkv_gemv_dense.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p,
                                       C.c_void_p]

@@ -1,0 +1,472 @@
+// Low-rank adapters of many requests beside shared projections: out[row] = y[row] + scale[id] * (x[row] A[id]^T) B[id]^T
+// for rows whose stream has adapter id, out[row] = y[row] for the others.  A [rank][K], B [N][rank] per adapter.
+//
+// Two launches.  The first forms h = x A^T (K long, rank short), the second adds h B^T onto y (rank short, N long).
+// Rows of one adapter share its weights: a CTA takes a tile of up to `rt` rows that all have the same adapter.  Streams of
+// rt rows or more are cut into tiles; shorter ones are gathered: CTA s looks through the ids of its window of kAdaptWindow
+// streams, in the order of the streams, and leads a tile where a multiple of rt rows of its adapter ends in front of one of
+// its rows.  So no pass sorts the rows and no count travels to the host; CTAs that lead nothing leave.
+//
+// Products run on the tensor cores (mma.sync m16n8k16) with fp32 sums.  Operands that are not of one 16-bit type are cut
+// into bfloat16 pieces: a float is exactly three (the upper 8 bits of its significand, the next 8, the last 8), a half
+// exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21 of the whole together and left out, and those of
+// the small pieces are summed apart from the large ones.  A piece of an infinity is NaN: a row of x that holds an infinity
+// or a NaN comes out as NaN, where it has an adapter.
+// What bounds both is memory: h takes rank multiplications per value of x, y takes rank per value.  At rank 64 with fp32 rows
+// that is 48 products of pieces a byte, below what mma.sync sustains beside the loads, so nothing is gained by staging
+// operands for tcgen05; fragments go from global memory to registers directly.  The index along a product is free to permute,
+// and is, so that a lane's elements are consecutive: 16 bytes of A, 8 of B.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int kAdaptMaxMats = 3;
+constexpr int kAdaptWindow = 1024;         // streams
+constexpr int kAdaptMaxRank = 256;
+constexpr int kAdaptMaxRows = 64;          // of a tile
+constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
+constexpr int kExpandThreads = 128, kExpandWarps = kExpandThreads / 32, kExpandCols = 32;   // columns of a warp at a time
+
+struct AdaptParams {
+  const void *a[kAdaptMaxMats], *b[kAdaptMaxMats], *x[kAdaptMaxMats], *y[kAdaptMaxMats];
+  void* out[kAdaptMaxMats];
+  const float* scale[kAdaptMaxMats];       // null: 1
+  float* h[kAdaptMaxMats];                 // [splits][rows][rank]
+  int n_out[kAdaptMaxMats];
+  int chunk_end[kAdaptMaxMats];            // second launch: column chunks of the matrices up to and including this one
+  int vec[kAdaptMaxMats];                  // rows of y and out start on boundaries of four elements
+  const long long* ids;
+  int nmat, adapters, rank, K, R, T, streams, rt, splits, chunk_cols;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Elements 2i and 2i + 1 of a lane's, as loaded (16-bit types) or as floats.
+template <typename T>
+struct AdaptType;
+template <> struct AdaptType<__nv_bfloat16> { static constexpr int kPieces = 1; };
+template <> struct AdaptType<__half> { static constexpr int kPieces = 2; };
+template <> struct AdaptType<float> { static constexpr int kPieces = 3; };
+
+// The upper halves of two floats, and what they leave (exactly).
+__device__ __forceinline__ uint32_t take_piece(float& lo, float& hi) {
+  const uint32_t l = __float_as_uint(lo), u = __float_as_uint(hi);
+  lo -= __uint_as_float(l & 0xffff0000u);
+  hi -= __uint_as_float(u & 0xffff0000u);
+  return __byte_perm(l, u, 0x7632);
+}
+template <int P>
+__device__ __forceinline__ void split_pair(float lo, float hi, uint32_t (&p)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) p[i] = take_piece(lo, hi);
+}
+
+// N consecutive elements of T (N * sizeof(T) a multiple of 8), zero where !ok.
+template <typename T, int N>
+struct AdaptRaw {
+  static constexpr int kWords = N * int(sizeof(T)) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p, bool ok) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    if (!ok) return;
+    if constexpr (kWords % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
+    }
+  }
+  // pieces of the pair of elements 2i, 2i + 1
+  template <int P>
+  __device__ __forceinline__ void pair(int i, uint32_t (&p)[P]) const {
+    if constexpr (P == 1) {
+      p[0] = w[i];
+    } else if constexpr (std::is_same<T, float>::value) {
+      split_pair<P>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), p);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      split_pair<P>(f.x, f.y, p);
+    }
+  }
+};
+
+// The rows of tile `tile` into rows[0..count): returns count, 0 where this CTA leads none.  *id: their adapter, -1: none.
+// All threads of the CTA take part; mask: kAdaptWindow / 32 words of shared memory.
+__device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* rows, uint32_t* mask, int* id) {
+  const int tid = threadIdx.x, nt = blockDim.x, T = P.T, rt = P.rt;
+  auto id_of = [&](int s) {
+    const long long v = __ldg(P.ids + s);
+    return v >= 0 && v < P.adapters ? int(v) : -1;
+  };
+  if (T >= rt) {
+    const int per = (T + rt - 1) / rt, s = tile / per, first = (tile - s * per) * rt, n = min(rt, T - first);
+    *id = id_of(s);
+    for (int i = tid; i < n; i += nt) rows[i] = s * T + first + i;
+    __syncthreads();
+    return n;
+  }
+  const int w0 = tile / kAdaptWindow * kAdaptWindow, count = min(kAdaptWindow, P.streams - w0);
+  const int mine = id_of(tile);
+  for (int i = tid; i < kAdaptWindow; i += nt) {
+    const unsigned m = __ballot_sync(0xffffffffu, i < count && id_of(w0 + i) == mine);
+    if ((i & 31) == 0) mask[i >> 5] = m;
+  }
+  __syncthreads();
+  int before = 0, all = 0;                               // streams of this adapter in front of this one, and in the window
+  for (int w = 0; w < kAdaptWindow / 32; ++w) {
+    const uint32_t m = mask[w];
+    const int at = tile - w0 - 32 * w;                   // bits of this word in front of the stream's own
+    before += __popc(at >= 32 ? m : at > 0 ? m & ((1u << at) - 1u) : 0u);
+    all += __popc(m);
+  }
+  const int lead = (before * T + rt - 1) / rt * rt;      // the first tile that starts at or behind this stream's first row
+  if (lead >= (before + 1) * T) return 0;
+  const int n = min(rt, all * T - lead);
+  *id = mine;
+  if (tid < n) {
+    int skip = (lead + tid) / T;                         // the stream of this row, counted among the adapter's
+    const int token = lead + tid - skip * T;
+    int w = 0;
+    while (skip >= __popc(mask[w])) skip -= __popc(mask[w++]);
+    uint32_t m = mask[w];
+    for (; skip > 0; --skip) m &= m - 1;
+    rows[tid] = (w0 + 32 * w + __ffs(m) - 1) * T + token;
+  }
+  __syncthreads();
+  return n;
+}
+
+// h[split][row][j] = sum over the split's K of x[row][k] A[id][j][k].  Grid (tiles, rank chunks of 16 * MT, matrices * splits).
+// A warp takes 16 rows (as columns of the products, 8 at a time) and, of the split's blocks of 32 k, every (8 / row ways)-th.
+template <typename TX, typename TW, int MT, int NT>
+__device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int mat, int split, int chunk, const int* rows,
+                                            int count, float* red) {
+  constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
+  constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
+  constexpr int RC = 16 * MT, kStride = RC + 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int K = P.K, rank = P.rank;
+  // row ways, ways along K: the same for every tile of a call, so that a row's sums do not depend on the rows beside it
+  const int rw = P.rt / 16, kw = kShrinkWarps / rw;
+  const int my_rows = (warp % rw) * 16, my_k = warp / rw;
+  const TX* xp[NT];
+  bool xok[NT];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) {
+    const int i = my_rows + q * 8 + g;
+    xok[q] = i < count;
+    xp[q] = x + size_t(xok[q] ? rows[i] : 0) * K + 8 * t;
+  }
+  const TW* ap[MT][2];
+  bool aok[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = chunk * RC + m * 16 + e * 8 + g;
+      aok[m][e] = j < rank;
+      ap[m][e] = a + size_t(aok[m][e] ? j : 0) * K + 8 * t;
+    }
+  float big[MT][NT][4], small[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) big[m][q][i] = small[m][q][i] = 0.f;
+  const int blocks = (K + 31) / 32, b0 = int((long long)blocks * split / P.splits), b1 = int((long long)blocks * (split + 1) / P.splits);
+#pragma unroll 2
+  for (int kb = b0 + my_k; kb < b1; kb += kw) {
+    const int k = kb * 32;
+    const bool in = k + 8 * t < K;                       // K is a multiple of 8
+    AdaptRaw<TX, 8> rx[NT];
+    AdaptRaw<TW, 8> ra[MT][2];
+#pragma unroll
+    for (int q = 0; q < NT; ++q) rx[q].load(xp[q] + k, in && xok[q]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) ra[m][e].load(ap[m][e] + k, in && aok[m][e]);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {               // elements 4 step .. 4 step + 3 of every lane
+      uint32_t fx[NT][2][PX];
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rx[q].template pair<PX>(2 * step + i, fx[q][i]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint32_t fa[4][PW];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ra[m][i & 1].template pair<PW>(2 * step + (i >> 1), fa[i]);
+#pragma unroll
+        for (int i = 0; i < PW; ++i) {
+          const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int j = 0; j < PX; ++j) {
+              if (i + j >= 3) continue;
+              if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(big[m][q], f, fx[q][0][j], fx[q][1][j]);
+              else mma_bf16(i + j ? small[m][q] : big[m][q], f, fx[q][0][j], fx[q][1][j]);
+            }
+        }
+      }
+    }
+  }
+  // products' rows are ranks (g, g + 8), their columns rows of x (2t, 2t + 1)
+  float* mine = red + warp * (16 * kStride);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[(q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = big[m][q][i] + small[m][q][i];
+  __syncthreads();
+  float* h = P.h[mat] + size_t(split) * P.R * rank;
+  for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
+    const int r = i / RC, j = i - r * RC;
+    if (chunk * RC + j >= rank) continue;
+    float s = 0.f;
+    for (int w = 0; w < kw; ++w) s += red[((w * rw + (r >> 4)) * 16 + (r & 15)) * kStride + j];
+    h[size_t(rows[r]) * rank + chunk * RC + j] = s;
+  }
+}
+
+template <typename TX, typename TW, int MT>
+__global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const AdaptParams P) {
+  __shared__ float red[kShrinkWarps * 16 * (16 * MT + 4)];
+  __shared__ int rows[kAdaptMaxRows];
+  __shared__ uint32_t mask[kAdaptWindow / 32];
+  griddep_launch_dependents();
+  int id = -1;
+  const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
+  if (count == 0 || id < 0) return;
+  const int mat = blockIdx.z / P.splits, split = blockIdx.z - mat * P.splits;
+  const TX* x = static_cast<const TX*>(P.x[mat]);
+  const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
+  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, red);
+  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, red);
+}
+
+// 16-byte blocks of a row of h in shared memory: an odd number of 32-byte groups, so that 8-byte reads of eight rows by four
+// lanes each meet every bank once.
+__host__ __device__ constexpr int expand_stride(int rank) { return ((rank + 15) / 16 | 1) * 16; }
+
+template <typename TY>
+__device__ __forceinline__ float adapt_load(const TY* p) {
+  if constexpr (std::is_same<TY, float>::value) return *p;
+  else if constexpr (std::is_same<TY, __half>::value) return __half2float(*p);
+  else return __bfloat162float(*p);
+}
+template <typename TY>
+__device__ __forceinline__ void adapt_store(TY* p, float v) {
+  if constexpr (std::is_same<TY, float>::value) *p = v;
+  else if constexpr (std::is_same<TY, __half>::value) *p = __float2half_rn(v);
+  else *p = __float2bfloat16_rn(v);
+}
+
+// Four consecutive elements as floats and back, through one access.
+template <typename TY>
+__device__ __forceinline__ float4 adapt_load4(const TY* p) {
+  if constexpr (std::is_same<TY, float>::value) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    float2 a, b;
+    if constexpr (std::is_same<TY, __half>::value) {
+      a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)); b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    } else {
+      a = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
+      b = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+    }
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+template <typename TY>
+__device__ __forceinline__ void adapt_store4(TY* p, float4 f) {
+  if constexpr (std::is_same<TY, float>::value) {
+    *reinterpret_cast<float4*>(p) = f;
+  } else {
+    uint2 v;
+    if constexpr (std::is_same<TY, __half>::value) {
+      *reinterpret_cast<__half2*>(&v.x) = __floats2half2_rn(f.x, f.y); *reinterpret_cast<__half2*>(&v.y) = __floats2half2_rn(f.z, f.w);
+    } else {
+      *reinterpret_cast<__nv_bfloat162*>(&v.x) = __floats2bfloat162_rn(f.x, f.y);
+      *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(f.z, f.w);
+    }
+    *reinterpret_cast<uint2*>(p) = v;
+  }
+}
+
+// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles, column chunks of all matrices).
+// A warp takes 32 columns and 32 rows at a time; the columns of two products are dealt out so that a lane ends up with four
+// consecutive ones.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16 bits, enough for a 16-bit y.
+template <typename TY, typename TW>
+__global__ void __launch_bounds__(kExpandThreads) adapt_expand_kernel(const AdaptParams P) {
+  extern __shared__ __align__(16) unsigned short hs[];     // [pieces][rt][stride]
+  __shared__ int rows[kAdaptMaxRows];
+  __shared__ uint32_t mask[kAdaptWindow / 32];
+  constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  int id = -1;
+  const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
+  int mat = 0;
+  while (mat < P.nmat - 1 && int(blockIdx.y) >= P.chunk_end[mat]) ++mat;
+  const int N = P.n_out[mat], chunk = int(blockIdx.y) - (mat ? P.chunk_end[mat - 1] : 0);
+  const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
+  const TY* y = static_cast<const TY*>(P.y[mat]);
+  TY* out = static_cast<TY*>(P.out[mat]);
+  if (count == 0) return;
+  if (id < 0) {                                            // no adapter: only a copy, where out is not y
+    if (y == out) return;
+    for (int i = warp; i < count; i += kExpandWarps) {
+      const size_t row = size_t(rows[i]) * N;
+      for (int c = c_begin + lane; c < c_end; c += 32) out[row + c] = y[row + c];
+    }
+    return;
+  }
+  const int rank = P.rank, ksteps = (rank + 15) / 16, stride = expand_stride(rank), padded = (count + 15) / 16 * 16;
+  griddep_wait();
+  {
+    const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
+    const int r4 = ksteps * 4, plane = P.rt * stride;      // groups of four ranks
+    for (int i = tid; i < padded * r4; i += kExpandThreads) {
+      const int r = i / r4, j = (i - r * r4) * 4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < count && j < rank) {                         // rank is a multiple of four
+        const float* h = P.h[mat] + size_t(rows[r]) * rank + j;
+        for (int p = 0; p < P.splits; ++p) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(h + size_t(p) * P.R * rank));
+          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+      }
+      uint32_t lo[PH], hi[PH];
+      split_pair<PH>(s.x * scale, s.y * scale, lo);
+      split_pair<PH>(s.z * scale, s.w * scale, hi);
+#pragma unroll
+      for (int p = 0; p < PH; ++p) *reinterpret_cast<uint2*>(hs + size_t(p) * plane + r * stride + j) = make_uint2(lo[p], hi[p]);
+    }
+  }
+  __syncthreads();
+  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  const int plane = P.rt * stride;
+  for (int c0 = c_begin + warp * kExpandCols; c0 < c_end; c0 += kExpandWarps * kExpandCols) {
+    for (int m0 = 0; m0 < count; m0 += 32) {
+      float acc[2][4][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+      const bool second = m0 + 16 < count;
+#pragma unroll 1
+      for (int ks = 0; ks < ksteps; ++ks) {
+        uint32_t fb[4][2][PW];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int c = c0 + (n >> 1) * 16 + 4 * (g >> 1) + 2 * (n & 1) + (g & 1), j = ks * 16 + 4 * t;
+          AdaptRaw<TW, 4> raw;
+          const bool ok = c < c_end && j < rank;
+          raw.load(b + (ok ? size_t(c) * rank + j : 0), ok);
+          raw.template pair<PW>(0, fb[n][0]);
+          raw.template pair<PW>(1, fb[n][1]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          if (m && !second) break;
+#pragma unroll
+          for (int p = 0; p < PH; ++p) {
+            const unsigned short* at = hs + size_t(p) * plane + (m0 + m * 16 + g) * stride + ks * 16 + 4 * t;
+            const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8 * stride);
+            const uint32_t f[4] = {u.x, v.x, u.y, v.y};
+#pragma unroll
+            for (int w = 0; w < PW; ++w) {
+              if (p + w >= PH) continue;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) mma_bf16(acc[m][n], f, fb[n][0][w], fb[n][1][w]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = m0 + m * 16 + e * 8 + g;
+          if (i >= count) continue;
+          const size_t row = size_t(rows[i]) * N;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int c = c0 + q * 16 + 4 * t;
+            const float4 d = make_float4(acc[m][2 * q][2 * e], acc[m][2 * q][2 * e + 1], acc[m][2 * q + 1][2 * e], acc[m][2 * q + 1][2 * e + 1]);
+            if (P.vec[mat]) {
+              if (c < c_end) {
+                const float4 v = adapt_load4(y + row + c);
+                adapt_store4(out + row + c, make_float4(v.x + d.x, v.y + d.y, v.z + d.z, v.w + d.w));
+              }
+            } else {
+              const float f[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (c + k < c_end) adapt_store(out + row + c + k, adapt_load(y + row + c + k) + f[k]);
+            }
+          }
+        }
+    }
+  }
+}
+
+struct AdaptShape {
+  int rt, tiles, splits, mt, chunk_cols, chunks;   // mt: ranks of a CTA of the first launch, in 16
+};
+
+// Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
+// Splits of K: as many as make two CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a multiple
+// of what its warps take at a time, the more the more tiles there are.
+inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
+  AdaptShape s;
+  s.rt = T >= kAdaptMaxRows ? kAdaptMaxRows : 16;
+  const bool gathered = T < s.rt;
+  s.tiles = gathered ? streams : streams * ((T + s.rt - 1) / s.rt);
+  const long long rows = (long long)streams * T;
+  long long busy = s.tiles;                              // tiles that lead rows
+  if (gathered && adapters + rows / s.rt + 1 < busy) busy = adapters + rows / s.rt + 1;
+  s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
+  const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
+  long long splits = 2LL * sms / ctas;
+  if (splits > K / 256) splits = K / 256;
+  s.splits = int(splits < 1 ? 1 : splits > 16 ? 16 : splits);
+  const int unit = kExpandWarps * kExpandCols;
+  long long units = 0;
+  for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
+  long long per = units * busy / (8LL * sms);            // column units a CTA takes for eight CTAs per SM
+  s.chunk_cols = unit * int(per < 1 ? 1 : per > 16 ? 16 : per);
+  s.chunks = 0;
+  for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
+  return s;
+}
+
+}  // namespace b200

@@ -14,6 +14,9 @@
 #include "decode_step.cuh"
 #include "dense_step.cuh"
 #include "dense_gemm.cuh"
+#include "adapters.cuh"
+#include "verify.cuh"
+#include "advance.cuh"
 
 namespace b200 {
 
@@ -727,6 +730,51 @@ static cudaError_t launch_sample(const float* x, int rows, int n, long long ldx,
     case 4: return as(launch_sample_as<true, 2>);
     default: return sample_part(n) <= kSampleMaxSlice ? as(launch_sample_as<true, 1>) : as(launch_sample_as<false, 1>);
   }
+}
+
+// ---------------------------------------------------------------------------------------- adapters, verification
+template <typename TX, typename TW>
+static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  const dim3 grid(sh.tiles, (P.rank + 16 * sh.mt - 1) / (16 * sh.mt), P.nmat * P.splits);
+  if (sh.mt == 1) return launch_chained(adapt_shrink_kernel<TX, TW, 1>, grid, dim3(kShrinkThreads), 0, stream, P);
+  if (sh.mt == 2) return launch_chained(adapt_shrink_kernel<TX, TW, 2>, grid, dim3(kShrinkThreads), 0, stream, P);
+  if constexpr (AdaptType<TW>::kPieces == 1) return launch_chained(adapt_shrink_kernel<TX, TW, 4>, grid, dim3(kShrinkThreads), 0, stream, P);
+  return cudaErrorInvalidValue;
+}
+
+template <typename TY, typename TW>
+static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  constexpr int pieces = sizeof(TY) == 2 ? 2 : 3;
+  static bool configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             pieces * kAdaptMaxRows * expand_stride(kAdaptMaxRank) * 2);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch_chained(adapt_expand_kernel<TY, TW>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
+                        size_t(pieces) * P.rt * expand_stride(P.rank) * 2, stream, P);
+}
+
+template <typename TY, typename TW>
+static cudaError_t launch_adapt(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  g_chain_launch = false;        // the first launch waits for the work in front of the call, which may still write its inputs
+  cudaError_t e = launch_adapt_shrink<TY, TW>(P, sh, stream);
+  return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, stream) : e;
+}
+
+static cudaError_t launch_verify(const VerifyParams& P, cudaStream_t stream) {
+  const long long items = (long long)P.B * (P.K + 1 + (P.draft ? P.K : 0)) * P.segs;
+  g_chain_launch = false;
+  cudaError_t e = launch_chained(verify_sums_kernel, dim3(unsigned((items + kVerifySumWarps - 1) / kVerifySumWarps)),
+                                 dim3(kVerifySumWarps * 32), 0, stream, P);
+  if (e != cudaSuccess) return e;
+  const int c = verify_cluster(P.B, P.segs, device_sms());
+  return launch_clustered(c, verify_draw_kernel, dim3(unsigned(P.B) * c), dim3(kVerifyThreads), 0, stream, P);
 }
 
 // ---------------------------------------------------------------------------------------- static scratch
@@ -1888,6 +1936,117 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
   cudaError_t e = launch_sample(x, rows, n, ldx, temp, tau, u, reinterpret_cast<long long*>(out), probs_out,
                                 reinterpret_cast<long long*>(history), history_count, history_capacity, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "sample_typical: %s", cudaGetErrorString(e));
+  return B200RWKV_OK;
+}
+
+// ---- many requests: adapters, verification of drafted tokens, the state after the accepted ones
+static int adapt_weight_pieces(int dtype) { return dtype == B200RWKV_F32 ? 3 : dtype == B200RWKV_F16 ? 2 : 1; }
+
+static const char* adapt_problem(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int streams, int tokens_per_stream) {
+  if (nmat < 1 || nmat > kAdaptMaxMats || !banks) return "1..3 banks";
+  if (n_adapters < 1 || rank < 4 || rank > kAdaptMaxRank || rank % 4) return "at least one adapter, rank a multiple of 4 up to 256";
+  if (k_in < 8 || k_in % 8) return "k_in a positive multiple of 8";
+  if (streams < 1 || tokens_per_stream < 1 || (long long)streams * tokens_per_stream > 65535) return "1..65535 rows";
+  for (int i = 0; i < nmat; ++i)
+    if (banks[i].n_out < 1 || banks[i].n_out > (1 << 22)) return "n_out 1..4194304";
+  return nullptr;
+}
+
+static AdaptShape adapt_shape_of(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, int streams, int T) {
+  int n_out[kAdaptMaxMats] = {0, 0, 0};
+  for (int i = 0; i < nmat; ++i) n_out[i] = banks[i].n_out;
+  return adapt_shape(nmat, n_out, n_adapters, rank, k_in, streams, T, adapt_weight_pieces(dtype), device_sms());
+}
+
+size_t b200rwkv_adapt_rows_workspace_bytes(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype,
+                                           int streams, int tokens_per_stream) {
+  if (adapt_problem(nmat, banks, n_adapters, rank, k_in, streams, tokens_per_stream) || !dense_elem_bytes(dtype) || device_sms() < 1) return 0;
+  const AdaptShape sh = adapt_shape_of(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
+  return size_t(nmat) * align256(size_t(sh.splits) * streams * tokens_per_stream * rank * 4);
+}
+
+int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, const void* const* x,
+                        const void* const* y, void* const* out, int row_dtype, const int64_t* ids, int streams, int tokens_per_stream,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (const char* p = adapt_problem(nmat, banks, n_adapters, rank, k_in, streams, tokens_per_stream))
+    return fail(B200RWKV_EINVAL, "adapt_rows: nmat=%d adapters=%d rank=%d k_in=%d streams=%d tokens=%d: %s", nmat, n_adapters, rank, k_in,
+                streams, tokens_per_stream, p);
+  if (!dense_elem_bytes(dtype) || (row_dtype != B200RWKV_F32 && row_dtype != dtype))
+    return fail(B200RWKV_EINVAL, "adapt_rows: weights f32, bf16 or f16, rows f32 or the weights' type (dtype=%d row_dtype=%d)", dtype, row_dtype);
+  if (!x || !y || !out || !ids || !workspace) return fail(B200RWKV_EINVAL, "adapt_rows: null argument");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return fail(B200RWKV_EINVAL, "adapt_rows: workspace must be 256-byte aligned");
+  if (device_sms() < 1) return fail(B200RWKV_ECUDA, "adapt_rows: no CUDA device");
+  const size_t need = b200rwkv_adapt_rows_workspace_bytes(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
+  if (workspace_bytes < need) return fail(B200RWKV_EINVAL, "adapt_rows: workspace %zu < %zu bytes", workspace_bytes, need);
+  const AdaptShape sh = adapt_shape_of(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
+  const size_t eb = size_t(dense_elem_bytes(row_dtype));
+  AdaptParams P;
+  memset(&P, 0, sizeof(P));
+  int chunks = 0;
+  for (int i = 0; i < nmat; ++i) {
+    const b200rwkv_adapters& m = banks[i];
+    if (!m.a || !m.b || !x[i] || !y[i] || !out[i] || !aligned16(m.a) || !aligned16(m.b) || !aligned16(x[i]))
+      return fail(B200RWKV_EINVAL, "adapt_rows: matrix %d: null pointer, or a, b or x not 16-byte aligned", i);
+    P.a[i] = m.a; P.b[i] = m.b; P.scale[i] = m.scale; P.x[i] = x[i]; P.y[i] = y[i]; P.out[i] = out[i]; P.n_out[i] = m.n_out;
+    P.h[i] = reinterpret_cast<float*>(static_cast<char*>(workspace) + size_t(i) * (need / nmat));
+    P.vec[i] = m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
+    chunks += (m.n_out + sh.chunk_cols - 1) / sh.chunk_cols;
+    P.chunk_end[i] = chunks;
+  }
+  P.ids = reinterpret_cast<const long long*>(ids);
+  P.nmat = nmat; P.adapters = n_adapters; P.rank = rank; P.K = k_in; P.R = streams * tokens_per_stream; P.T = tokens_per_stream;
+  P.streams = streams; P.rt = sh.rt; P.splits = sh.splits; P.chunk_cols = sh.chunk_cols;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (dtype == B200RWKV_F32) e = launch_adapt<float, float>(P, sh, s);
+  else if (dtype == B200RWKV_BF16) e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __nv_bfloat16>(P, sh, s) : launch_adapt<__nv_bfloat16, __nv_bfloat16>(P, sh, s);
+  else e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __half>(P, sh, s) : launch_adapt<__half, __half>(P, sh, s);
+  if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "adapt_rows: %s", cudaGetErrorString(e));
+  return B200RWKV_OK;
+}
+
+size_t b200rwkv_verify_drafts_workspace_bytes(int streams, int drafts, int n) {
+  if (streams < 1 || streams > 65535 || drafts < 0 || drafts > kVerifyMaxDrafts || n < 1 || n > kVerifySeg * kVerifyMaxSegs) return 0;
+  return size_t(streams) * (2 * drafts + 1) * verify_segs(n) * 8;
+}
+
+int b200rwkv_verify_drafts(const float* target, int64_t target_stream_stride, int64_t target_row_stride, const float* draft,
+                           int64_t draft_stream_stride, int64_t draft_row_stride, const int64_t* tokens, const float* u,
+                           const int64_t* lengths, int streams, int drafts, int n, int64_t* out, int64_t* accepted, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  const size_t need = b200rwkv_verify_drafts_workspace_bytes(streams, drafts, n);
+  if (!need) return fail(B200RWKV_EINVAL, "verify_drafts: streams=%d (1..65535) drafts=%d (0..%d) n=%d (1..%d)", streams, drafts, kVerifyMaxDrafts, n, kVerifySeg * kVerifyMaxSegs);
+  if (!target || (drafts > 0 && !tokens) || !u || !out || !accepted || !workspace) return fail(B200RWKV_EINVAL, "verify_drafts: null argument");
+  if (target_row_stride < 0 || target_stream_stride < 0 || (draft && (draft_row_stride < 0 || draft_stream_stride < 0)))
+    return fail(B200RWKV_EINVAL, "verify_drafts: negative stride");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 7u) != 0 || workspace_bytes < need)
+    return fail(B200RWKV_EINVAL, "verify_drafts: workspace must be 8-byte aligned and hold %zu bytes", need);
+  VerifyParams P;
+  memset(&P, 0, sizeof(P));
+  P.target = target; P.target_stream = target_stream_stride; P.target_row = target_row_stride;
+  P.draft = drafts > 0 ? draft : nullptr; P.draft_stream = draft_stream_stride; P.draft_row = draft_row_stride;
+  P.tokens = reinterpret_cast<const long long*>(tokens); P.lengths = reinterpret_cast<const long long*>(lengths); P.u = u;
+  P.sums = static_cast<double*>(workspace); P.out = reinterpret_cast<long long*>(out); P.accepted = reinterpret_cast<long long*>(accepted);
+  P.B = streams; P.K = drafts; P.V = n; P.segs = verify_segs(n);
+  cudaError_t e = launch_verify(P, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "verify_drafts: %s", cudaGetErrorString(e));
+  return B200RWKV_OK;
+}
+
+int b200rwkv_advance_state(const float* state, float* out, const int64_t* counts, const float* trace, const float* params, int streams,
+                           int layers, int tokens, int channels, void* stream) {
+  if (!state || !out || !counts || !trace || !params) return fail(B200RWKV_EINVAL, "advance_state: null argument");
+  if (streams < 1 || layers < 1 || tokens < 1 || channels < 4 || channels % 4 || (long long)streams * layers > (1 << 24) || channels > (1 << 20))
+    return fail(B200RWKV_EINVAL, "advance_state: streams=%d layers=%d tokens=%d channels=%d (channels a multiple of 4)", streams, layers, tokens, channels);
+  if (!aligned16(state) || !aligned16(out) || !aligned16(trace) || !aligned16(params))
+    return fail(B200RWKV_EINVAL, "advance_state: state, out, trace and params must be 16-byte aligned");
+  AdvanceParams P;
+  P.state = state; P.out = out; P.trace = trace; P.params = params; P.counts = reinterpret_cast<const long long*>(counts);
+  P.B = streams; P.L = layers; P.T = tokens; P.C = channels;
+  advance_state_kernel<<<dim3(streams * layers, 2 + (channels / 4 + kAdvanceThreads - 1) / kAdvanceThreads), kAdvanceThreads, 0,
+                         static_cast<cudaStream_t>(stream)>>>(P);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "advance_state: %s", cudaGetErrorString(e));
   return B200RWKV_OK;
 }
 

@@ -8,7 +8,7 @@ launch on torch's current stream.  No CPU path.
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -195,6 +195,145 @@ def gemv_dense(w: torch.Tensor, x: torch.Tensor, y: Optional[torch.Tensor] = Non
         _lib.check(_lib.lib().b200rwkv_gemv_dense(w.data_ptr(), _DENSE_DTYPES[w.dtype], k_in, n_out, w.stride(0),
                                                   x.data_ptr(), y.data_ptr(), _stream(w.device)))
     return y
+
+
+def pack_adapters(adapters: Sequence[Tuple[torch.Tensor, torch.Tensor, float]], dtype: Optional[torch.dtype] = None,
+                  device=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A bank for ``adapt_rows`` from one projection's adapters ``(a [r,in], b [out,r], scale)``, whose ranks r may differ:
+    ``(a [n,rank,in], b [n,out,rank], scale f32 [n])`` with rank the largest one, rounded up to a multiple of 4; the
+    ranks that an adapter lacks are zeros.  Laid out once, when adapters are loaded."""
+    if not adapters:
+        raise ValueError("pack_adapters needs at least one adapter")
+    a0, b0, _ = adapters[0]
+    dtype, device = dtype or a0.dtype, device or a0.device
+    for a, b, _ in adapters:
+        if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[1] != a0.shape[1] or b.shape[0] != b0.shape[0]:
+            raise ValueError("pack_adapters takes a [r,in] and b [out,r] of one projection")
+    rank = max(4, -(-max(a.shape[0] for a, _, _ in adapters) // 4) * 4)
+    pa = torch.zeros(len(adapters), rank, a0.shape[1], dtype=dtype, device=device)
+    pb = torch.zeros(len(adapters), b0.shape[0], rank, dtype=dtype, device=device)
+    for i, (a, b, _) in enumerate(adapters):
+        pa[i, :a.shape[0]] = a.to(device=device, dtype=dtype)
+        pb[i, :, :b.shape[1]] = b.to(device=device, dtype=dtype)
+    return pa, pb, torch.tensor([float(s) for _, _, s in adapters], dtype=torch.float32, device=device)
+
+
+def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]], xs: Sequence[torch.Tensor], ids: torch.Tensor,
+               ys: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+    """Low-rank adapters of many requests beside 1..3 shared projections of equal k_in (``gemm_u8``'s or
+    others'): ``outs[i][r] = ys[i][r] + scale_i[id] * (xs[i][r] @ A_i[id].T) @ B_i[id].T`` with the adapter
+    ``id = ids[r // T]`` of the row's stream, T = rows // len(ids); an id outside ``[0, n)`` (say -1) means none.
+
+    ``banks[i] = (a [n,rank,k_in], b [n,n_out_i,rank], scale f32 [n] or None)`` of bf16, fp16 or fp32 (see
+    ``pack_adapters``), ``xs[i] [rows,k_in]`` and ``ys[i] [rows,n_out_i]`` of fp32 or the banks' type, ``ids`` int64
+    ``[streams]``; all contiguous on one CUDA device.  In place on ``ys`` when ``outs`` is omitted.  ``h = x A^T`` stays
+    fp32 and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
+    adapter; rows without one are left as they are."""
+    n = len(banks)
+    outs = ys if outs is None else outs
+    if n < 1 or n > 3 or len(xs) != n or len(ys) != n or len(outs) != n:
+        raise ValueError("adapt_rows takes 1..3 banks and as many inputs and outputs")
+    a0 = banks[0][0]
+    dev, dt, row_dt = a0.device, a0.dtype, xs[0].dtype
+    if dev.type != "cuda":
+        raise RuntimeError("adapt_rows needs CUDA tensors (no CPU path)")
+    if dt not in _DENSE_DTYPES or row_dt not in (torch.float32, dt):
+        raise ValueError("adapt_rows needs banks of bf16, fp16 or fp32 and rows of fp32 or the banks' type")
+    if a0.dim() != 3 or xs[0].dim() != 2 or ids.dim() != 1:
+        raise ValueError("adapt_rows needs a [n,rank,k_in], x [rows,k_in] and ids [streams]")
+    count, rank, k_in = a0.shape
+    rows, streams = xs[0].shape[0], ids.shape[0]
+    if ids.dtype != torch.int64 or ids.device != dev or not ids.is_contiguous() or (rows % streams if streams else rows):
+        raise ValueError("ids must be contiguous int64 on the banks' device, one per stream, and the rows a multiple of them")
+    for (a, b, s), x, y, o in zip(banks, xs, ys, outs):
+        if tuple(a.shape) != (count, rank, k_in) or b.dim() != 3 or b.shape[0] != count or b.shape[2] != rank:
+            raise ValueError("adapt_rows banks must share n, rank and k_in: a [n,rank,k_in], b [n,n_out,rank]")
+        if a.dtype != dt or b.dtype != dt or not a.is_contiguous() or not b.is_contiguous() or a.device != dev or b.device != dev:
+            raise ValueError("adapt_rows banks must be contiguous, of one type, on one device")
+        if s is not None and (s.dtype != torch.float32 or s.device != dev or tuple(s.shape) != (count,) or not s.is_contiguous()):
+            raise ValueError("an adapter bank's scale must be contiguous fp32 [n] on its device")
+        for t, shape in ((x, (rows, k_in)), (y, (rows, b.shape[1])), (o, (rows, b.shape[1]))):
+            if tuple(t.shape) != shape or t.dtype != row_dt or t.device != dev or not t.is_contiguous():
+                raise ValueError("adapt_rows rows must be contiguous, of one type, on the banks' device, and match their bank")
+    if rows == 0:
+        return list(outs)
+    cb = (_lib.Adapters * n)(*[_lib.Adapters(a.data_ptr(), b.data_ptr(), _lib.ptr(s), b.shape[1]) for a, b, s in banks])
+    cx, cy, co = ((C.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (xs, ys, outs))
+    shape = (count, rank, k_in, _DENSE_DTYPES[dt])
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        nbytes = int(L.b200rwkv_adapt_rows_workspace_bytes(n, cb, *shape, streams, rows // streams))
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+        _lib.check(L.b200rwkv_adapt_rows(n, cb, *shape, cx, cy, co, _DENSE_DTYPES[row_dt], ids.data_ptr(), streams, rows // streams,
+                                         ws.data_ptr(), ws.numel(), _stream(dev)))
+    return list(outs)
+
+
+def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, u: torch.Tensor,
+                  lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Accept or replace drafted tokens so that what comes out is distributed as the target's own draws.
+
+    ``target`` fp32 ``[B,K+1,V]``: the target's weights behind each of the K drafted tokens and in front of the first
+    (``sample_typical``'s ``return_probs``: they need not sum to one; what is not above zero counts as zero).  ``draft``
+    fp32 ``[B,K,V]``: the weights that ``tokens`` int64 ``[B,K]`` were drawn from, or None where the draft is sure of
+    them.  ``u`` fp32 ``[B,K+1]`` uniform in [0,1): one number per drafted token and one for the draw.  ``lengths`` int64
+    ``[B]``: how many of the K tokens a stream has (all, when omitted).  Token t is accepted where
+    ``u_t q_t/Q_t < p_t/P_t``; the first refused one is replaced by a draw from ``max(0, p/P - q/Q)``, and where none is,
+    one more is drawn from the target's next row.  Returns int64 ``[B,K+1]`` (the accepted tokens, the drawn one, -1
+    behind it) and the number accepted, int64 ``[B]``.  Rows must be contiguous; streams and rows may be strided."""
+    if target.dim() != 3 or tokens.dim() != 2 or target.dtype != torch.float32 or target.device.type != "cuda":
+        raise ValueError("verify_drafts needs fp32 CUDA weights [B,K+1,V] and tokens [B,K]")
+    dev = target.device
+    (B, K), V = tokens.shape, target.shape[2]
+    if tuple(target.shape) != (B, K + 1, V) or (V > 1 and target.stride(2) != 1):
+        raise ValueError(f"target must be [{B},{K + 1},V] with contiguous rows, got {tuple(target.shape)}")
+    if draft is not None and (tuple(draft.shape) != (B, K, V) or draft.dtype != torch.float32 or draft.device != dev or (V > 1 and draft.stride(2) != 1)):
+        raise ValueError(f"draft must be fp32 [{B},{K},{V}] with contiguous rows on the target's device")
+    if tokens.dtype != torch.int64 or tokens.device != dev or not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous int64 on the target's device")
+    if u.dtype != torch.float32 or u.device != dev or tuple(u.shape) != (B, K + 1) or not u.is_contiguous():
+        raise ValueError(f"u must be contiguous fp32 [{B},{K + 1}] on the target's device")
+    if lengths is not None and (lengths.dtype != torch.int64 or lengths.device != dev or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
+        raise ValueError(f"lengths must be contiguous int64 [{B}] on the target's device")
+    out = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int64, device=dev)
+    if B == 0:
+        return out, accepted
+    L = _lib.lib()
+    ds = (0, 0) if draft is None else draft.stride()[:2]
+    with torch.cuda.device(dev):
+        ws = torch.empty(max(int(L.b200rwkv_verify_drafts_workspace_bytes(B, K, V)), 8), dtype=torch.uint8, device=dev)
+        _lib.check(L.b200rwkv_verify_drafts(target.data_ptr(), target.stride(0), target.stride(1), _lib.ptr(draft), ds[0], ds[1],
+                                            tokens.data_ptr(), u.data_ptr(), _lib.ptr(lengths), B, K, V, out.data_ptr(),
+                                            accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+    return out, accepted
+
+
+def advance_state(state: torch.Tensor, counts: torch.Tensor, trace: torch.Tensor, params: torch.Tensor,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The state of B streams after the first ``counts[b]`` of a step's T tokens, for a step whose later tokens were refused
+    (a recurrent state cannot drop them).  ``state`` fp32 ``[B,L,5,C]`` in front of the step, ``counts`` int64 ``[B]``
+    (clamped to 0..T; 0 leaves the state as it is), ``trace`` fp32 ``[L,4,B,T,C]``: of every block and token the residual
+    stream in front of ln1, in front of ln2, the key and the value; ``params`` fp32 ``[L,5,C]``: ln1 weight and bias, ln2
+    weight and bias, ``-exp(time_decay)``.  Carries become the layer norms of the last accepted token, the WKV sums take
+    ``counts[b]`` steps (agnosticRwkv.py:68-103).  In place when ``out`` is omitted; returns the new state."""
+    out = state if out is None else out
+    if state.dim() != 4 or state.shape[2] != 5 or trace.dim() != 5:
+        raise ValueError("advance_state needs state [B,L,5,C] and trace [L,4,B,T,C]")
+    B, L, _, Cc = state.shape
+    T = trace.shape[3]
+    shapes = ((state, (B, L, 5, Cc)), (out, (B, L, 5, Cc)), (trace, (L, 4, B, T, Cc)), (params, (L, 5, Cc)))
+    for t, shape in shapes:
+        if t.dtype != torch.float32 or t.device != state.device or t.device.type != "cuda" or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError("advance_state needs contiguous fp32 CUDA tensors: state and out [B,L,5,C], trace [L,4,B,T,C], params [L,5,C]")
+    if counts.dtype != torch.int64 or counts.device != state.device or tuple(counts.shape) != (B,) or not counts.is_contiguous():
+        raise ValueError(f"counts must be contiguous int64 [{B}] on the state's device")
+    if B == 0 or T == 0:
+        return out if out.data_ptr() == state.data_ptr() else out.copy_(state)
+    with torch.cuda.device(state.device):
+        _lib.check(_lib.lib().b200rwkv_advance_state(state.data_ptr(), out.data_ptr(), counts.data_ptr(), trace.data_ptr(), params.data_ptr(),
+                                                     B, L, T, Cc, _stream(state.device)))
+    return out
 
 
 def matvec(W: torch.Tensor, x: torch.Tensor) -> torch.Tensor:

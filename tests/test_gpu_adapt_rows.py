@@ -1,0 +1,223 @@
+"""Low-rank adapters beside shared projections (``ops.adapt_rows``) against the formula in 64 bits.
+
+The bound of every element follows from the arithmetic: h = x A^T is a sum of K exact products (pieces of 8 bits) in fp32, in
+at most 3 K / 16 + 32 additions that may each lose a unit in the last place (2^-23 of the running sum, which the sum of
+magnitudes bounds); what the pieces leave out is below 2^-21 of a product; the second product the same with the rank in K's
+place; y + delta is rounded once (fp32 2^-24, bf16 2^-8, fp16 2^-11 of the value; subnormal halves half of 2^-24).  For 16-bit rows h goes in with 16 of
+its bits (2^-15), and with fp16 weights products of two second pieces are left out (2^-14)."""
+import pytest
+import torch
+
+from rwkvstic_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def make(streams, T, k, outs, rank, adapters, w, t, seed=0, none=0.2):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s, std=1.0: torch.randn(*s, generator=g) * std
+    banks = [(rnd(adapters, rank, k, std=k ** -0.5).to(w).to(DEV), rnd(adapters, o, rank, std=rank ** -0.5).to(w).to(DEV),
+              (torch.rand(adapters, generator=g) + 0.5).to(DEV)) for o in outs]
+    ids = torch.randint(0, adapters, (streams,), generator=g)
+    ids[torch.rand(streams, generator=g) < none] = -1
+    xs = [rnd(streams * T, k).to(t).to(DEV) for _ in outs]
+    ys = [rnd(streams * T, o).to(t).to(DEV) for o in outs]
+    return banks, xs, ids.to(DEV), ys
+
+
+def reference(bank, x, ids, y):
+    """(result, bound) in fp64."""
+    a, b, scale = bank
+    n, T = a.shape[0], x.shape[0] // ids.shape[0]
+    want, bound = y.double().clone(), torch.zeros_like(y, dtype=torch.float64)
+    k, rank = a.shape[2], a.shape[1]
+    half = y.dtype != torch.float32
+    c1 = (3 * k / 16 + 32) * 2.0 ** -23 + 2.0 ** -21
+    c2 = (3 * rank / 16 + 8) * 2.0 ** -23 + (2.0 ** -15 + (2.0 ** -14 if a.dtype == torch.float16 else 0.0) if half else 2.0 ** -21)
+    for i, j in enumerate(ids.tolist()):
+        if not 0 <= j < n:
+            continue
+        at = slice(i * T, (i + 1) * T)
+        s = 1.0 if scale is None else float(scale[j])
+        h = x[at].double() @ a[j].double().T
+        hm = x[at].double().abs() @ a[j].double().abs().T
+        want[at] += s * (h @ b[j].double().T)
+        bound[at] = s * ((c1 * hm + c2 * h.abs()) @ b[j].double().abs().T)
+    eps = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[y.dtype]
+    return want, bound * (1 + eps) + eps * want.abs() + (2.0 ** -25 if y.dtype == torch.float16 else 1e-38)
+
+
+def check(banks, xs, ids, ys, outs=None, untouched=True):
+    wants = [reference(b, x, ids, y) for b, x, y in zip(banks, xs, ys)]
+    before = [y.clone() for y in ys]
+    got = ops.adapt_rows(banks, xs, ids, ys, outs)
+    torch.cuda.synchronize()
+    n, T = banks[0][0].shape[0], xs[0].shape[0] // ids.shape[0]
+    none = ~((ids >= 0) & (ids < n)).repeat_interleave(T)
+    for y0, y, o, g, (want, bound) in zip(before, ys, outs or ys, got, wants):
+        assert g is o
+        assert torch.equal(g[none], y0[none])
+        err = ((g.double() - want).abs() - bound)[~none]           # rows without an adapter may hold infinities; they were compared above
+        assert err.numel() == 0 or float(err.max()) <= 0.0, float(err.max())
+        if outs is not None and untouched:
+            assert torch.equal(y, y0)
+
+
+COMBOS = [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f16", "f16")]
+SHAPES = [
+    (1, 1, 128, [64, 64, 128], 4, 1),        # one row, three projections
+    (1, 1, 2048, [2048], 16, 3),             # K cut over CTAs
+    (7, 1, 768, [770, 3], 8, 2),             # few rows of shared adapters, odd outputs
+    (40, 1, 264, [130], 20, 1),              # one adapter for more rows than a tile
+    (150, 1, 136, [64], 12, 40),
+    (1100, 1, 64, [36], 8, 3),               # more streams than a window
+    (48, 5, 256, [1029], 8, 20),             # tiles that begin and end inside a stream
+    (33, 31, 72, [65, 1], 4, 2),
+    (3, 33, 128, [100], 36, 2),
+    (1, 63, 512, [256], 64, 1),
+    (2, 64, 128, [132], 100, 2),             # tiles of one stream
+    (3, 65, 200, [67], 128, 3),
+    (2, 333, 1024, [260, 64], 64, 5),
+    (2, 70, 8, [5], 256, 2),                 # the shortest K, the largest rank
+    (9, 2, 520, [1], 200, 4),
+]
+
+
+@pytest.mark.parametrize("w,t", COMBOS)
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}_k{s[2]}_r{s[4]}" for s in SHAPES])
+def test_against_formula(shape, w, t):
+    banks, xs, ids, ys = make(*shape, TYPES[w], TYPES[t], seed=len(str(shape)))
+    check(banks, xs, ids, ys, [torch.full_like(y, 7.0) for y in ys])
+    check(banks, xs, ids, ys)
+
+
+@pytest.mark.parametrize("w,t", COMBOS)
+def test_rows_without_adapter_are_not_read(w, t):
+    """Their x may hold anything, and ids outside the bank mean none."""
+    banks, xs, ids, ys = make(12, 3, 64, [40], 8, 3, TYPES[w], TYPES[t], none=0.0)
+    ids[2], ids[5], ids[7], ids[11] = -1, 3, -(2 ** 40), 2 ** 40
+    for i in (2, 5, 7, 11):
+        xs[0][3 * i:3 * i + 3] = float("nan")
+        ys[0][3 * i] = float("inf")
+    outs = [torch.zeros_like(ys[0])]
+    check(banks, xs, ids, ys, outs)
+    ids.fill_(-1)
+    check(banks, xs, ids, ys, outs)
+    check(banks, xs, ids, ys)
+
+
+def test_no_scale_means_one_and_infinite_inputs_give_nan():
+    banks, xs, ids, ys = make(3, 1, 128, [64], 8, 2, torch.bfloat16, torch.float32, none=0.0)
+    banks = [(a, b, None) for a, b, _ in banks]
+    check(banks, xs, ids, ys, [torch.empty_like(ys[0])])
+    xs[0][1, 17] = float("inf")
+    out = ops.adapt_rows(banks, xs, ids, ys, [torch.empty_like(ys[0])])[0]
+    assert torch.isnan(out[1]).all() and not torch.isnan(out[[0, 2]]).any()
+
+
+def test_unaligned_rows_of_y():
+    """y and out may start anywhere: four elements at a time only where both allow it."""
+    banks, xs, ids, ys = make(5, 2, 64, [68], 8, 2, torch.bfloat16, torch.float32)
+    flat = torch.zeros(10 * 68 + 3, device=DEV)
+    flat[3:] = ys[0].reshape(-1)
+    y = flat[3:].reshape(10, 68)
+    check(banks, xs, ids, [y], [torch.empty_like(ys[0])])
+    check(banks, xs, ids, [y])
+    assert float(flat[:3].abs().sum()) == 0.0
+
+
+def test_extreme_values():
+    """Large and small activations keep their relative accuracy (pieces share the float's exponent range)."""
+    for scale in (1e30, 1e-30):
+        banks, xs, ids, ys = make(4, 3, 256, [64], 16, 2, torch.bfloat16, torch.float32)
+        xs = [x * scale for x in xs]
+        ys = [y * scale for y in ys]
+        check(banks, xs, ids, ys, [torch.empty_like(ys[0])])
+
+
+def test_repeats_its_bits_and_rows_do_not_depend_on_their_tile():
+    banks, xs, ids, ys = make(64, 1, 512, [300], 16, 4, torch.bfloat16, torch.float32)
+    outs = [torch.empty_like(ys[0])]
+    first = ops.adapt_rows(banks, xs, ids, ys, outs)[0].clone()
+    for _ in range(3):
+        assert torch.equal(ops.adapt_rows(banks, xs, ids, ys, outs)[0], first)
+    turn = torch.randperm(64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    moved = ops.adapt_rows(banks, [xs[0][turn].contiguous()], ids[turn].contiguous(), [ys[0][turn].contiguous()], outs)[0]
+    assert torch.equal(moved, first[turn])
+
+
+def test_captured_call_follows_its_ids():
+    banks, xs, ids, ys = make(6, 2, 128, [64, 33], 8, 3, torch.bfloat16, torch.bfloat16)
+    outs = [torch.empty_like(y) for y in ys]
+    ops.adapt_rows(banks, xs, ids, ys, outs)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            ops.adapt_rows(banks, xs, ids, ys, outs)
+    for seed in range(3):
+        ids.copy_(torch.randint(-1, 3, (6,), generator=torch.Generator().manual_seed(seed)))
+        want = [o.clone() for o in ops.adapt_rows(banks, xs, ids, ys, [torch.empty_like(y) for y in ys])]
+        for g in graphs:
+            for o in outs:
+                o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_two_streams_at_once():
+    cases = [make(32, 1, 1024, [512], 16, 8, torch.bfloat16, torch.float32, seed=s) for s in range(2)]
+    want = [ops.adapt_rows(b, x, i, y, [torch.empty_like(y[0])])[0] for b, x, i, y in cases]
+    outs = [[torch.empty_like(c[3][0])] for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        for (b, x, i, y), o, s in zip(cases, outs, streams):
+            with torch.cuda.stream(s):
+                ops.adapt_rows(b, x, i, y, o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o[0], w) for o, w in zip(outs, want))
+
+
+def test_pack_adapters_of_different_ranks():
+    g = torch.Generator().manual_seed(5)
+    parts = [(torch.randn(r, 64, generator=g) / 8, torch.randn(40, r, generator=g) / 2, 0.25 * (r + 1)) for r in (3, 8, 1)]
+    bank = ops.pack_adapters(parts, torch.bfloat16, DEV)
+    assert tuple(bank[0].shape) == (3, 8, 64) and tuple(bank[1].shape) == (3, 40, 8)
+    x, y = torch.randn(6, 64, generator=g).to(DEV), torch.randn(6, 40, generator=g).to(DEV)
+    ids = torch.tensor([2, 0, 1], device=DEV)
+    check([bank], [x], ids, [y], [torch.empty_like(y)])
+    for i, j in enumerate(ids.tolist()):
+        a, b, s = parts[j]
+        want = y[2 * i:2 * i + 2].double().cpu() + s * x[2 * i:2 * i + 2].cpu().double() @ a.bfloat16().double().T @ b.bfloat16().double().T
+        got = ops.adapt_rows([bank], [x], ids, [y], [torch.empty_like(y)])[0][2 * i:2 * i + 2].double().cpu()
+        assert float((got - want).abs().max()) < 1e-5       # (3 64 / 16 + 32) 2^-23 of sums of magnitude below 2
+
+
+def test_refusals():
+    banks, xs, ids, ys = make(4, 2, 64, [32], 8, 2, torch.bfloat16, torch.float32)
+    a, b, s = banks[0]
+    bad = [
+        dict(banks=[]), dict(xs=[]), dict(banks=banks * 4, xs=xs * 4, ys=ys * 4),
+        dict(banks=[(a.double(), b.double(), s)]), dict(xs=[xs[0].half()]), dict(ys=[ys[0].bfloat16()]),
+        dict(ids=ids.int()), dict(ids=ids[:3]), dict(ids=ids.cpu()), dict(ids=ids.repeat(2)[::2]),
+        dict(banks=[(a, b[:, :, :4].contiguous(), s)]), dict(banks=[(a[:1], b, s)]), dict(banks=[(a, b, s.double())]), dict(banks=[(a, b, s[:1])]),
+        dict(xs=[xs[0][:, :56].contiguous()]), dict(ys=[ys[0][:, :31].contiguous()]), dict(outs=[ys[0][:4]]),
+        dict(xs=[xs[0].t().contiguous().t()]), dict(banks=[(a.transpose(1, 2).contiguous().transpose(1, 2), b, s)]),
+    ]
+    for change in bad:
+        args = {**dict(banks=banks, xs=xs, ids=ids, ys=ys, outs=None), **change}
+        with pytest.raises(ValueError):
+            ops.adapt_rows(args["banks"], args["xs"], args["ids"], args["ys"], args["outs"])
+    with pytest.raises(RuntimeError):
+        ops.adapt_rows([(a.cpu(), b.cpu(), s.cpu())], [xs[0].cpu()], ids.cpu(), [ys[0].cpu()])
+    for rank, k in ((6, 64), (260, 64), (8, 60)):
+        with pytest.raises(_lib.B200RWKVError):
+            ops.adapt_rows([(torch.zeros(2, rank, k, device=DEV), torch.zeros(2, 32, rank, device=DEV), None)], [torch.zeros(8, k, device=DEV)],
+                           ids, [torch.zeros(8, 32, device=DEV)])
+    empty = torch.zeros(0, 64, device=DEV)
+    assert ops.adapt_rows(banks, [empty], ids, [torch.zeros(0, 32, device=DEV)])[0].shape == (0, 32)
+    assert ops.adapt_rows(banks, [empty], ids[:0], [torch.zeros(0, 32, device=DEV)])[0].shape == (0, 32)
