@@ -9,8 +9,8 @@
 //
 // Products run on the tensor cores (mma.sync m16n8k16) with fp32 sums.  Operands that are not of one 16-bit type are cut
 // into bfloat16 pieces: a float is exactly three (the upper 8 bits of its significand, the next 8, the last 8), a half
-// exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21 of the whole together and left out, and those of
-// the small pieces are summed apart from the large ones.  A piece of an infinity is NaN: a row of x that holds an infinity
+// exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21 of the whole together and left out.  The tensor cores
+// cut their sums off, so no chain is longer than 64 k before its part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity
 // or a NaN comes out as NaN, where it has an adapter.
 // What bounds both is memory: h takes rank multiplications per value of x, y takes rank per value.  At rank 64 with fp32 rows
 // that is 48 products of pieces a byte, below what mma.sync sustains beside the loads, so nothing is gained by staging
@@ -32,7 +32,7 @@ constexpr int kAdaptWindow = 1024;         // streams
 constexpr int kAdaptMaxRank = 256;
 constexpr int kAdaptMaxRows = 64;          // of a tile
 constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
-constexpr int kExpandThreads = 128, kExpandWarps = kExpandThreads / 32, kExpandCols = 32;   // columns of a warp at a time
+constexpr int kExpandThreads = 128, kExpandWarps = kExpandThreads / 32;
 
 struct AdaptParams {
   const void *a[kAdaptMaxMats], *b[kAdaptMaxMats], *x[kAdaptMaxMats], *y[kAdaptMaxMats];
@@ -41,7 +41,6 @@ struct AdaptParams {
   float* h[kAdaptMaxMats];                 // [splits][rows][rank]
   int n_out[kAdaptMaxMats];
   int chunk_end[kAdaptMaxMats];            // second launch: column chunks of the matrices up to and including this one
-  int vec[kAdaptMaxMats];                  // rows of y and out start on boundaries of four elements
   const long long* ids;
   int nmat, adapters, rank, K, R, T, streams, rt, splits, chunk_cols;
 };
@@ -128,13 +127,14 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
   }
   const int w0 = tile / kAdaptWindow * kAdaptWindow, count = min(kAdaptWindow, P.streams - w0);
   const int mine = id_of(tile);
-  for (int i = tid; i < kAdaptWindow; i += nt) {
+  const int words = (count + 31) / 32;
+  for (int i = tid; i < 32 * words; i += nt) {
     const unsigned m = __ballot_sync(0xffffffffu, i < count && id_of(w0 + i) == mine);
     if ((i & 31) == 0) mask[i >> 5] = m;
   }
   __syncthreads();
   int before = 0, all = 0;                               // streams of this adapter in front of this one, and in the window
-  for (int w = 0; w < kAdaptWindow / 32; ++w) {
+  for (int w = 0; w < words; ++w) {
     const uint32_t m = mask[w];
     const int at = tile - w0 - 32 * w;                   // bits of this word in front of the stream's own
     before += __popc(at >= 32 ? m : at > 0 ? m & ((1u << at) - 1u) : 0u);
@@ -188,52 +188,71 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
       aok[m][e] = j < rank;
       ap[m][e] = a + size_t(aok[m][e] ? j : 0) * K + 8 * t;
     }
-  float big[MT][NT][4], small[MT][NT][4];
+  float sum[MT][NT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int q = 0; q < NT; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) big[m][q][i] = small[m][q][i] = 0.f;
+      for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
   const int blocks = (K + 31) / 32, b0 = int((long long)blocks * split / P.splits), b1 = int((long long)blocks * (split + 1) / P.splits);
-#pragma unroll 2
-  for (int kb = b0 + my_k; kb < b1; kb += kw) {
-    const int k = kb * 32;
-    const bool in = k + 8 * t < K;                       // K is a multiple of 8
-    AdaptRaw<TX, 8> rx[NT];
-    AdaptRaw<TW, 8> ra[MT][2];
+  for (int kb = b0 + my_k; kb < b1; kb += 2 * kw) {
+    // two blocks of 32 k: all loads first
+    AdaptRaw<TX, 8> rx[2][NT];
+    AdaptRaw<TW, 8> ra[2][MT][2];
 #pragma unroll
-    for (int q = 0; q < NT; ++q) rx[q].load(xp[q] + k, in && xok[q]);
+    for (int o = 0; o < 2; ++o) {
+      const int k = (kb + o * kw) * 32;
+      const bool in = kb + o * kw < b1 && k + 8 * t < K;  // K is a multiple of 8
+#pragma unroll
+      for (int q = 0; q < NT; ++q) rx[o][q].load(xp[q] + k, in && xok[q]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) ra[o][m][e].load(ap[m][e] + k, in && aok[m][e]);
+    }
+    float part[MT][NT][4];                               // the tensor cores cut their sums off; the running sum rounds
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) ra[m][e].load(ap[m][e] + k, in && aok[m][e]);
+      for (int q = 0; q < NT; ++q)
 #pragma unroll
-    for (int step = 0; step < 2; ++step) {               // elements 4 step .. 4 step + 3 of every lane
-      uint32_t fx[NT][2][PX];
+        for (int i = 0; i < 4; ++i) part[m][q][i] = 0.f;
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {             // elements 4 step .. 4 step + 3 of every lane
+        uint32_t fx[NT][2][PX];
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) rx[o][q].template pair<PX>(2 * step + i, fx[q][i]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t fa[4][PW];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ra[o][m][i & 1].template pair<PW>(2 * step + (i >> 1), fa[i]);
+#pragma unroll
+          for (int i = PW - 1; i >= 0; --i) {
+            const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
+#pragma unroll
+            for (int j = PX - 1; j >= 0; --j) {
+              if (i + j >= 3) continue;
+#pragma unroll
+              for (int q = 0; q < NT; ++q) {
+                if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
+                else mma_bf16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int q = 0; q < NT; ++q)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) rx[q].template pair<PX>(2 * step + i, fx[q][i]);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        uint32_t fa[4][PW];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ra[m][i & 1].template pair<PW>(2 * step + (i >> 1), fa[i]);
-#pragma unroll
-        for (int i = 0; i < PW; ++i) {
-          const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
-#pragma unroll
-          for (int q = 0; q < NT; ++q)
-#pragma unroll
-            for (int j = 0; j < PX; ++j) {
-              if (i + j >= 3) continue;
-              if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(big[m][q], f, fx[q][0][j], fx[q][1][j]);
-              else mma_bf16(i + j ? small[m][q] : big[m][q], f, fx[q][0][j], fx[q][1][j]);
-            }
-        }
-      }
-    }
+        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
   }
   // products' rows are ranks (g, g + 8), their columns rows of x (2t, 2t + 1)
   float* mine = red + warp * (16 * kStride);
@@ -242,7 +261,7 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 #pragma unroll
     for (int q = 0; q < NT; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[(q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = big[m][q][i] + small[m][q][i];
+      for (int i = 0; i < 4; ++i) mine[(q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = sum[m][q][i];
   __syncthreads();
   float* h = P.h[mat] + size_t(split) * P.R * rank;
   for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
@@ -275,10 +294,10 @@ __global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const Adap
 __host__ __device__ constexpr int expand_stride(int rank) { return ((rank + 15) / 16 | 1) * 16; }
 
 template <typename TY>
-__device__ __forceinline__ float adapt_load(const TY* p) {
-  if constexpr (std::is_same<TY, float>::value) return *p;
-  else if constexpr (std::is_same<TY, __half>::value) return __half2float(*p);
-  else return __bfloat162float(*p);
+__device__ __forceinline__ float adapt_float(TY v) {
+  if constexpr (std::is_same<TY, float>::value) return v;
+  else if constexpr (std::is_same<TY, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
 }
 template <typename TY>
 __device__ __forceinline__ void adapt_store(TY* p, float v) {
@@ -287,48 +306,61 @@ __device__ __forceinline__ void adapt_store(TY* p, float v) {
   else *p = __float2bfloat16_rn(v);
 }
 
-// Four consecutive elements as floats and back, through one access.
+// Four consecutive elements of a row, held as loaded.
 template <typename TY>
-__device__ __forceinline__ float4 adapt_load4(const TY* p) {
-  if constexpr (std::is_same<TY, float>::value) {
-    return *reinterpret_cast<const float4*>(p);
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    float2 a, b;
-    if constexpr (std::is_same<TY, __half>::value) {
-      a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)); b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+struct AdaptFour {
+  uint32_t w[sizeof(TY)];
+  __device__ __forceinline__ void load(const TY* p) {
+    if constexpr (sizeof(TY) == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     } else {
-      a = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
-      b = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
     }
-    return make_float4(a.x, a.y, b.x, b.y);
   }
-}
-template <typename TY>
-__device__ __forceinline__ void adapt_store4(TY* p, float4 f) {
-  if constexpr (std::is_same<TY, float>::value) {
-    *reinterpret_cast<float4*>(p) = f;
-  } else {
-    uint2 v;
-    if constexpr (std::is_same<TY, __half>::value) {
-      *reinterpret_cast<__half2*>(&v.x) = __floats2half2_rn(f.x, f.y); *reinterpret_cast<__half2*>(&v.y) = __floats2half2_rn(f.z, f.w);
+  // + f, rounded once
+  __device__ __forceinline__ void add_store(TY* p, const float (&f)[4]) const {
+    if constexpr (std::is_same<TY, float>::value) {
+      *reinterpret_cast<float4*>(p) = make_float4(__uint_as_float(w[0]) + f[0], __uint_as_float(w[1]) + f[1], __uint_as_float(w[2]) + f[2],
+                                                  __uint_as_float(w[3]) + f[3]);
     } else {
-      *reinterpret_cast<__nv_bfloat162*>(&v.x) = __floats2bfloat162_rn(f.x, f.y);
-      *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(f.z, f.w);
+      uint32_t o[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (std::is_same<TY, __half>::value) {
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          const __half2 r = __floats2half2_rn(a.x + f[2 * i], a.y + f[2 * i + 1]);
+          o[i] = *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+          const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) + f[2 * i], __uint_as_float(w[i] & 0xffff0000u) + f[2 * i + 1]);
+          o[i] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+      }
+      *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
     }
-    *reinterpret_cast<uint2*>(p) = v;
   }
-}
+};
+
+// Products of 8 columns that a warp forms at a time: more where a column has few bytes, so that its loads are as many.
+__host__ __device__ constexpr int expand_nb(int ks, int mr, int w_pieces) { return mr == 1 && ks < 4 && w_pieces == 1 ? 8 : 4; }
 
 // out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles, column chunks of all matrices).
-// A warp takes 32 columns and 32 rows at a time; the columns of two products are dealt out so that a lane ends up with four
-// consecutive ones.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16 bits, enough for a 16-bit y.
-template <typename TY, typename TW>
-__global__ void __launch_bounds__(kExpandThreads) adapt_expand_kernel(const AdaptParams P) {
-  extern __shared__ __align__(16) unsigned short hs[];     // [pieces][rt][stride]
-  __shared__ int rows[kAdaptMaxRows];
-  __shared__ uint32_t mask[kAdaptWindow / 32];
+// A warp takes 8 * NB columns and 16 * MB rows at a time; the columns of two products are dealt out so that a lane ends up with
+// four consecutive ones.  Its fragments of B for the next columns are requested in front of the stores of the present ones,
+// its y in front of the products.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16 bits, enough
+// for a 16-bit y.  Rows that do not start on boundaries of four elements (an odd number of columns) are turned in shared memory,
+// so that a warp's access is one line of a row instead of quarters of eight.
+// KS: steps of 16 ranks whose fragments are held (ranks beyond are fetched step by step); MR: tiles of 16 * MR rows; VEC: all
+// rows of y and out start on boundaries of four elements.
+template <typename TY, typename TW, int KS, int MR, bool VEC>
+__global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_kernel(const AdaptParams P) {
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  constexpr int NB = expand_nb(KS, MR, PW), MB = MR == 1 ? 1 : 2, COLS = 8 * NB;
+  extern __shared__ __align__(16) unsigned short hs[];     // [pieces][16 MR][stride]
+  __shared__ float turn[VEC ? 1 : kExpandWarps][VEC ? 1 : 16 * MB][COLS + 1];
+  __shared__ int rows[16 * MR];
+  __shared__ uint32_t mask[kAdaptWindow / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   int id = -1;
   const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
@@ -348,14 +380,32 @@ __global__ void __launch_bounds__(kExpandThreads) adapt_expand_kernel(const Adap
     return;
   }
   const int rank = P.rank, ksteps = (rank + 15) / 16, stride = expand_stride(rank), padded = (count + 15) / 16 * 16;
+  const bool held = ksteps <= KS;
+  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  AdaptRaw<TW, 4> raw[NB][KS];
+  auto fetch = [&](int c0, int k0) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int c = c0 + (n >> 1) * 16 + 4 * (g >> 1) + 2 * (n & 1) + (g & 1);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int j = (k0 + s) * 16 + 4 * t;
+        const bool ok = c < c_end && j < rank;             // rank is a multiple of four
+        raw[n][s].load(b + (ok ? size_t(c) * rank + j : 0), ok);
+      }
+    }
+  };
+  int c0 = c_begin + warp * COLS;
+  if (held) fetch(c0, 0);                                  // weights: no part of what the first launch writes
+  const int plane = 16 * MR * stride;
   griddep_wait();
   {
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
-    const int r4 = ksteps * 4, plane = P.rt * stride;      // groups of four ranks
+    const int r4 = ksteps * 4;                             // groups of four ranks
     for (int i = tid; i < padded * r4; i += kExpandThreads) {
       const int r = i / r4, j = (i - r * r4) * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < count && j < rank) {                         // rank is a multiple of four
+      if (r < count && j < rank) {
         const float* h = P.h[mat] + size_t(rows[r]) * rank + j;
         for (int p = 0; p < P.splits; ++p) {
           const float4 v = __ldcg(reinterpret_cast<const float4*>(h + size_t(p) * P.R * rank));
@@ -370,77 +420,108 @@ __global__ void __launch_bounds__(kExpandThreads) adapt_expand_kernel(const Adap
     }
   }
   __syncthreads();
-  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
-  const int plane = P.rt * stride;
-  for (int c0 = c_begin + warp * kExpandCols; c0 < c_end; c0 += kExpandWarps * kExpandCols) {
-    for (int m0 = 0; m0 < count; m0 += 32) {
-      float acc[2][4][4];
+  for (; c0 < c_end; c0 += kExpandWarps * COLS) {
+    for (int m0 = 0; m0 < count; m0 += 16 * MB) {
+      AdaptFour<TY> four[MB][2][NB / 2];                   // y: rows m0 + 16 m + 8 e + g, columns c0 + 16 q + 4 t ..
+      TY line[16 * MB][COLS / 32];                         // or rows m0 + i, columns c0 + 32 q + lane
+      if constexpr (VEC) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+          for (int e = 0; e < 2; ++e) {
+            const int i = m0 + m * 16 + e * 8 + g;
+            const TY* p = y + size_t(i < count ? rows[i] : 0) * N + c0 + 4 * t;
+#pragma unroll
+            for (int q = 0; q < NB / 2; ++q)
+              if (i < count && c0 + q * 16 + 4 * t < c_end) four[m][e][q].load(p + q * 16);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16 * MB; ++i)
+          if (m0 + i < count) {
+            const TY* p = y + size_t(rows[m0 + i]) * N + c0 + lane;
+#pragma unroll
+            for (int q = 0; q < COLS / 32; ++q)
+              if (c0 + q * 32 + lane < c_end) line[i][q] = p[q * 32];
+          }
+      }
+      float acc[MB][NB][4];
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-      const bool second = m0 + 16 < count;
-#pragma unroll 1
-      for (int ks = 0; ks < ksteps; ++ks) {
-        uint32_t fb[4][2][PW];
+      for (int k0 = 0; k0 < ksteps; k0 += KS) {
+        if (!held) fetch(c0, k0);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int c = c0 + (n >> 1) * 16 + 4 * (g >> 1) + 2 * (n & 1) + (g & 1), j = ks * 16 + 4 * t;
-          AdaptRaw<TW, 4> raw;
-          const bool ok = c < c_end && j < rank;
-          raw.load(b + (ok ? size_t(c) * rank + j : 0), ok);
-          raw.template pair<PW>(0, fb[n][0]);
-          raw.template pair<PW>(1, fb[n][1]);
-        }
+        for (int s = 0; s < KS; ++s) {
+          if (k0 + s >= ksteps) break;
+          uint32_t fb[NB][2][PW];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (m && !second) break;
+          for (int n = 0; n < NB; ++n) {
+            raw[n][s].template pair<PW>(0, fb[n][0]);
+            raw[n][s].template pair<PW>(1, fb[n][1]);
+          }
 #pragma unroll
-          for (int p = 0; p < PH; ++p) {
-            const unsigned short* at = hs + size_t(p) * plane + (m0 + m * 16 + g) * stride + ks * 16 + 4 * t;
-            const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8 * stride);
-            const uint32_t f[4] = {u.x, v.x, u.y, v.y};
+          for (int m = 0; m < MB; ++m) {
+            if (m && m0 + 16 * m >= count) break;
 #pragma unroll
-            for (int w = 0; w < PW; ++w) {
-              if (p + w >= PH) continue;
+            for (int p = PH - 1; p >= 0; --p) {
+              const unsigned short* at = hs + size_t(p) * plane + (m0 + m * 16 + g) * stride + (k0 + s) * 16 + 4 * t;
+              const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8 * stride);
+              const uint32_t f[4] = {u.x, v.x, u.y, v.y};
 #pragma unroll
-              for (int n = 0; n < 4; ++n) mma_bf16(acc[m][n], f, fb[n][0][w], fb[n][1][w]);
+              for (int w = PW - 1; w >= 0; --w) {
+                if (p + w >= PH) continue;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mma_bf16(acc[m][n], f, fb[n][0][w], fb[n][1][w]);
+              }
             }
           }
         }
       }
+      const int next = c0 + kExpandWarps * COLS;
+      if (held && m0 + 16 * MB >= count && next < c_end) fetch(next, 0);
+      if constexpr (VEC) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = m0 + m * 16 + e * 8 + g;
-          if (i >= count) continue;
-          const size_t row = size_t(rows[i]) * N;
+          for (int e = 0; e < 2; ++e) {
+            const int i = m0 + m * 16 + e * 8 + g;
+            if (i >= count) continue;
+            TY* p = out + size_t(rows[i]) * N + c0 + 4 * t;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int c = c0 + q * 16 + 4 * t;
-            const float4 d = make_float4(acc[m][2 * q][2 * e], acc[m][2 * q][2 * e + 1], acc[m][2 * q + 1][2 * e], acc[m][2 * q + 1][2 * e + 1]);
-            if (P.vec[mat]) {
-              if (c < c_end) {
-                const float4 v = adapt_load4(y + row + c);
-                adapt_store4(out + row + c, make_float4(v.x + d.x, v.y + d.y, v.z + d.z, v.w + d.w));
-              }
-            } else {
-              const float f[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (c + k < c_end) adapt_store(out + row + c + k, adapt_load(y + row + c + k) + f[k]);
+            for (int q = 0; q < NB / 2; ++q) {
+              const float d[4] = {acc[m][2 * q][2 * e], acc[m][2 * q][2 * e + 1], acc[m][2 * q + 1][2 * e], acc[m][2 * q + 1][2 * e + 1]};
+              if (c0 + q * 16 + 4 * t < c_end) four[m][e][q].add_store(p + q * 16, d);
             }
           }
-        }
+      } else {
+        __syncwarp();
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              turn[warp][m * 16 + (i >> 1) * 8 + g][(n >> 1) * 16 + 4 * t + 2 * (n & 1) + (i & 1)] = acc[m][n][i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16 * MB; ++i)
+          if (m0 + i < count) {
+            TY* p = out + size_t(rows[m0 + i]) * N + c0 + lane;
+#pragma unroll
+            for (int q = 0; q < COLS / 32; ++q)
+              if (c0 + q * 32 + lane < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[warp][i][q * 32 + lane]);
+          }
+      }
     }
   }
 }
 
 struct AdaptShape {
-  int rt, tiles, splits, mt, chunk_cols, chunks;   // mt: ranks of a CTA of the first launch, in 16
+  int rt, tiles, splits, mt, ks, chunk_cols, chunks;   // mt: ranks of a CTA of the first launch, ks: of fragments held in the second, in 16
 };
 
 // Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
@@ -455,11 +536,12 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   long long busy = s.tiles;                              // tiles that lead rows
   if (gathered && adapters + rows / s.rt + 1 < busy) busy = adapters + rows / s.rt + 1;
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
+  s.ks = rank <= 16 ? 1 : rank <= 32 || w_pieces > 2 ? 2 : 4;
   const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
   long long splits = 2LL * sms / ctas;
   if (splits > K / 256) splits = K / 256;
   s.splits = int(splits < 1 ? 1 : splits > 16 ? 16 : splits);
-  const int unit = kExpandWarps * kExpandCols;
+  const int unit = kExpandWarps * 8 * expand_nb(s.ks, s.rt / 16, w_pieces);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
   long long per = units * busy / (8LL * sms);            // column units a CTA takes for eight CTAs per SM

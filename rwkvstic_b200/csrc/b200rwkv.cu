@@ -742,8 +742,8 @@ static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& s
   return cudaErrorInvalidValue;
 }
 
-template <typename TY, typename TW>
-static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+template <typename TY, typename TW, int KS, int MR, bool VEC>
+static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
   constexpr int pieces = sizeof(TY) == 2 ? 2 : 3;
   static bool configured[64];
   int dev = 0;
@@ -751,20 +751,35 @@ static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& s
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             pieces * kAdaptMaxRows * expand_stride(kAdaptMaxRank) * 2);
+    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KS, MR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             pieces * 16 * MR * expand_stride(kAdaptMaxRank) * 2);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_chained(adapt_expand_kernel<TY, TW>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
-                        size_t(pieces) * P.rt * expand_stride(P.rank) * 2, stream, P);
+  return launch_chained(adapt_expand_kernel<TY, TW, KS, MR, VEC>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
+                        size_t(pieces) * 16 * MR * expand_stride(P.rank) * 2, stream, P);
+}
+
+template <typename TY, typename TW, int KS>
+static cudaError_t launch_adapt_expand_ks(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+  constexpr int many = kAdaptMaxRows / 16;
+  if (sh.rt == 16) return vec ? launch_adapt_expand_as<TY, TW, KS, 1, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, 1, false>(P, sh, stream);
+  return vec ? launch_adapt_expand_as<TY, TW, KS, many, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, many, false>(P, sh, stream);
 }
 
 template <typename TY, typename TW>
-static cudaError_t launch_adapt(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+  if (sh.ks == 1) return launch_adapt_expand_ks<TY, TW, 1>(P, sh, vec, stream);
+  if (sh.ks == 2) return launch_adapt_expand_ks<TY, TW, 2>(P, sh, vec, stream);
+  if constexpr (AdaptType<TW>::kPieces < 3) return launch_adapt_expand_ks<TY, TW, 4>(P, sh, vec, stream);
+  return cudaErrorInvalidValue;
+}
+
+template <typename TY, typename TW>
+static cudaError_t launch_adapt(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   g_chain_launch = false;        // the first launch waits for the work in front of the call, which may still write its inputs
   cudaError_t e = launch_adapt_shrink<TY, TW>(P, sh, stream);
-  return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, stream) : e;
+  return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, vec, stream) : e;
 }
 
 static cudaError_t launch_verify(const VerifyParams& P, cudaStream_t stream) {
@@ -1983,13 +1998,14 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
   AdaptParams P;
   memset(&P, 0, sizeof(P));
   int chunks = 0;
+  bool vec = true;               // rows of y and out start on boundaries of four elements
   for (int i = 0; i < nmat; ++i) {
     const b200rwkv_adapters& m = banks[i];
     if (!m.a || !m.b || !x[i] || !y[i] || !out[i] || !aligned16(m.a) || !aligned16(m.b) || !aligned16(x[i]))
       return fail(B200RWKV_EINVAL, "adapt_rows: matrix %d: null pointer, or a, b or x not 16-byte aligned", i);
     P.a[i] = m.a; P.b[i] = m.b; P.scale[i] = m.scale; P.x[i] = x[i]; P.y[i] = y[i]; P.out[i] = out[i]; P.n_out[i] = m.n_out;
     P.h[i] = reinterpret_cast<float*>(static_cast<char*>(workspace) + size_t(i) * (need / nmat));
-    P.vec[i] = m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
+    vec = vec && m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
     chunks += (m.n_out + sh.chunk_cols - 1) / sh.chunk_cols;
     P.chunk_end[i] = chunks;
   }
@@ -1998,9 +2014,9 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
   P.streams = streams; P.rt = sh.rt; P.splits = sh.splits; P.chunk_cols = sh.chunk_cols;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (dtype == B200RWKV_F32) e = launch_adapt<float, float>(P, sh, s);
-  else if (dtype == B200RWKV_BF16) e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __nv_bfloat16>(P, sh, s) : launch_adapt<__nv_bfloat16, __nv_bfloat16>(P, sh, s);
-  else e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __half>(P, sh, s) : launch_adapt<__half, __half>(P, sh, s);
+  if (dtype == B200RWKV_F32) e = launch_adapt<float, float>(P, sh, vec, s);
+  else if (dtype == B200RWKV_BF16) e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __nv_bfloat16>(P, sh, vec, s) : launch_adapt<__nv_bfloat16, __nv_bfloat16>(P, sh, vec, s);
+  else e = row_dtype == B200RWKV_F32 ? launch_adapt<float, __half>(P, sh, vec, s) : launch_adapt<__half, __half>(P, sh, vec, s);
   if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "adapt_rows: %s", cudaGetErrorString(e));
   return B200RWKV_OK;
 }

@@ -22,7 +22,7 @@ constexpr int kVerifySeg = 1024;           // weights per segment
 constexpr int kVerifySumWarps = 8;
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMaxDrafts = 64;
-constexpr int kVerifyMaxSegs = 512;        // vocabularies up to 524288
+constexpr int kVerifyMaxSegs = 512;        // vocabularies up to 524288; at most 16 a lane
 constexpr int kVerifyMaxCluster = 8;
 
 struct VerifyParams {
@@ -73,11 +73,9 @@ __global__ void __launch_bounds__(kVerifySumWarps * 32) verify_sums_kernel(const
 struct VerifyShared {
   double p_sum[kVerifyMaxDrafts + 1], q_sum[kVerifyMaxDrafts];
   double seg[kVerifyMaxSegs];              // of the distribution that is drawn from; rank 0's is used
+  double turn[32][33];                     // the weights of the segment that holds the number
   int ok[kVerifyMaxDrafts];
-  double P, Q;
-  int accepted, length, token;             // token: the refused one
-  int found;
-  double before, total;
+  int any;                                 // the distribution has a weight above zero
 };
 
 // The sum of one row's segments, by a warp.
@@ -85,6 +83,16 @@ __device__ __forceinline__ double verify_row_sum(const double* s, int segs) {
   double v = 0.0;
   for (int i = threadIdx.x & 31; i < segs; i += 32) v += __ldcg(s + i);
   return warp_sum_f64(v);
+}
+
+__device__ __forceinline__ double warp_inclusive_f64(double v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
 }
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const VerifyParams P) {
@@ -97,20 +105,33 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
   const float *target = P.target + b * P.target_stream, *draft = P.draft ? P.draft + b * P.draft_stream : nullptr;
   const long long* tokens = P.tokens + (long long)b * K;
   const float* u = P.u + (long long)b * (K + 1);
-  griddep_wait();
   const double* sums = P.sums + (long long)b * rows * segs;
+  if (tid == 0) S.any = 0;
+  // what was drafted, before the dependency: none of it comes from the first launch
+  double pd = 0.0, qd = 1.0, ut = 0.0;
+  if (warp < len) {
+    const long long d = __ldg(tokens + warp);
+    const bool known = d >= 0 && d < V;                            // any other token is refused
+    ut = double(__ldg(u + warp));
+    if (known) pd = verify_weight(__ldg(target + warp * P.target_row + d));
+    if (known && draft) qd = verify_weight(__ldg(draft + warp * P.draft_row + d));
+  }
+  griddep_wait();
   for (int r = warp; r <= len; r += kVerifyWarps) {
     const double p = verify_row_sum(sums + (long long)r * segs, segs);
     const double q = draft && r < len ? verify_row_sum(sums + (long long)(K + 1 + r) * segs, segs) : 1.0;
+    if (r > warp && r < len) {                                     // beyond the first: rare, many drafts
+      const long long d = __ldg(tokens + r);
+      const bool known = d >= 0 && d < V;
+      ut = double(__ldg(u + r));
+      pd = known ? verify_weight(__ldg(target + r * P.target_row + d)) : 0.0;
+      qd = known && draft ? verify_weight(__ldg(draft + r * P.draft_row + d)) : 1.0;
+    }
     if (lane == 0) {
       S.p_sum[r] = p;
       if (r < len) {
         S.q_sum[r] = q;
-        const long long d = __ldg(tokens + r);
-        const bool known = d >= 0 && d < V;                        // any other token is refused
-        const double pd = known ? verify_weight(__ldg(target + r * P.target_row + d)) : 0.0;
-        const double qd = known && draft ? verify_weight(__ldg(draft + r * P.draft_row + d)) : 1.0;
-        S.ok[r] = double(u[r]) * qd * p < pd * q;
+        S.ok[r] = ut * qd * p < pd * q;
       }
     }
   }
@@ -118,75 +139,89 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
   int n = 0;
   while (n < len && S.ok[n]) ++n;
   // the distribution: 0 the row itself, 1 without the refused token, 2 what the draft leaves of it
-  const int kind = n == len ? 0 : draft ? 2 : 1;
-  const float *pr = target + n * P.target_row, *qr = kind == 2 ? draft + n * P.draft_row : nullptr;
+  int kind = n == len ? 0 : draft ? 2 : 1;
+  const float *pr = target + n * P.target_row, *qr = kind == 2 ? draft + n * P.draft_row : pr;
   const double Ps = S.p_sum[n], Qs = kind == 2 ? S.q_sum[n] : 1.0;
   const long long refused = kind ? __ldg(tokens + n) : -1;
-  auto weight = [&](int i, int how) -> double {
-    const double p = verify_weight(__ldg(pr + i));
-    if (how == 0) return p;
-    if (how == 1) return i == refused ? 0.0 : p;
-    return fmax(p * Qs - verify_weight(__ldg(qr + i)) * Ps, 0.0);
+  auto weight = [&](float pf, float qf, int i) -> double {
+    const double p = verify_weight(pf);
+    if (kind == 0) return p;
+    if (kind == 1) return i == refused ? 0.0 : p;
+    return fmax(p * Qs - verify_weight(qf) * Ps, 0.0);
   };
+  constexpr int kPer = kVerifySeg / 32;
   VerifyShared* S0 = cluster.map_shared_rank(&S, 0);
   cluster.sync();                                                  // all CTAs run, so their shared memory exists
-  int how = kind;
   for (;;) {                                                       // a second time where the first distribution is empty
     for (int s = rank * kVerifyWarps + warp; s < segs; s += C * kVerifyWarps) {
+      const int first = s * kVerifySeg, m = V - first;
       double v = 0.0;
-#pragma unroll 8
-      for (int i = 0; i < kVerifySeg / 32; ++i) {
-        const int at = s * kVerifySeg + i * 32 + lane;
-        if (at < V) v += weight(at, how);
+      if (kind == 0) {                                             // the first launch has these
+        v = lane == 0 ? __ldcg(sums + (long long)n * segs + s) : 0.0;
+      } else {
+        float p[kPer], q[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int at = i * 32 + lane;
+          p[i] = at < m ? __ldg(pr + first + at) : 0.f;
+          q[i] = kind == 2 && at < m ? __ldg(qr + first + at) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v += weight(p[i], q[i], first + i * 32 + lane);
+        v = warp_sum_f64(v);
       }
-      v = warp_sum_f64(v);
-      if (lane == 0) S0->seg[s] = v;
+      if (lane == 0) {
+        S0->seg[s] = v;
+        if (v > 0.0)
+          for (int c = 0; c < C; ++c) cluster.map_shared_rank(&S, c)->any = 1;
+      }
     }
     cluster.sync();
-    double any = 0.0;
-    if (how) {
-      for (int s = 0; s < segs; ++s) any += S0->seg[s];
-      cluster.sync();                                              // read before it is written again
-    }
-    if (how == 0 || any > 0.0) break;
-    how = 0;
+    if (kind == 0 || S.any) break;                                 // the same in all CTAs
+    kind = 0;
+    cluster.sync();
   }
-  if (rank != 0) return;
-  if (warp == 0) {
-    double total = 0.0;
-    for (int s = 0; s < segs; ++s) total += S.seg[s];
-    const double aim = double(u[K]) * total;
-    int found = -1;
-    double run = 0.0, before = 0.0;
-    for (int s = 0; s < segs; ++s) {
-      const double v = S.seg[s];
-      if (v > 0.0) {
-        found = s; before = run;
-        if (run + v >= aim) break;
-      }
-      run += v;
-    }
-    long long pick = -1;
-    if (found >= 0) {
-      run = before;
-      for (int i = 0; i < kVerifySeg / 32; ++i) {
-        const int at = found * kVerifySeg + i * 32 + lane;
-        const double w = at < V ? weight(at, how) : 0.0;
-        double inc = w;
+  if (rank != 0 || warp != 0) return;
+  // the segment that holds the number: a lane has `per` consecutive ones
+  const int per = (segs + 31) / 32, s0 = min(segs, lane * per), s1 = min(segs, s0 + per);
+  double mine = 0.0;
+  for (int s = s0; s < s1; ++s) mine += S.seg[s];
+  const double upto = warp_inclusive_f64(mine), total = __shfl_sync(0xffffffffu, upto, 31), aim = double(__ldg(u + K)) * total;
+  // the first with weight whose running sum reaches the aim, else (rounding) the last with weight
+  auto choose = [&](bool some, bool reached) {
+    const unsigned hit = __ballot_sync(0xffffffffu, some && reached), any = __ballot_sync(0xffffffffu, some);
+    return hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : -1;
+  };
+  const int who = choose(mine > 0.0, upto >= aim);
+  long long pick = -1;
+  if (who >= 0) {
+    double run = __shfl_sync(0xffffffffu, upto - mine, who);
+    const int w0 = who * per;
+    const double seg = lane < per && w0 + lane < segs ? S.seg[w0 + lane] : 0.0;
+    const double seg_upto = warp_inclusive_f64(seg) + run;
+    const int at = choose(seg > 0.0, seg_upto >= aim), first = (w0 + at) * kVerifySeg, m = V - first;
+    run = __shfl_sync(0xffffffffu, seg_upto - seg, at);
+    float p[kPer], q[kPer];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += x;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + inc >= aim), some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (some) pick = found * kVerifySeg + i * 32 + (hit ? __ffs(hit) - 1 : 31 - __clz(some));
-        if (hit) break;
-        run += __shfl_sync(0xffffffffu, inc, 31);
-      }
+    for (int i = 0; i < kPer; ++i) {
+      const int j = i * 32 + lane;
+      p[i] = j < m ? __ldg(pr + first + j) : 0.f;
+      q[i] = kind == 2 && j < m ? __ldg(qr + first + j) : 0.f;
     }
-    for (int i = lane; i <= K; i += 32) P.out[(long long)b * (K + 1) + i] = i < n ? tokens[i] : i == n ? pick : -1;
-    if (lane == 0) P.accepted[b] = n;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) S.turn[i][lane] = weight(p[i], q[i], first + i * 32 + lane);
+    __syncwarp();
+    double sum = 0.0;                                              // of the lane's 32 consecutive weights
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += S.turn[lane][i];
+    const double sum_upto = warp_inclusive_f64(sum) + run;
+    const int group = choose(sum > 0.0, sum_upto >= aim);
+    run = __shfl_sync(0xffffffffu, sum_upto - sum, group);
+    const double w = S.turn[group][lane], w_upto = warp_inclusive_f64(w) + run;
+    pick = first + group * 32 + choose(w > 0.0, w_upto >= aim);
   }
+  for (int i = lane; i <= K; i += 32) P.out[(long long)b * (K + 1) + i] = i < n ? __ldg(tokens + i) : i == n ? pick : -1;
+  if (lane == 0) P.accepted[b] = n;
 }
 
 inline int verify_segs(int V) { return (V + kVerifySeg - 1) / kVerifySeg; }
