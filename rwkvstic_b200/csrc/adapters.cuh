@@ -32,6 +32,7 @@ constexpr int kAdaptWindow = 1024;         // streams
 constexpr int kAdaptMaxRank = 256;
 constexpr int kAdaptMaxRows = 64;          // of a tile
 constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
+constexpr int kShrinkChunk = 64, kShrinkStages = 4;   // k of a stage of the tiled form
 constexpr int kExpandThreads = 128, kExpandWarps = kExpandThreads / 32;
 
 struct AdaptParams {
@@ -158,7 +159,8 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
 }
 
 // h[split][row][j] = sum over the split's K of x[row][k] A[id][j][k].  Grid (tiles, rank chunks of 16 * MT, matrices * splits).
-// A warp takes 16 rows (as columns of the products, 8 at a time) and, of the split's blocks of 32 k, every (8 / row ways)-th.
+// For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter: from global memory to
+// registers.  A warp takes every eighth block of 32 k of the split.
 template <typename TX, typename TW, int MT, int NT>
 __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int mat, int split, int chunk, const int* rows,
                                             int count, float* red) {
@@ -167,14 +169,11 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
   constexpr int RC = 16 * MT, kStride = RC + 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int K = P.K, rank = P.rank;
-  // row ways, ways along K: the same for every tile of a call, so that a row's sums do not depend on the rows beside it
-  const int rw = P.rt / 16, kw = kShrinkWarps / rw;
-  const int my_rows = (warp % rw) * 16, my_k = warp / rw;
   const TX* xp[NT];
   bool xok[NT];
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
-    const int i = my_rows + q * 8 + g;
+    const int i = q * 8 + g;
     xok[q] = i < count;
     xp[q] = x + size_t(xok[q] ? rows[i] : 0) * K + 8 * t;
   }
@@ -196,14 +195,14 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
   const int blocks = (K + 31) / 32, b0 = int((long long)blocks * split / P.splits), b1 = int((long long)blocks * (split + 1) / P.splits);
-  for (int kb = b0 + my_k; kb < b1; kb += 2 * kw) {
+  for (int kb = b0 + warp; kb < b1; kb += 2 * kShrinkWarps) {
     // two blocks of 32 k: all loads first
     AdaptRaw<TX, 8> rx[2][NT];
     AdaptRaw<TW, 8> ra[2][MT][2];
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      const int k = (kb + o * kw) * 32;
-      const bool in = kb + o * kw < b1 && k + 8 * t < K;  // K is a multiple of 8
+      const int k = (kb + o * kShrinkWarps) * 32;
+      const bool in = kb + o * kShrinkWarps < b1 && k + 8 * t < K;  // K is a multiple of 8
 #pragma unroll
       for (int q = 0; q < NT; ++q) rx[o][q].load(xp[q] + k, in && xok[q]);
 #pragma unroll
@@ -268,7 +267,7 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
     const int r = i / RC, j = i - r * RC;
     if (chunk * RC + j >= rank) continue;
     float s = 0.f;
-    for (int w = 0; w < kw; ++w) s += red[((w * rw + (r >> 4)) * 16 + (r & 15)) * kStride + j];
+    for (int w = 0; w < kShrinkWarps; ++w) s += red[(w * 16 + r) * kStride + j];
     h[size_t(rows[r]) * rank + chunk * RC + j] = s;
   }
 }
@@ -287,6 +286,149 @@ __global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const Adap
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
   if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, red);
   else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, red);
+}
+
+// The same for tiles of 64 rows of one stream: x and A are staged in shared memory, 64 k at a time, four stages ahead of the
+// products.  Four warps take 16 rows each, for one half of a stage's k; four more the other half.
+template <typename T>
+struct StageTile {                         // 64 elements of each row, in 16-byte units dealt out so that fragment reads meet no bank twice
+  static constexpr int kUnits = kShrinkChunk * int(sizeof(T)) / 16, kRowBytes = kUnits * 16;
+  __device__ static __forceinline__ int swizzle(int row, int unit) { return sizeof(T) == 2 ? unit ^ ((row & 3) << 1) : unit ^ ((row & 1) << 2); }
+  // rows of `ld` elements at src, those below `rows`, from element k (of `end`) on
+  template <int R>
+  __device__ static __forceinline__ void request(uint32_t dst, const T* src, int rows, size_t ld, int k, int end) {
+    for (int i = threadIdx.x; i < R * kUnits; i += kShrinkThreads) {
+      const int r = i / kUnits, u = i % kUnits, at = k + u * (16 / int(sizeof(T)));
+      const bool ok = r < rows && at < end;
+      cp_async16(dst + r * kRowBytes + swizzle(r, u) * 16, src + (ok ? size_t(r) * ld + at : 0), ok);
+    }
+  }
+  // elements 16 step + 4 t .. + 3 of a row
+  __device__ static __forceinline__ void read(const char* tile, int row, int step, int t, AdaptRaw<T, 4>& f) {
+    if constexpr (sizeof(T) == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(tile + row * kRowBytes + swizzle(row, 2 * step + (t >> 1)) * 16 + (t & 1) * 8);
+      f.w[0] = v.x; f.w[1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + swizzle(row, 4 * step + t) * 16);
+      f.w[0] = v.x; f.w[1] = v.y; f.w[2] = v.z; f.w[3] = v.w;
+    }
+  }
+};
+
+template <typename TX, typename TW, int MT>
+constexpr int shrink_tile_smem() {
+  const int stages = kShrinkStages * (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
+  const int sums = kShrinkWarps * 16 * (16 * MT + 4) * 4;
+  return stages > sums ? stages : sums;
+}
+
+template <typename TX, typename TW, int MT>
+__global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(const AdaptParams P) {
+  constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
+  constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
+  constexpr int RC = 16 * MT, kStride = RC + 4, NT = 2;
+  constexpr int kBytesX = kAdaptMaxRows * StageTile<TX>::kRowBytes, kBytes = kBytesX + RC * StageTile<TW>::kRowBytes;
+  extern __shared__ __align__(128) char stages[];
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int per = (P.T + kAdaptMaxRows - 1) / kAdaptMaxRows, s = blockIdx.x / per, first = (blockIdx.x - s * per) * kAdaptMaxRows;
+  const int count = min(kAdaptMaxRows, P.T - first), row0 = s * P.T + first, K = P.K, rank = P.rank;
+  const long long asked = __ldg(P.ids + s);
+  if (asked < 0 || asked >= P.adapters) return;
+  const int mat = blockIdx.z / P.splits, split = blockIdx.z - mat * P.splits, j0 = blockIdx.y * RC, ranks = min(RC, rank - j0);
+  const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
+  const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
+  const int chunks = (K + kShrinkChunk - 1) / kShrinkChunk, c0 = int((long long)chunks * split / P.splits), c1 = int((long long)chunks * (split + 1) / P.splits);
+  const uint32_t base = smem_u32(stages);
+  auto request = [&](int c) {
+    if (c < c1) {
+      const uint32_t at = base + (c - c0) % kShrinkStages * kBytes;
+      StageTile<TX>::template request<kAdaptMaxRows>(at, x, count, K, c * kShrinkChunk, K);
+      StageTile<TW>::template request<RC>(at + kBytesX, a, ranks, K, c * kShrinkChunk, K);
+    }
+    cp_async_commit();                     // a group per stage, also an empty one
+  };
+#pragma unroll
+  for (int i = 0; i < kShrinkStages - 1; ++i) request(c0 + i);
+  const int my_rows = (warp & 3) * 16, half = warp >> 2;
+  float sum[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
+  for (int c = c0; c < c1; ++c) {
+    cp_async_wait<kShrinkStages - 2>();
+    __syncthreads();                       // the stage has arrived; everyone is done with the one that is requested next
+    request(c + kShrinkStages - 1);
+    const char* tx = stages + (c - c0) % kShrinkStages * kBytes;
+    const char* ta = tx + kBytesX;
+    float part[MT][NT][4];                 // the tensor cores cut their sums off; the running sum rounds
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[m][q][i] = 0.f;
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      const int step = 2 * half + o;
+      uint32_t fx[NT][2][PX];
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        AdaptRaw<TX, 4> f;
+        StageTile<TX>::read(tx, my_rows + q * 8 + g, step, t, f);
+        f.template pair<PX>(0, fx[q][0]);
+        f.template pair<PX>(1, fx[q][1]);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint32_t fa[4][PW];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          AdaptRaw<TW, 4> f;
+          StageTile<TW>::read(ta, m * 16 + e * 8 + g, step, t, f);
+          f.template pair<PW>(0, fa[e]);
+          f.template pair<PW>(1, fa[2 + e]);
+        }
+#pragma unroll
+        for (int i = PW - 1; i >= 0; --i) {
+          const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
+#pragma unroll
+          for (int j = PX - 1; j >= 0; --j) {
+            if (i + j >= 3) continue;
+#pragma unroll
+            for (int q = 0; q < NT; ++q) {
+              if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
+              else mma_bf16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
+  }
+  cp_async_wait<0>();
+  __syncthreads();                         // the stages become the table of sums
+  float* red = reinterpret_cast<float*>(stages);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[(warp * 16 + q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = sum[m][q][i];
+  __syncthreads();
+  float* h = P.h[mat] + (size_t(split) * P.R + row0) * rank + j0;
+  for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
+    const int r = i / RC, j = i - r * RC;
+    if (j < ranks) h[size_t(r) * rank + j] = red[r * kStride + j] + red[(64 + r) * kStride + j];
+  }
 }
 
 // 16-byte blocks of a row of h in shared memory: an odd number of 32-byte groups, so that 8-byte reads of eight rows by four
@@ -319,6 +461,10 @@ struct AdaptFour {
       w[0] = v.x; w[1] = v.y;
     }
   }
+  __device__ __forceinline__ void store(TY* p) const {
+    if constexpr (sizeof(TY) == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
   // + f, rounded once
   __device__ __forceinline__ void add_store(TY* p, const float (&f)[4]) const {
     if constexpr (std::is_same<TY, float>::value) {
@@ -342,6 +488,33 @@ struct AdaptFour {
   }
 };
 
+// Columns c_begin .. c_end of `count` rows, eight accesses of a thread in flight.
+template <typename TY, bool VEC>
+__device__ __forceinline__ void adapt_copy(const TY* y, TY* out, const int* rows, int count, int N, int c_begin, int c_end) {
+  constexpr int W = VEC ? 4 : 1, U = 8;
+  const int wide = (c_end - c_begin) / W, items = count * wide;
+  for (int first = threadIdx.x; first < items; first += U * kExpandThreads) {
+    AdaptFour<TY> four[U];
+    TY one[U];
+    size_t at[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = first + k * kExpandThreads;
+      if (i >= items) continue;
+      const int r = i / wide;
+      at[k] = size_t(rows[r]) * N + c_begin + size_t(i - r * wide) * W;
+      if constexpr (VEC) four[k].load(y + at[k]);
+      else one[k] = y[at[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (first + k * kExpandThreads >= items) continue;
+      if constexpr (VEC) four[k].store(out + at[k]);
+      else out[at[k]] = one[k];
+    }
+  }
+}
+
 // Products of 8 columns that a warp forms at a time: more where a column has few bytes, so that its loads are as many.
 __host__ __device__ constexpr int expand_nb(int ks, int mr, int w_pieces) { return mr == 1 && ks < 4 && w_pieces == 1 ? 8 : 4; }
 
@@ -354,11 +527,13 @@ __host__ __device__ constexpr int expand_nb(int ks, int mr, int w_pieces) { retu
 // KS: steps of 16 ranks whose fragments are held (ranks beyond are fetched step by step); MR: tiles of 16 * MR rows; VEC: all
 // rows of y and out start on boundaries of four elements.
 template <typename TY, typename TW, int KS, int MR, bool VEC>
-__global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_kernel(const AdaptParams P) {
+__global__ void __launch_bounds__(kExpandThreads, MR == 1 || VEC ? 4 : 3) adapt_expand_kernel(const AdaptParams P) {
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
   constexpr int NB = expand_nb(KS, MR, PW), MB = MR == 1 ? 1 : 2, COLS = 8 * NB;
   extern __shared__ __align__(16) unsigned short hs[];     // [pieces][16 MR][stride]
+  constexpr bool kRing = VEC && MR > 1;
   __shared__ float turn[VEC ? 1 : kExpandWarps][VEC ? 1 : 16 * MB][COLS + 1];
+  __shared__ __align__(16) TY ring[kRing ? kExpandWarps : 1][2][kRing ? 16 * MB * COLS : 8];
   __shared__ int rows[16 * MR];
   __shared__ uint32_t mask[kAdaptWindow / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -372,11 +547,7 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_
   TY* out = static_cast<TY*>(P.out[mat]);
   if (count == 0) return;
   if (id < 0) {                                            // no adapter: only a copy, where out is not y
-    if (y == out) return;
-    for (int i = warp; i < count; i += kExpandWarps) {
-      const size_t row = size_t(rows[i]) * N;
-      for (int c = c_begin + lane; c < c_end; c += 32) out[row + c] = y[row + c];
-    }
+    if (y != out) adapt_copy<TY, VEC>(y, out, rows, count, N, c_begin, c_end);
     return;
   }
   const int rank = P.rank, ksteps = (rank + 15) / 16, stride = expand_stride(rank), padded = (count + 15) / 16 * 16;
@@ -397,6 +568,26 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_
   };
   int c0 = c_begin + warp * COLS;
   if (held) fetch(c0, 0);                                  // weights: no part of what the first launch writes
+  // y of 32 rows and 32 columns into one of the warp's two tiles, in units of four elements dealt out so that reads of eight rows
+  // by four lanes each meet no bank twice
+  auto ring_unit = [](int row, int unit) { return row * (COLS / 4) + (unit ^ (sizeof(TY) == 4 ? (row & 1) << 2 : (row & 2) << 1)); };
+  auto ring_fill = [&](int buf, int c, int m0) {
+    if constexpr (kRing) {
+#pragma unroll
+      for (int k = 0; k < 16 * MB * COLS / 4 / 32; ++k) {
+        const int i = (k * 32 + lane) / (COLS / 4), u = (k * 32 + lane) % (COLS / 4);
+        if (m0 + i < count && c + 4 * u < c_end) {
+          const uint32_t dst = smem_u32(&ring[warp][buf][ring_unit(i, u) * 4]);
+          const TY* src = y + size_t(rows[m0 + i]) * N + c + 4 * u;
+          if constexpr (sizeof(TY) == 4) cp_async16(dst, src, true);
+          else cp_async8(dst, src, true);
+        }
+      }
+      cp_async_commit();
+    }
+  };
+  int turn_of = 0;
+  if (c0 < c_end) ring_fill(0, c0, 0);
   const int plane = 16 * MR * stride;
   griddep_wait();
   {
@@ -422,9 +613,13 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_
   __syncthreads();
   for (; c0 < c_end; c0 += kExpandWarps * COLS) {
     for (int m0 = 0; m0 < count; m0 += 16 * MB) {
+      const int next = c0 + kExpandWarps * COLS;
       AdaptFour<TY> four[MB][2][NB / 2];                   // y: rows m0 + 16 m + 8 e + g, columns c0 + 16 q + 4 t ..
       TY line[16 * MB][COLS / 32];                         // or rows m0 + i, columns c0 + 32 q + lane
-      if constexpr (VEC) {
+      if constexpr (kRing) {
+        const bool more = m0 + 16 * MB < count;
+        if (more || next < c_end) ring_fill(turn_of ^ 1, more ? c0 : next, more ? m0 + 16 * MB : 0);
+      } else if constexpr (VEC) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -481,8 +676,19 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_
           }
         }
       }
-      const int next = c0 + kExpandWarps * COLS;
-      if (held && m0 + 16 * MB >= count && next < c_end) fetch(next, 0);
+      const bool last = m0 + 16 * MB >= count;
+      if (held && last && next < c_end) fetch(next, 0);
+      if constexpr (kRing) {
+        if (last && next >= c_end) cp_async_wait<0>();
+        else cp_async_wait<1>();
+        __syncwarp();
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int q = 0; q < NB / 2; ++q) four[m][e][q].load(&ring[warp][turn_of][ring_unit(m * 16 + e * 8 + g, 4 * q + t) * 4]);
+      }
       if constexpr (VEC) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
@@ -515,6 +721,10 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 ? 4 : 3) adapt_expand_
             for (int q = 0; q < COLS / 32; ++q)
               if (c0 + q * 32 + lane < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[warp][i][q * 32 + lane]);
           }
+      }
+      if constexpr (kRing) {
+        __syncwarp();                                      // the tile is read before it is filled again
+        turn_of ^= 1;
       }
     }
   }

@@ -733,12 +733,29 @@ static cudaError_t launch_sample(const float* x, int rows, int n, long long ldx,
 }
 
 // ---------------------------------------------------------------------------------------- adapters, verification
+template <typename TX, typename TW, int MT>
+static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  const dim3 grid(sh.tiles, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat * P.splits);
+  if (sh.rt == 16) return launch_chained(adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), 0, stream, P);
+  static bool configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  constexpr int smem = shrink_tile_smem<TX, TW, MT>();
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(adapt_shrink_tile_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch_chained(adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), smem, stream, P);
+}
+
 template <typename TX, typename TW>
 static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  const dim3 grid(sh.tiles, (P.rank + 16 * sh.mt - 1) / (16 * sh.mt), P.nmat * P.splits);
-  if (sh.mt == 1) return launch_chained(adapt_shrink_kernel<TX, TW, 1>, grid, dim3(kShrinkThreads), 0, stream, P);
-  if (sh.mt == 2) return launch_chained(adapt_shrink_kernel<TX, TW, 2>, grid, dim3(kShrinkThreads), 0, stream, P);
-  if constexpr (AdaptType<TW>::kPieces == 1) return launch_chained(adapt_shrink_kernel<TX, TW, 4>, grid, dim3(kShrinkThreads), 0, stream, P);
+  if (sh.mt == 1) return launch_adapt_shrink_as<TX, TW, 1>(P, sh, stream);
+  if (sh.mt == 2) return launch_adapt_shrink_as<TX, TW, 2>(P, sh, stream);
+  if constexpr (AdaptType<TW>::kPieces == 1) return launch_adapt_shrink_as<TX, TW, 4>(P, sh, stream);
   return cudaErrorInvalidValue;
 }
 
