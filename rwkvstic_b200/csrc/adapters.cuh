@@ -33,7 +33,7 @@ constexpr int kAdaptMaxRank = 256;
 constexpr int kAdaptMaxRows = 64;          // of a tile
 constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
 constexpr int kShrinkChunk = 64, kShrinkStages = 4;   // k of a stage of the tiled form
-constexpr int kExpandThreads = 128, kExpandWarps = kExpandThreads / 32;
+constexpr int kExpandThreads = 256, kExpandWarps = kExpandThreads / 32;
 
 struct AdaptParams {
   const void *a[kAdaptMaxMats], *b[kAdaptMaxMats], *x[kAdaptMaxMats], *y[kAdaptMaxMats];
@@ -431,10 +431,6 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(co
   }
 }
 
-// 16-byte blocks of a row of h in shared memory: an odd number of 32-byte groups, so that 8-byte reads of eight rows by four
-// lanes each meet every bank once.
-__host__ __device__ constexpr int expand_stride(int rank) { return ((rank + 15) / 16 | 1) * 16; }
-
 template <typename TY>
 __device__ __forceinline__ float adapt_float(TY v) {
   if constexpr (std::is_same<TY, float>::value) return v;
@@ -516,25 +512,30 @@ __device__ __forceinline__ void adapt_copy(const TY* y, TY* out, const int* rows
 }
 
 // Products of 8 columns that a warp forms at a time: more where a column has few bytes, so that its loads are as many.
-__host__ __device__ constexpr int expand_nb(int ks, int mr, int w_pieces) { return mr == 1 && ks < 4 && w_pieces == 1 ? 8 : 4; }
+__host__ __device__ constexpr int expand_nb(int ks, int w_pieces) { return ks < 4 && w_pieces < 3 ? 8 : 4; }
+constexpr int kExpandStages = 2;           // of y, per warp
+// Shared memory: h in the fragments' own order, [row tile][step of 16 ranks][piece][lane] of 16 bytes; then per warp the stages of
+// y, or the table in which odd rows are turned.
+template <typename TY>
+__host__ __device__ constexpr int expand_h_bytes(int row_tiles, int rank) { return row_tiles * ((rank + 15) / 16) * (sizeof(TY) == 2 ? 2 : 3) * 512; }
+template <typename TY, int NB, bool VEC>
+__host__ __device__ constexpr int expand_warp_bytes() { return VEC ? kExpandStages * 16 * 8 * NB * int(sizeof(TY)) : 16 * (8 * NB + 1) * 4; }
 
 // out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles, column chunks of all matrices).
-// A warp takes 8 * NB columns and 16 * MB rows at a time; the columns of two products are dealt out so that a lane ends up with
-// four consecutive ones.  Its fragments of B for the next columns are requested in front of the stores of the present ones,
-// its y in front of the products.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16 bits, enough
-// for a 16-bit y.  Rows that do not start on boundaries of four elements (an odd number of columns) are turned in shared memory,
-// so that a warp's access is one line of a row instead of quarters of eight.
-// KS: steps of 16 ranks whose fragments are held (ranks beyond are fetched step by step); MR: tiles of 16 * MR rows; VEC: all
-// rows of y and out start on boundaries of four elements.
-template <typename TY, typename TW, int KS, int MR, bool VEC>
-__global__ void __launch_bounds__(kExpandThreads, MR == 1 || VEC ? 4 : 3) adapt_expand_kernel(const AdaptParams P) {
+// A warp has 16 rows and takes 8 * NB columns at a time; the columns of two products are dealt out so that a lane ends up with
+// four consecutive ones of two rows.  In a tile of 64 rows four warps take the same columns, in one of 16 all take their own.
+// Fragments of B for the next columns are requested in front of the stores of the present ones; a lane's y comes by asynchronous
+// copies into slots of its own, one step ahead.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16
+// bits, enough for a 16-bit y.  Rows that do not start on boundaries of four elements (an odd number of columns) are turned in
+// shared memory, so that a warp's access is one line of a row instead of quarters of eight.
+// KS: steps of 16 ranks whose fragments are held (with more, all are fetched in KS at a time); VEC: all rows of y and out start
+// on boundaries of four elements.
+template <typename TY, typename TW, int KS, bool VEC>
+__global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const AdaptParams P) {
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
-  constexpr int NB = expand_nb(KS, MR, PW), MB = MR == 1 ? 1 : 2, COLS = 8 * NB;
-  extern __shared__ __align__(16) unsigned short hs[];     // [pieces][16 MR][stride]
-  constexpr bool kRing = VEC && MR > 1;
-  __shared__ float turn[VEC ? 1 : kExpandWarps][VEC ? 1 : 16 * MB][COLS + 1];
-  __shared__ __align__(16) TY ring[kRing ? kExpandWarps : 1][2][kRing ? 16 * MB * COLS : 8];
-  __shared__ int rows[16 * MR];
+  constexpr int NB = expand_nb(KS, PW), COLS = 8 * NB;
+  extern __shared__ __align__(16) char shared[];
+  __shared__ int rows[kAdaptMaxRows];
   __shared__ uint32_t mask[kAdaptWindow / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   int id = -1;
@@ -550,51 +551,66 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 || VEC ? 4 : 3) adapt_
     if (y != out) adapt_copy<TY, VEC>(y, out, rows, count, N, c_begin, c_end);
     return;
   }
-  const int rank = P.rank, ksteps = (rank + 15) / 16, stride = expand_stride(rank), padded = (count + 15) / 16 * 16;
+  const int rank = P.rank, ksteps = (rank + 15) / 16;
   const bool held = ksteps <= KS;
-  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  const int row_ways = P.rt / 16, my_rows = warp % row_ways * 16, step = kExpandWarps / row_ways * COLS;
+  int c0 = c_begin + warp / row_ways * COLS;
+  const bool mine = my_rows < count && c0 < c_end;         // this warp has anything to do
+  // a lane's column of product n is col + (n / 2) * 16 + (n % 2) * 2, its ranks of a step 4 t .. 4 t + 3
+  const int col = 4 * (g >> 1) + (g & 1);
+  const TW* b = static_cast<const TW*>(P.b[mat]) + (size_t(id) * N + col) * rank + 4 * t;
+  const bool tail = (ksteps - 1) * 16 + 4 * t < rank;      // the lane's ranks of the last step exist (rank is a multiple of four)
   AdaptRaw<TW, 4> raw[NB][KS];
-  auto fetch = [&](int c0, int k0) {
+  auto fetch = [&](int c, int k0) {
+    const TW* at = b + size_t(c) * rank + k0 * 16;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int c = c0 + (n >> 1) * 16 + 4 * (g >> 1) + 2 * (n & 1) + (g & 1);
+      const int off = (n >> 1) * 16 + (n & 1) * 2;
+      const bool in = c + col + off < c_end;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int j = (k0 + s) * 16 + 4 * t;
-        const bool ok = c < c_end && j < rank;             // rank is a multiple of four
-        raw[n][s].load(b + (ok ? size_t(c) * rank + j : 0), ok);
-      }
+      for (int s = 0; s < KS; ++s)
+        raw[n][s].load(at + off * rank + s * 16, in && (k0 + s < ksteps - 1 || (k0 + s == ksteps - 1 && tail)));
     }
   };
-  int c0 = c_begin + warp * COLS;
-  if (held) fetch(c0, 0);                                  // weights: no part of what the first launch writes
-  // y of 32 rows and 32 columns into one of the warp's two tiles, in units of four elements dealt out so that reads of eight rows
-  // by four lanes each meet no bank twice
-  auto ring_unit = [](int row, int unit) { return row * (COLS / 4) + (unit ^ (sizeof(TY) == 4 ? (row & 1) << 2 : (row & 2) << 1)); };
-  auto ring_fill = [&](int buf, int c, int m0) {
-    if constexpr (kRing) {
+  // y: rows g and g + 8 of the warp's, columns c + 16 q + 4 t .. + 3
+  const TY* yp[2];
+  TY* op[2];
+  bool row_ok[2];
 #pragma unroll
-      for (int k = 0; k < 16 * MB * COLS / 4 / 32; ++k) {
-        const int i = (k * 32 + lane) / (COLS / 4), u = (k * 32 + lane) % (COLS / 4);
-        if (m0 + i < count && c + 4 * u < c_end) {
-          const uint32_t dst = smem_u32(&ring[warp][buf][ring_unit(i, u) * 4]);
-          const TY* src = y + size_t(rows[m0 + i]) * N + c + 4 * u;
-          if constexpr (sizeof(TY) == 4) cp_async16(dst, src, true);
-          else cp_async8(dst, src, true);
-        }
+  for (int e = 0; e < 2; ++e) {
+    const int i = my_rows + e * 8 + g;
+    row_ok[e] = i < count;
+    const size_t at = size_t(row_ok[e] ? rows[i] : rows[0]) * N + 4 * t;
+    yp[e] = y + at; op[e] = out + at;
+  }
+  char* slots = shared + expand_h_bytes<TY>(row_ways, rank) + warp * expand_warp_bytes<TY, NB, VEC>();
+  constexpr int kUnit = 4 * sizeof(TY), kStage = NB * 32 * kUnit;
+  auto request = [&](int stage, int c) {
+    if constexpr (VEC) {
+      if (c < c_end) {
+        const uint32_t dst = smem_u32(slots) + stage * kStage + lane * kUnit;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < NB / 2; ++q)
+            if (row_ok[e] && c + q * 16 + 4 * t < c_end) {
+              if constexpr (sizeof(TY) == 4) cp_async16(dst + (e * (NB / 2) + q) * 32 * kUnit, yp[e] + c + q * 16, true);
+              else cp_async8(dst + (e * (NB / 2) + q) * 32 * kUnit, yp[e] + c + q * 16, true);
+            }
       }
-      cp_async_commit();
+      cp_async_commit();                                   // a group per step, also an empty one
     }
   };
-  int turn_of = 0;
-  if (c0 < c_end) ring_fill(0, c0, 0);
-  const int plane = 16 * MR * stride;
+  if (mine) {                                              // neither weights nor y come from the first launch
+    if (held) fetch(c0, 0);
+    request(0, c0);
+  }
   griddep_wait();
   {
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
-    const int r4 = ksteps * 4;                             // groups of four ranks
+    const int r4 = ksteps * 4, padded = (count + 15) / 16 * 16;      // groups of four ranks; rows
     for (int i = tid; i < padded * r4; i += kExpandThreads) {
-      const int r = i / r4, j = (i - r * r4) * 4;
+      const int r = i / r4, j4 = i - r * r4, j = j4 * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < count && j < rank) {
         const float* h = P.h[mat] + size_t(rows[r]) * rank + j;
@@ -606,128 +622,92 @@ __global__ void __launch_bounds__(kExpandThreads, MR == 1 || VEC ? 4 : 3) adapt_
       uint32_t lo[PH], hi[PH];
       split_pair<PH>(s.x * scale, s.y * scale, lo);
       split_pair<PH>(s.z * scale, s.w * scale, hi);
+      uint32_t* f = reinterpret_cast<uint32_t*>(shared) + (((r >> 4) * ksteps + (j4 >> 2)) * PH * 32 + (r & 7) * 4 + (j4 & 3)) * 4 + ((r >> 3) & 1);
 #pragma unroll
-      for (int p = 0; p < PH; ++p) *reinterpret_cast<uint2*>(hs + size_t(p) * plane + r * stride + j) = make_uint2(lo[p], hi[p]);
+      for (int p = 0; p < PH; ++p) { f[p * 128] = lo[p]; f[p * 128 + 2] = hi[p]; }
     }
   }
   __syncthreads();
-  for (; c0 < c_end; c0 += kExpandWarps * COLS) {
-    for (int m0 = 0; m0 < count; m0 += 16 * MB) {
-      const int next = c0 + kExpandWarps * COLS;
-      AdaptFour<TY> four[MB][2][NB / 2];                   // y: rows m0 + 16 m + 8 e + g, columns c0 + 16 q + 4 t ..
-      TY line[16 * MB][COLS / 32];                         // or rows m0 + i, columns c0 + 32 q + lane
-      if constexpr (kRing) {
-        const bool more = m0 + 16 * MB < count;
-        if (more || next < c_end) ring_fill(turn_of ^ 1, more ? c0 : next, more ? m0 + 16 * MB : 0);
-      } else if constexpr (VEC) {
+  if (!mine) return;
+  const uint4* hf = reinterpret_cast<const uint4*>(shared) + (my_rows / 16 * ksteps) * PH * 32 + lane;
+  for (int stage = 0; c0 < c_end; c0 += step, stage ^= 1) {
+    TY line[VEC ? 1 : 16][VEC ? 1 : COLS / 32];            // not VEC: rows i, columns c0 + 32 q + lane
+    if constexpr (VEC) {
+      request(stage ^ 1, c0 + step);
+    } else {
 #pragma unroll
-        for (int m = 0; m < MB; ++m)
+      for (int i = 0; i < 16; ++i)
+        if (my_rows + i < count) {
+          const TY* p = y + size_t(rows[my_rows + i]) * N + c0 + lane;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = m0 + m * 16 + e * 8 + g;
-            const TY* p = y + size_t(i < count ? rows[i] : 0) * N + c0 + 4 * t;
+          for (int q = 0; q < COLS / 32; ++q)
+            if (c0 + q * 32 + lane < c_end) line[i][q] = p[q * 32];
+        }
+    }
+    float acc[NB][4];
 #pragma unroll
-            for (int q = 0; q < NB / 2; ++q)
-              if (i < count && c0 + q * 16 + 4 * t < c_end) four[m][e][q].load(p + q * 16);
-          }
-      } else {
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16 * MB; ++i)
-          if (m0 + i < count) {
-            const TY* p = y + size_t(rows[m0 + i]) * N + c0 + lane;
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    for (int k0 = 0; k0 < ksteps; k0 += KS) {
+      if (!held) fetch(c0, k0);
 #pragma unroll
-            for (int q = 0; q < COLS / 32; ++q)
-              if (c0 + q * 32 + lane < c_end) line[i][q] = p[q * 32];
-          }
-      }
-      float acc[MB][NB][4];
+      for (int s = 0; s < KS; ++s) {
+        if (k0 + s >= ksteps) break;
+        uint32_t fb[NB][2][PW];
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
+        for (int n = 0; n < NB; ++n) {
+          raw[n][s].template pair<PW>(0, fb[n][0]);
+          raw[n][s].template pair<PW>(1, fb[n][1]);
+        }
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int p = PH - 1; p >= 0; --p) {
+          const uint4 v = hf[((k0 + s) * PH + p) * 32];
+          const uint32_t f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-      for (int k0 = 0; k0 < ksteps; k0 += KS) {
-        if (!held) fetch(c0, k0);
+          for (int w = PW - 1; w >= 0; --w) {
+            if (p + w >= PH) continue;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          if (k0 + s >= ksteps) break;
-          uint32_t fb[NB][2][PW];
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            raw[n][s].template pair<PW>(0, fb[n][0]);
-            raw[n][s].template pair<PW>(1, fb[n][1]);
-          }
-#pragma unroll
-          for (int m = 0; m < MB; ++m) {
-            if (m && m0 + 16 * m >= count) break;
-#pragma unroll
-            for (int p = PH - 1; p >= 0; --p) {
-              const unsigned short* at = hs + size_t(p) * plane + (m0 + m * 16 + g) * stride + (k0 + s) * 16 + 4 * t;
-              const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8 * stride);
-              const uint32_t f[4] = {u.x, v.x, u.y, v.y};
-#pragma unroll
-              for (int w = PW - 1; w >= 0; --w) {
-                if (p + w >= PH) continue;
-#pragma unroll
-                for (int n = 0; n < NB; ++n) mma_bf16(acc[m][n], f, fb[n][0][w], fb[n][1][w]);
-              }
-            }
+            for (int n = 0; n < NB; ++n) mma_bf16(acc[n], f, fb[n][0][w], fb[n][1][w]);
           }
         }
       }
-      const bool last = m0 + 16 * MB >= count;
-      if (held && last && next < c_end) fetch(next, 0);
-      if constexpr (kRing) {
-        if (last && next >= c_end) cp_async_wait<0>();
-        else cp_async_wait<1>();
-        __syncwarp();
+    }
+    if (held && c0 + step < c_end) fetch(c0 + step, 0);
+    if constexpr (VEC) {
+      cp_async_wait<1>();
+      const char* from = slots + stage * kStage + lane * kUnit;
 #pragma unroll
-        for (int m = 0; m < MB; ++m)
+      for (int e = 0; e < 2; ++e) {
+        if (!row_ok[e]) continue;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int q = 0; q < NB / 2; ++q) four[m][e][q].load(&ring[warp][turn_of][ring_unit(m * 16 + e * 8 + g, 4 * q + t) * 4]);
-      }
-      if constexpr (VEC) {
-#pragma unroll
-        for (int m = 0; m < MB; ++m)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = m0 + m * 16 + e * 8 + g;
-            if (i >= count) continue;
-            TY* p = out + size_t(rows[i]) * N + c0 + 4 * t;
-#pragma unroll
-            for (int q = 0; q < NB / 2; ++q) {
-              const float d[4] = {acc[m][2 * q][2 * e], acc[m][2 * q][2 * e + 1], acc[m][2 * q + 1][2 * e], acc[m][2 * q + 1][2 * e + 1]};
-              if (c0 + q * 16 + 4 * t < c_end) four[m][e][q].add_store(p + q * 16, d);
-            }
-          }
-      } else {
-        __syncwarp();
-#pragma unroll
-        for (int m = 0; m < MB; ++m)
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              turn[warp][m * 16 + (i >> 1) * 8 + g][(n >> 1) * 16 + 4 * t + 2 * (n & 1) + (i & 1)] = acc[m][n][i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 16 * MB; ++i)
-          if (m0 + i < count) {
-            TY* p = out + size_t(rows[m0 + i]) * N + c0 + lane;
-#pragma unroll
-            for (int q = 0; q < COLS / 32; ++q)
-              if (c0 + q * 32 + lane < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[warp][i][q * 32 + lane]);
+        for (int q = 0; q < NB / 2; ++q)
+          if (c0 + q * 16 + 4 * t < c_end) {
+            AdaptFour<TY> four;
+            four.load(reinterpret_cast<const TY*>(from + (e * (NB / 2) + q) * 32 * kUnit));
+            const float d[4] = {acc[2 * q][2 * e], acc[2 * q][2 * e + 1], acc[2 * q + 1][2 * e], acc[2 * q + 1][2 * e + 1]};
+            four.add_store(op[e] + c0 + q * 16, d);
           }
       }
-      if constexpr (kRing) {
-        __syncwarp();                                      // the tile is read before it is filled again
-        turn_of ^= 1;
-      }
+    } else {
+      float* turn = reinterpret_cast<float*>(slots);       // [16][COLS + 1]
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn[((i >> 1) * 8 + g) * (COLS + 1) + (n >> 1) * 16 + 4 * t + 2 * (n & 1) + (i & 1)] = acc[n][i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (my_rows + i < count) {
+          TY* p = out + size_t(rows[my_rows + i]) * N + c0 + lane;
+#pragma unroll
+          for (int q = 0; q < COLS / 32; ++q)
+            if (c0 + q * 32 + lane < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[i * (COLS + 1) + q * 32 + lane]);
+        }
     }
   }
+  if constexpr (VEC) cp_async_wait<0>();
 }
 
 struct AdaptShape {
@@ -735,7 +715,7 @@ struct AdaptShape {
 };
 
 // Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
-// Splits of K: as many as make two CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a multiple
+// Splits of K: as many as make eight CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a multiple
 // of what its warps take at a time, the more the more tiles there are.
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
   AdaptShape s;
@@ -748,10 +728,10 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.ks = rank <= 16 ? 1 : rank <= 32 || w_pieces > 2 ? 2 : 4;
   const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
-  long long splits = 2LL * sms / ctas;
+  long long splits = 8LL * sms / ctas;
   if (splits > K / 256) splits = K / 256;
   s.splits = int(splits < 1 ? 1 : splits > 16 ? 16 : splits);
-  const int unit = kExpandWarps * 8 * expand_nb(s.ks, s.rt / 16, w_pieces);
+  const int unit = kExpandWarps / (s.rt / 16) * 8 * expand_nb(s.ks, w_pieces);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
   long long per = units * busy / (8LL * sms);            // column units a CTA takes for eight CTAs per SM

@@ -759,29 +759,27 @@ static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& s
   return cudaErrorInvalidValue;
 }
 
-template <typename TY, typename TW, int KS, int MR, bool VEC>
+template <typename TY, typename TW, int KS, bool VEC>
 static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  constexpr int pieces = sizeof(TY) == 2 ? 2 : 3;
+  constexpr int warps = kExpandWarps * expand_warp_bytes<TY, expand_nb(KS, AdaptType<TW>::kPieces), VEC>();
   static bool configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KS, MR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             pieces * 16 * MR * expand_stride(kAdaptMaxRank) * 2);
+    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KS, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             warps + expand_h_bytes<TY>(kAdaptMaxRows / 16, kAdaptMaxRank));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_chained(adapt_expand_kernel<TY, TW, KS, MR, VEC>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
-                        size_t(pieces) * 16 * MR * expand_stride(P.rank) * 2, stream, P);
+  return launch_chained(adapt_expand_kernel<TY, TW, KS, VEC>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
+                        size_t(warps) + expand_h_bytes<TY>(P.rt / 16, P.rank), stream, P);
 }
 
 template <typename TY, typename TW, int KS>
 static cudaError_t launch_adapt_expand_ks(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
-  constexpr int many = kAdaptMaxRows / 16;
-  if (sh.rt == 16) return vec ? launch_adapt_expand_as<TY, TW, KS, 1, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, 1, false>(P, sh, stream);
-  return vec ? launch_adapt_expand_as<TY, TW, KS, many, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, many, false>(P, sh, stream);
+  return vec ? launch_adapt_expand_as<TY, TW, KS, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, false>(P, sh, stream);
 }
 
 template <typename TY, typename TW>
