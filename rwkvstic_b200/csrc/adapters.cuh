@@ -10,7 +10,7 @@
 // Products run on the tensor cores (mma.sync m16n8k16) with fp32 sums.  Operands that are not of one 16-bit type are cut
 // into bfloat16 pieces: a float is exactly three (the upper 8 bits of its significand, the next 8, the last 8), a half
 // exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21 of the whole together and left out.  The tensor cores
-// cut their sums off, so no chain is longer than 64 k before its part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity
+// cut their sums off, so no chain is longer than 64 k of a lane before its part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity
 // or a NaN comes out as NaN, where it has an adapter.
 // What bounds both is memory: h takes rank multiplications per value of x, y takes rank per value.  At rank 64 with fp32 rows
 // that is 48 products of pieces a byte, below what mma.sync sustains beside the loads, so nothing is gained by staging
@@ -47,14 +47,25 @@ struct AdaptParams {
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// d = a b (no sum so far) or d += a b
+template <bool HALF>
+__device__ __forceinline__ void mma_to(bool first, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (first) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = 0.f;
+  }
+  if constexpr (HALF) mma_f16(d, a, b0, b1);
+  else mma_bf16(d, a, b0, b1);
 }
 
 // Elements 2i and 2i + 1 of a lane's, as loaded (16-bit types) or as floats.
@@ -358,23 +369,19 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(co
     for (int q = 0; q < NT; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
+  float part[MT][NT][4];                   // the tensor cores cut their sums off; the running sum rounds, every second stage
+#pragma unroll 2
   for (int c = c0; c < c1; ++c) {
     cp_async_wait<kShrinkStages - 2>();
     __syncthreads();                       // the stage has arrived; everyone is done with the one that is requested next
     request(c + kShrinkStages - 1);
     const char* tx = stages + (c - c0) % kShrinkStages * kBytes;
     const char* ta = tx + kBytesX;
-    float part[MT][NT][4];                 // the tensor cores cut their sums off; the running sum rounds
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < NT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[m][q][i] = 0.f;
+    const bool even = ((c - c0) & 1) == 0;
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
       const int step = 2 * half + o;
-      uint32_t fx[NT][2][PX];
+      uint32_t fx[NT][2][PX], fa[MT][PW][4];
 #pragma unroll
       for (int q = 0; q < NT; ++q) {
         AdaptRaw<TX, 4> f;
@@ -383,36 +390,38 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(co
         f.template pair<PX>(1, fx[q][1]);
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        uint32_t fa[4][PW];
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           AdaptRaw<TW, 4> f;
           StageTile<TW>::read(ta, m * 16 + e * 8 + g, step, t, f);
-          f.template pair<PW>(0, fa[e]);
-          f.template pair<PW>(1, fa[2 + e]);
+          uint32_t lo[PW], hi[PW];
+          f.template pair<PW>(0, lo);
+          f.template pair<PW>(1, hi);
+#pragma unroll
+          for (int i = 0; i < PW; ++i) { fa[m][i][e] = lo[i]; fa[m][i][2 + e] = hi[i]; }
         }
+      bool first = even && o == 0;
 #pragma unroll
-        for (int i = PW - 1; i >= 0; --i) {
-          const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
+      for (int i = PW - 1; i >= 0; --i)
 #pragma unroll
-          for (int j = PX - 1; j >= 0; --j) {
-            if (i + j >= 3) continue;
+        for (int j = PX - 1; j >= 0; --j) {
+          if (i + j >= 3) continue;
 #pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
-              else mma_bf16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
-            }
-          }
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+              mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
+          first = false;
         }
-      }
     }
+    if (!even || c + 1 == c1)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int q = 0; q < NT; ++q)
+        for (int q = 0; q < NT; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
+          for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
   }
   cp_async_wait<0>();
   __syncthreads();                         // the stages become the table of sums
@@ -614,9 +623,14 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < count && j < rank) {
         const float* h = P.h[mat] + size_t(rows[r]) * rank + j;
-        for (int p = 0; p < P.splits; ++p) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(h + size_t(p) * P.R * rank));
-          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        const size_t part = size_t(P.R) * rank;
+        for (int p = 0; p < P.splits; p += 4) {            // four in flight, added in their order
+          float4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[k] = p + k < P.splits ? __ldcg(reinterpret_cast<const float4*>(h + (p + k) * part)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
         }
       }
       uint32_t lo[PH], hi[PH];
@@ -710,13 +724,171 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   if constexpr (VEC) cp_async_wait<0>();
 }
 
+// The same for tiles of 64 rows of one stream, 16-bit weights, ranks up to 64 and rows on boundaries of four elements.  What
+// bounds it then is the traffic of the SM's L1 (272 clocks per 16 x 32 values of the form above, of which fragments of B from
+// global memory 128 and those of h 48): so a warp keeps its 16 rows' fragments of h in registers, and B and y pass through
+// shared memory, copied in whole lines, 64 columns a step and two steps ahead.
+// KS: steps of 16 ranks.
+constexpr int kExpandTileStages = 3, kExpandTileCols = 64;
+template <typename TY, int KS>
+__host__ __device__ constexpr int expand_tile_smem() {
+  return kExpandTileStages * (kExpandTileCols * KS * 32 + kExpandWarps * 16 * 32 * int(sizeof(TY)));
+}
+
+template <typename TY, typename TW, int KS>
+__global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(const AdaptParams P) {
+  constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  constexpr int kPitch = KS * 32, kBytesB = kExpandTileCols * kPitch, kUnit = 4 * int(sizeof(TY)), kBytesY = 16 * 8 * kUnit;
+  constexpr int kStage = kBytesB + kExpandWarps * kBytesY;
+  extern __shared__ __align__(128) char shared[];
+  __shared__ int rows[kAdaptMaxRows];
+  __shared__ uint32_t mask[kAdaptWindow / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  int id = -1;
+  const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
+  int mat = 0;
+  while (mat < P.nmat - 1 && int(blockIdx.y) >= P.chunk_end[mat]) ++mat;
+  const int N = P.n_out[mat], chunk = int(blockIdx.y) - (mat ? P.chunk_end[mat - 1] : 0), rank = P.rank;
+  const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
+  const TY* y = static_cast<const TY*>(P.y[mat]);
+  TY* out = static_cast<TY*>(P.out[mat]);
+  if (id < 0) {
+    if (y != out) adapt_copy<TY, true>(y, out, rows, count, N, c_begin, c_end);
+    return;
+  }
+  const int my_rows = (warp & 3) * 16, my_cols = (warp >> 2) * 32;
+  const size_t row0 = rows[0];
+  // B: a column is a row of kPitch bytes at place_of(column), so that fragment reads (columns 0, 1, 4, 5 of eight by half a warp)
+  // meet no bank twice
+  auto place_of = [](int c) { return (c & ~7) | (c & 1) | ((c >> 1) & 2) | ((c << 1) & 4); };
+  auto turned = [](int place, int unit) { return KS == 4 ? unit ^ ((place & 3) << 1) : KS == 2 ? unit ^ (place & 2) : unit; };
+  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  const bool wide = rank % 8 == 0;                         // rows of B start on 16 bytes, else on 8
+  auto y_unit = [](int row, int unit) { return row * 8 + (unit ^ (sizeof(TY) == 4 ? (row & 1) << 2 : (row & 2) << 1)); };
+  const int yu = lane & 7, yr = lane >> 3;
+  const TY* yp = y + (row0 + my_rows + yr) * N + my_cols + 4 * yu;
+  auto request = [&](int stage, int c0) {
+    if (c0 < c_end) {
+      char* to = shared + stage * kStage;
+      for (int i = tid; i < kExpandTileCols * KS * 2; i += kExpandThreads) {
+        const int c = i / (KS * 2), u = i % (KS * 2), place = place_of(c);
+        if (c0 + c >= c_end) continue;
+        const uint32_t dst = smem_u32(to + place * kPitch + turned(place, u) * 16);
+        const TW* src = b + size_t(c0 + c) * rank + 8 * u;
+        if (wide) {
+          cp_async16(dst, 8 * u < rank ? src : b, 8 * u < rank);
+        } else {
+          cp_async8(dst, 8 * u < rank ? src : b, 8 * u < rank);
+          cp_async8(dst + 8, 8 * u + 4 < rank ? src + 4 : b, 8 * u + 4 < rank);
+        }
+      }
+      const uint32_t dst = smem_u32(to + kBytesB + warp * kBytesY);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (my_rows + yr + 4 * k < count && c0 + my_cols + 4 * yu < c_end) {
+          if constexpr (sizeof(TY) == 4) cp_async16(dst + y_unit(yr + 4 * k, yu) * kUnit, yp + size_t(4 * k) * N + c0, true);
+          else cp_async8(dst + y_unit(yr + 4 * k, yu) * kUnit, yp + size_t(4 * k) * N + c0, true);
+        }
+    }
+    cp_async_commit();                                     // a group per step, also an empty one
+  };
+#pragma unroll
+  for (int i = 0; i < kExpandTileStages - 1; ++i) request(i, c_begin + i * kExpandTileCols);   // none of it comes from the first launch
+  griddep_wait();
+  uint32_t h[KS][PH][4];
+  {
+    const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
+    const size_t part = size_t(P.R) * rank;
+    float4 sum[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sum[s][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < P.splits; ++p)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = my_rows + e * 8 + g, j = s * 16 + 4 * t;
+          if (i >= count || j >= rank) continue;
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + p * part + (row0 + i) * rank + j));
+          sum[s][e].x += v.x; sum[s][e].y += v.y; sum[s][e].z += v.z; sum[s][e].w += v.w;
+        }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t lo[PH], hi[PH];
+        split_pair<PH>(sum[s][e].x * scale, sum[s][e].y * scale, lo);
+        split_pair<PH>(sum[s][e].z * scale, sum[s][e].w * scale, hi);
+#pragma unroll
+        for (int p = 0; p < PH; ++p) { h[s][p][e] = lo[p]; h[s][p][2 + e] = hi[p]; }
+      }
+  }
+  TY* op[2];
+  bool row_ok[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = my_rows + e * 8 + g;
+    row_ok[e] = i < count;
+    op[e] = out + (row0 + (row_ok[e] ? i : 0)) * N + my_cols + 4 * t;
+  }
+  const int place = place_of(4 * (g >> 1) + (g & 1));      // of a lane's column of product 0; that of product n: + (n / 2) * 16 + (n % 2) * 4
+  int stage = 0;
+  for (int c0 = c_begin; c0 < c_end; c0 += kExpandTileCols) {
+    cp_async_wait<kExpandTileStages - 2>();
+    __syncthreads();                                       // the stage has arrived; everyone is done with the one that is requested next
+    const int ahead = stage == 0 ? kExpandTileStages - 1 : stage - 1;
+    request(ahead, c0 + (kExpandTileStages - 1) * kExpandTileCols);
+    const char* from = shared + stage * kStage;
+    float acc[4][4];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t fb[4][2][PW];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int at = place + (n >> 1) * 16 + (n & 1) * 4 + my_cols;
+        const uint2 v = *reinterpret_cast<const uint2*>(from + at * kPitch + turned(at, 2 * s + (t >> 1)) * 16 + (t & 1) * 8);
+        AdaptRaw<TW, 4> raw;
+        raw.w[0] = v.x; raw.w[1] = v.y;
+        raw.template pair<PW>(0, fb[n][0]);
+        raw.template pair<PW>(1, fb[n][1]);
+      }
+      bool first = s == 0;
+#pragma unroll
+      for (int p = PH - 1; p >= 0; --p)
+#pragma unroll
+        for (int w = PW - 1; w >= 0; --w) {
+          if (p + w >= PH) continue;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) mma_to<false>(first, acc[n], h[s][p], fb[n][0][w], fb[n][1][w]);
+          first = false;
+        }
+    }
+    const char* mine = from + kBytesB + warp * kBytesY;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (row_ok[e] && c0 + my_cols + q * 16 + 4 * t < c_end) {
+          AdaptFour<TY> four;
+          four.load(reinterpret_cast<const TY*>(mine + y_unit(e * 8 + g, 4 * q + t) * kUnit));
+          const float d[4] = {acc[2 * q][2 * e], acc[2 * q][2 * e + 1], acc[2 * q + 1][2 * e], acc[2 * q + 1][2 * e + 1]};
+          four.add_store(op[e] + c0 + q * 16, d);
+        }
+    stage = stage == kExpandTileStages - 1 ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+}
+
 struct AdaptShape {
+  bool tiled;                              // the second launch may take its form for 64 rows
   int rt, tiles, splits, mt, ks, chunk_cols, chunks;   // mt: ranks of a CTA of the first launch, ks: of fragments held in the second, in 16
 };
 
 // Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
-// Splits of K: as many as make eight CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a multiple
-// of what its warps take at a time, the more the more tiles there are.
+// Splits of K: as many as make two CTAs per SM (one wave), with 256 or more k each.  Columns of a CTA of the second launch: a
+// multiple of what its warps take at a time, the more the more tiles there are.
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
   AdaptShape s;
   s.rt = T >= kAdaptMaxRows ? kAdaptMaxRows : 16;
@@ -728,14 +900,15 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.ks = rank <= 16 ? 1 : rank <= 32 || w_pieces > 2 ? 2 : 4;
   const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
-  long long splits = 8LL * sms / ctas;
+  long long splits = 2LL * sms / ctas;
   if (splits > K / 256) splits = K / 256;
   s.splits = int(splits < 1 ? 1 : splits > 16 ? 16 : splits);
-  const int unit = kExpandWarps / (s.rt / 16) * 8 * expand_nb(s.ks, w_pieces);
+  s.tiled = s.rt == kAdaptMaxRows && w_pieces < 3 && rank <= 64;
+  const int unit = s.tiled ? kExpandTileCols : kExpandWarps / (s.rt / 16) * 8 * expand_nb(s.ks, w_pieces);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  long long per = units * busy / (8LL * sms);            // column units a CTA takes for eight CTAs per SM
-  s.chunk_cols = unit * int(per < 1 ? 1 : per > 16 ? 16 : per);
+  long long per = units * busy / (6LL * sms);            // column units a CTA takes for six CTAs per SM
+  s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
   s.chunks = 0;
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
   return s;

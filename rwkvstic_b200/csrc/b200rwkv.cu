@@ -782,8 +782,31 @@ static cudaError_t launch_adapt_expand_ks(const AdaptParams& P, const AdaptShape
   return vec ? launch_adapt_expand_as<TY, TW, KS, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, false>(P, sh, stream);
 }
 
+template <typename TY, typename TW, int KS>
+static cudaError_t launch_adapt_expand_tile(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  constexpr int smem = expand_tile_smem<TY, KS>();
+  static bool configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(adapt_expand_tile_kernel<TY, TW, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch_chained(adapt_expand_tile_kernel<TY, TW, KS>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads), smem, stream, P);
+}
+
 template <typename TY, typename TW>
 static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+  if constexpr (sizeof(TW) == 2)
+    if (sh.tiled && vec) switch ((P.rank + 15) / 16) {
+      case 1: return launch_adapt_expand_tile<TY, TW, 1>(P, sh, stream);
+      case 2: return launch_adapt_expand_tile<TY, TW, 2>(P, sh, stream);
+      case 3: return launch_adapt_expand_tile<TY, TW, 3>(P, sh, stream);
+      default: return launch_adapt_expand_tile<TY, TW, 4>(P, sh, stream);
+    }
   if (sh.ks == 1) return launch_adapt_expand_ks<TY, TW, 1>(P, sh, vec, stream);
   if (sh.ks == 2) return launch_adapt_expand_ks<TY, TW, 2>(P, sh, vec, stream);
   if constexpr (AdaptType<TW>::kPieces < 3) return launch_adapt_expand_ks<TY, TW, 4>(P, sh, vec, stream);
