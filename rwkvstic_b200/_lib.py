@@ -146,7 +146,7 @@ def lib() -> C.CDLL:
     L.b200rwkv_adapt_rows_workspace_bytes.restype = C.c_size_t
     L.b200rwkv_adapt_rows_workspace_bytes.argtypes = [C.c_int, C.POINTER(Adapters)] + [C.c_int] * 6
     L.b200rwkv_adapt_rows.restype = C.c_int
-    L.b200rwkv_adapt_rows.argtypes = ([C.c_int, C.POINTER(Adapters)] + [C.c_int] * 4 + [C.POINTER(C.c_void_p)] * 3 +
+    L.b200rwkv_adapt_rows.argtypes = ([C.c_int, C.c_void_p] + [C.c_int] * 4 + [C.c_void_p] * 3 +      # arrays, or their bytes
                                       [C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p])
     L.b200rwkv_verify_drafts_workspace_bytes.restype = C.c_size_t
     L.b200rwkv_verify_drafts_workspace_bytes.argtypes = [C.c_int] * 3

@@ -8,6 +8,9 @@ launch on torch's current stream.  No CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+from contextlib import nullcontext
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -18,6 +21,16 @@ from .quant import QuantMatrix
 
 def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# The operators below are called once per projection or step with a few rows, where the host's share of a call counts: a
+# raw stream handle instead of a stream object, and no change of device where it is the current one already.
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _on(index: int):
+    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _cmatrix(m: QuantMatrix) -> _lib.Matrix:
@@ -233,40 +246,56 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     outs = ys if outs is None else outs
     if n < 1 or n > 3 or len(xs) != n or len(ys) != n or len(outs) != n:
         raise ValueError("adapt_rows takes 1..3 banks and as many inputs and outputs")
-    a0 = banks[0][0]
-    dev, dt, row_dt = a0.device, a0.dtype, xs[0].dtype
-    if dev.type != "cuda":
+    a0, x0 = banks[0][0], xs[0]
+    index, dt, row_dt = a0.get_device(), a0.dtype, x0.dtype
+    if index < 0:
         raise RuntimeError("adapt_rows needs CUDA tensors (no CPU path)")
-    if dt not in _DENSE_DTYPES or row_dt not in (torch.float32, dt):
+    if dt not in _DENSE_DTYPES or (row_dt != torch.float32 and row_dt != dt):
         raise ValueError("adapt_rows needs banks of bf16, fp16 or fp32 and rows of fp32 or the banks' type")
-    if a0.dim() != 3 or xs[0].dim() != 2 or ids.dim() != 1:
+    bank_shape, x_shape = a0.shape, x0.shape
+    if len(bank_shape) != 3 or len(x_shape) != 2 or ids.dim() != 1:
         raise ValueError("adapt_rows needs a [n,rank,k_in], x [rows,k_in] and ids [streams]")
-    count, rank, k_in = a0.shape
-    rows, streams = xs[0].shape[0], ids.shape[0]
-    if ids.dtype != torch.int64 or ids.device != dev or not ids.is_contiguous() or (rows % streams if streams else rows):
+    count, rank, k_in = bank_shape
+    rows, streams = x_shape[0], ids.shape[0]
+    if ids.dtype != torch.int64 or ids.get_device() != index or not ids.is_contiguous() or (rows % streams if streams else rows):
         raise ValueError("ids must be contiguous int64 on the banks' device, one per stream, and the rows a multiple of them")
+    packed, px, py, po, n_out = [], [], [], [], []
     for (a, b, s), x, y, o in zip(banks, xs, ys, outs):
-        if tuple(a.shape) != (count, rank, k_in) or b.dim() != 3 or b.shape[0] != count or b.shape[2] != rank:
+        b_shape = b.shape
+        if a.shape != bank_shape or len(b_shape) != 3 or b_shape[0] != count or b_shape[2] != rank:
             raise ValueError("adapt_rows banks must share n, rank and k_in: a [n,rank,k_in], b [n,n_out,rank]")
-        if a.dtype != dt or b.dtype != dt or not a.is_contiguous() or not b.is_contiguous() or a.device != dev or b.device != dev:
+        if (a.dtype != dt or b.dtype != dt or not a.is_contiguous() or not b.is_contiguous() or a.get_device() != index
+                or b.get_device() != index):
             raise ValueError("adapt_rows banks must be contiguous, of one type, on one device")
-        if s is not None and (s.dtype != torch.float32 or s.device != dev or tuple(s.shape) != (count,) or not s.is_contiguous()):
+        if s is not None and (s.dtype != torch.float32 or s.get_device() != index or s.shape != (count,) or not s.is_contiguous()):
             raise ValueError("an adapter bank's scale must be contiguous fp32 [n] on its device")
-        for t, shape in ((x, (rows, k_in)), (y, (rows, b.shape[1])), (o, (rows, b.shape[1]))):
-            if tuple(t.shape) != shape or t.dtype != row_dt or t.device != dev or not t.is_contiguous():
-                raise ValueError("adapt_rows rows must be contiguous, of one type, on the banks' device, and match their bank")
+        y_shape = (rows, b_shape[1])
+        if (x.shape != (rows, k_in) or y.shape != y_shape or x.dtype != row_dt or y.dtype != row_dt or x.get_device() != index
+                or y.get_device() != index or not x.is_contiguous() or not y.is_contiguous()):
+            raise ValueError("adapt_rows rows must be contiguous, of one type, on the banks' device, and match their bank")
+        if o is not y and (o.shape != y_shape or o.dtype != row_dt or o.get_device() != index or not o.is_contiguous()):
+            raise ValueError("adapt_rows outputs must be contiguous, of the rows' type and shape, on the banks' device")
+        packed += (a.data_ptr(), b.data_ptr(), 0 if s is None else s.data_ptr(), b_shape[1])
+        px.append(x.data_ptr()); py.append(y.data_ptr()); po.append(o.data_ptr()); n_out.append(b_shape[1])
     if rows == 0:
         return list(outs)
-    cb = (_lib.Adapters * n)(*[_lib.Adapters(a.data_ptr(), b.data_ptr(), _lib.ptr(s), b.shape[1]) for a, b, s in banks])
-    cx, cy, co = ((C.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (xs, ys, outs))
+    # the C side's arrays as bytes: b200rwkv_adapters (three pointers, an int32 and its padding) and pointers
+    banks_c, pointers = struct.pack("=" + "QQQi4x" * n, *packed), "=%dQ" % n
     shape = (count, rank, k_in, _DENSE_DTYPES[dt])
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        nbytes = int(L.b200rwkv_adapt_rows_workspace_bytes(n, cb, *shape, streams, rows // streams))
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-        _lib.check(L.b200rwkv_adapt_rows(n, cb, *shape, cx, cy, co, _DENSE_DTYPES[row_dt], ids.data_ptr(), streams, rows // streams,
-                                         ws.data_ptr(), ws.numel(), _stream(dev)))
+    with _on(index):
+        ws = torch.empty(_adapt_workspace(index, tuple(n_out), *shape, streams, rows // streams), dtype=torch.uint8, device=a0.device)
+        _lib.check(_lib.lib().b200rwkv_adapt_rows(n, banks_c, *shape, struct.pack(pointers, *px), struct.pack(pointers, *py),
+                                                  struct.pack(pointers, *po), _DENSE_DTYPES[row_dt], ids.data_ptr(), streams,
+                                                  rows // streams, ws.data_ptr(), ws.numel(), _raw_stream(index)))
     return list(outs)
+
+
+@lru_cache(maxsize=1024)
+def _adapt_workspace(index: int, n_out: Tuple[int, ...], count: int, rank: int, k_in: int, dtype: int, streams: int, tokens: int) -> int:
+    """Bytes of scratch for a call of this shape on this device (the current one); a refused shape gets a few, for the call to
+    say why."""
+    banks = (_lib.Adapters * len(n_out))(*[_lib.Adapters(None, None, None, o) for o in n_out])
+    return max(256, int(_lib.lib().b200rwkv_adapt_rows_workspace_bytes(len(n_out), banks, count, rank, k_in, dtype, streams, tokens)))
 
 
 def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, u: torch.Tensor,
@@ -281,32 +310,40 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     ``u_t q_t/Q_t < p_t/P_t``; the first refused one is replaced by a draw from ``max(0, p/P - q/Q)``, and where none is,
     one more is drawn from the target's next row.  Returns int64 ``[B,K+1]`` (the accepted tokens, the drawn one, -1
     behind it) and the number accepted, int64 ``[B]``.  Rows must be contiguous; streams and rows may be strided."""
-    if target.dim() != 3 or tokens.dim() != 2 or target.dtype != torch.float32 or target.device.type != "cuda":
+    index = target.get_device()
+    if target.dim() != 3 or tokens.dim() != 2 or target.dtype != torch.float32 or index < 0:
         raise ValueError("verify_drafts needs fp32 CUDA weights [B,K+1,V] and tokens [B,K]")
-    dev = target.device
     (B, K), V = tokens.shape, target.shape[2]
-    if tuple(target.shape) != (B, K + 1, V) or (V > 1 and target.stride(2) != 1):
+    t_stream, t_row, t_step = target.stride()
+    if target.shape != (B, K + 1, V) or (V > 1 and t_step != 1):
         raise ValueError(f"target must be [{B},{K + 1},V] with contiguous rows, got {tuple(target.shape)}")
-    if draft is not None and (tuple(draft.shape) != (B, K, V) or draft.dtype != torch.float32 or draft.device != dev or (V > 1 and draft.stride(2) != 1)):
-        raise ValueError(f"draft must be fp32 [{B},{K},{V}] with contiguous rows on the target's device")
-    if tokens.dtype != torch.int64 or tokens.device != dev or not tokens.is_contiguous():
+    d_ptr, d_stream, d_row = None, 0, 0
+    if draft is not None:
+        if draft.shape != (B, K, V) or draft.dtype != torch.float32 or draft.get_device() != index or (V > 1 and draft.stride(2) != 1):
+            raise ValueError(f"draft must be fp32 [{B},{K},{V}] with contiguous rows on the target's device")
+        d_ptr, (d_stream, d_row, _) = draft.data_ptr(), draft.stride()
+    if tokens.dtype != torch.int64 or tokens.get_device() != index or not tokens.is_contiguous():
         raise ValueError("tokens must be contiguous int64 on the target's device")
-    if u.dtype != torch.float32 or u.device != dev or tuple(u.shape) != (B, K + 1) or not u.is_contiguous():
+    if u.dtype != torch.float32 or u.get_device() != index or u.shape != (B, K + 1) or not u.is_contiguous():
         raise ValueError(f"u must be contiguous fp32 [{B},{K + 1}] on the target's device")
-    if lengths is not None and (lengths.dtype != torch.int64 or lengths.device != dev or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
+    if lengths is not None and (lengths.dtype != torch.int64 or lengths.get_device() != index or lengths.shape != (B,) or not lengths.is_contiguous()):
         raise ValueError(f"lengths must be contiguous int64 [{B}] on the target's device")
-    out = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
-    accepted = torch.empty(B, dtype=torch.int64, device=dev)
+    device = target.device
+    out = torch.empty((B, K + 1), dtype=torch.int64, device=device)
+    accepted = torch.empty(B, dtype=torch.int64, device=device)
     if B == 0:
         return out, accepted
-    L = _lib.lib()
-    ds = (0, 0) if draft is None else draft.stride()[:2]
-    with torch.cuda.device(dev):
-        ws = torch.empty(max(int(L.b200rwkv_verify_drafts_workspace_bytes(B, K, V)), 8), dtype=torch.uint8, device=dev)
-        _lib.check(L.b200rwkv_verify_drafts(target.data_ptr(), target.stride(0), target.stride(1), _lib.ptr(draft), ds[0], ds[1],
-                                            tokens.data_ptr(), u.data_ptr(), _lib.ptr(lengths), B, K, V, out.data_ptr(),
-                                            accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+    with _on(index):
+        ws = torch.empty(_verify_workspace(B, K, V), dtype=torch.uint8, device=device)
+        _lib.check(_lib.lib().b200rwkv_verify_drafts(target.data_ptr(), t_stream, t_row, d_ptr, d_stream, d_row, tokens.data_ptr(),
+                                                     u.data_ptr(), None if lengths is None else lengths.data_ptr(), B, K, V, out.data_ptr(),
+                                                     accepted.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(index)))
     return out, accepted
+
+
+@lru_cache(maxsize=1024)
+def _verify_workspace(B: int, K: int, V: int) -> int:
+    return max(8, int(_lib.lib().b200rwkv_verify_drafts_workspace_bytes(B, K, V)))
 
 
 def advance_state(state: torch.Tensor, counts: torch.Tensor, trace: torch.Tensor, params: torch.Tensor,
@@ -317,22 +354,22 @@ def advance_state(state: torch.Tensor, counts: torch.Tensor, trace: torch.Tensor
     stream in front of ln1, in front of ln2, the key and the value; ``params`` fp32 ``[L,5,C]``: ln1 weight and bias, ln2
     weight and bias, ``-exp(time_decay)``.  Carries become the layer norms of the last accepted token, the WKV sums take
     ``counts[b]`` steps (agnosticRwkv.py:68-103).  In place when ``out`` is omitted; returns the new state."""
-    out = state if out is None else out
-    if state.dim() != 4 or state.shape[2] != 5 or trace.dim() != 5:
+    index, shape = state.get_device(), state.shape
+    if len(shape) != 4 or shape[2] != 5 or trace.dim() != 5:
         raise ValueError("advance_state needs state [B,L,5,C] and trace [L,4,B,T,C]")
-    B, L, _, Cc = state.shape
+    B, L, _, Cc = shape
     T = trace.shape[3]
-    shapes = ((state, (B, L, 5, Cc)), (out, (B, L, 5, Cc)), (trace, (L, 4, B, T, Cc)), (params, (L, 5, Cc)))
-    for t, shape in shapes:
-        if t.dtype != torch.float32 or t.device != state.device or t.device.type != "cuda" or tuple(t.shape) != shape or not t.is_contiguous():
+    out = state if out is None else out
+    for t, want in ((state, shape), (out, shape), (trace, (L, 4, B, T, Cc)), (params, (L, 5, Cc))):
+        if t.dtype != torch.float32 or index < 0 or t.get_device() != index or t.shape != want or not t.is_contiguous():
             raise ValueError("advance_state needs contiguous fp32 CUDA tensors: state and out [B,L,5,C], trace [L,4,B,T,C], params [L,5,C]")
-    if counts.dtype != torch.int64 or counts.device != state.device or tuple(counts.shape) != (B,) or not counts.is_contiguous():
+    if counts.dtype != torch.int64 or counts.get_device() != index or counts.shape != (B,) or not counts.is_contiguous():
         raise ValueError(f"counts must be contiguous int64 [{B}] on the state's device")
     if B == 0 or T == 0:
-        return out if out.data_ptr() == state.data_ptr() else out.copy_(state)
-    with torch.cuda.device(state.device):
+        return out if out is state else out.copy_(state)
+    with _on(index):
         _lib.check(_lib.lib().b200rwkv_advance_state(state.data_ptr(), out.data_ptr(), counts.data_ptr(), trace.data_ptr(), params.data_ptr(),
-                                                     B, L, T, Cc, _stream(state.device)))
+                                                     B, L, T, Cc, _raw_stream(index)))
     return out
 
 
