@@ -354,7 +354,7 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
  *   x, y, out device [streams * tokens_per_stream][k_in] and [...][n_out_i] of row_dtype (f32, or the weights' type), x
  *             16-byte aligned; out_i may be y_i and overlaps nothing else.  Rows <= 65535
  *   ids       device int64 [streams], read on the device (a captured call follows them)
- *   workspace b200rwkv_adapt_rows_workspace_bytes(...) (0: a size that is not taken, or no device), 256-byte aligned; nothing
+ *   workspace b200rwkv_adapt_rows_workspace_bytes(...) (0: a size that is not taken), 256-byte aligned; nothing
  *             is kept in it between calls
  * Sums are f32 over exact products of 16-bit pieces, h = x A^T stays f32, and out is rounded once.  Sums go over fixed parts
  * in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row of x that holds an infinity or a NaN comes out as NaN where it has an

@@ -18,6 +18,7 @@
 // and is, so that a lane's elements are consecutive: 16 bytes of A, 8 of B.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -31,15 +32,16 @@ constexpr int kAdaptMaxMats = 3;
 constexpr int kAdaptWindow = 1024;         // streams
 constexpr int kAdaptMaxRank = 256;
 constexpr int kAdaptMaxRows = 64;          // of a tile
+constexpr int kAdaptMaxSplits = 8;         // of K: a cluster of CTAs
 constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
-constexpr int kShrinkChunk = 64, kShrinkStages = 4;   // k of a stage of the tiled form
+constexpr int kShrinkChunk = 64;           // k of a stage of the tiled form
 constexpr int kExpandThreads = 256, kExpandWarps = kExpandThreads / 32;
 
 struct AdaptParams {
   const void *a[kAdaptMaxMats], *b[kAdaptMaxMats], *x[kAdaptMaxMats], *y[kAdaptMaxMats];
   void* out[kAdaptMaxMats];
   const float* scale[kAdaptMaxMats];       // null: 1
-  float* h[kAdaptMaxMats];                 // [splits][rows][rank]
+  float* h[kAdaptMaxMats];                 // [rows][rank]
   int n_out[kAdaptMaxMats];
   int chunk_end[kAdaptMaxMats];            // second launch: column chunks of the matrices up to and including this one
   const long long* ids;
@@ -61,11 +63,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 template <bool HALF>
 __device__ __forceinline__ void mma_to(bool first, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (first) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = 0.f;
+    if constexpr (HALF)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  } else if constexpr (HALF) {
+    mma_f16(d, a, b0, b1);
+  } else {
+    mma_bf16(d, a, b0, b1);
   }
-  if constexpr (HALF) mma_f16(d, a, b0, b1);
-  else mma_bf16(d, a, b0, b1);
 }
 
 // Elements 2i and 2i + 1 of a lane's, as loaded (16-bit types) or as floats.
@@ -169,12 +177,38 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
   return n;
 }
 
-// h[split][row][j] = sum over the split's K of x[row][k] A[id][j][k].  Grid (tiles, rank chunks of 16 * MT, matrices * splits).
+// h[row][j] = sum_k x[row][k] A[id][j][k].  Grid (tiles * splits of K, rank chunks of 16 * MT, matrices); the CTAs of a tile's
+// splits are a cluster, whose sums meet in shared memory, in the order of the splits.
 // For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter: from global memory to
 // registers.  A warp takes every eighth block of 32 k of the split.
+template <typename Put>
+__device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_sums, int n, Put put) {
+  const int S = P.splits;
+  if (S == 1) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kShrinkThreads) put(i, part_sums[i]);
+    return;
+  }
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = int(cluster.block_rank());
+  cluster.sync();
+  // every CTA adds up a part of the table; all of a thread's remote reads are in flight at once
+  for (int i = rank * kShrinkThreads + threadIdx.x; i < n; i += S * kShrinkThreads) {
+    float v[kAdaptMaxSplits];
+#pragma unroll
+    for (int c = 0; c < kAdaptMaxSplits; ++c) v[c] = c < S ? *cluster.map_shared_rank(part_sums + i, c) : 0.f;
+    float s = v[0];
+#pragma unroll
+    for (int c = 1; c < kAdaptMaxSplits; ++c) s += v[c];
+    put(i, s);
+  }
+  cluster.sync();                          // the tables are read before their CTAs leave
+}
+
 template <typename TX, typename TW, int MT, int NT>
 __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int mat, int split, int chunk, const int* rows,
-                                            int count, float* red) {
+                                            int count, float* red, float* part_sums) {
   constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
   constexpr int RC = 16 * MT, kStride = RC + 4;
@@ -273,47 +307,41 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 #pragma unroll
       for (int i = 0; i < 4; ++i) mine[(q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = sum[m][q][i];
   __syncthreads();
-  float* h = P.h[mat] + size_t(split) * P.R * rank;
   for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
     const int r = i / RC, j = i - r * RC;
-    if (chunk * RC + j >= rank) continue;
     float s = 0.f;
     for (int w = 0; w < kShrinkWarps; ++w) s += red[(w * 16 + r) * kStride + j];
-    h[size_t(rows[r]) * rank + chunk * RC + j] = s;
+    part_sums[i] = s;
   }
+  shrink_join(P, part_sums, count * RC, [&](int i, float s) {
+    const int r = i / RC, j = chunk * RC + i - r * RC;
+    if (j < rank) P.h[mat][size_t(rows[r]) * rank + j] = s;
+  });
 }
 
 template <typename TX, typename TW, int MT>
 __global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const AdaptParams P) {
   __shared__ float red[kShrinkWarps * 16 * (16 * MT + 4)];
+  __shared__ float part_sums[16 * 16 * MT];
   __shared__ int rows[kAdaptMaxRows];
   __shared__ uint32_t mask[kAdaptWindow / 32];
   griddep_launch_dependents();
   int id = -1;
-  const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
-  if (count == 0 || id < 0) return;
-  const int mat = blockIdx.z / P.splits, split = blockIdx.z - mat * P.splits;
+  const int tile = blockIdx.x / P.splits, split = blockIdx.x - tile * P.splits, mat = blockIdx.z;
+  const int count = adapt_tile(P, tile, rows, mask, &id);
+  if (count == 0 || id < 0) return;        // the whole cluster
   const TX* x = static_cast<const TX*>(P.x[mat]);
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
-  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, red);
-  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, red);
+  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, red, part_sums);
+  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, red, part_sums);
 }
 
-// The same for tiles of 64 rows of one stream: x and A are staged in shared memory, 64 k at a time, four stages ahead of the
-// products.  Four warps take 16 rows each, for one half of a stage's k; four more the other half.
+// The same for tiles of 64 rows of one stream: x and A are staged in shared memory, 64 k at a time, several stages ahead of
+// the products.  Four warps take 16 rows each, for one half of a stage's k; four more the other half.
 template <typename T>
 struct StageTile {                         // 64 elements of each row, in 16-byte units dealt out so that fragment reads meet no bank twice
   static constexpr int kUnits = kShrinkChunk * int(sizeof(T)) / 16, kRowBytes = kUnits * 16;
   __device__ static __forceinline__ int swizzle(int row, int unit) { return sizeof(T) == 2 ? unit ^ ((row & 3) << 1) : unit ^ ((row & 1) << 2); }
-  // rows of `ld` elements at src, those below `rows`, from element k (of `end`) on
-  template <int R>
-  __device__ static __forceinline__ void request(uint32_t dst, const T* src, int rows, size_t ld, int k, int end) {
-    for (int i = threadIdx.x; i < R * kUnits; i += kShrinkThreads) {
-      const int r = i / kUnits, u = i % kUnits, at = k + u * (16 / int(sizeof(T)));
-      const bool ok = r < rows && at < end;
-      cp_async16(dst + r * kRowBytes + swizzle(r, u) * 16, src + (ok ? size_t(r) * ld + at : 0), ok);
-    }
-  }
   // elements 16 step + 4 t .. + 3 of a row
   __device__ static __forceinline__ void read(const char* tile, int row, int step, int t, AdaptRaw<T, 4>& f) {
     if constexpr (sizeof(T) == 2) {
@@ -326,10 +354,47 @@ struct StageTile {                         // 64 elements of each row, in 16-byt
   }
 };
 
+// What one thread copies of every stage of R rows: the same units of rows kThreadRows apart, 64 elements further each time.
+template <typename T, int R>
+struct StageCopy {
+  static constexpr int kThreadRows = kShrinkThreads / StageTile<T>::kUnits, kCopies = R / kThreadRows > 0 ? R / kThreadRows : 1;
+  const T* src;                            // of the first copy, in the next stage
+  size_t hop;                              // kThreadRows rows
+  uint32_t dst;                            // in stage 0 (the swizzle of a row kThreadRows further is the same)
+  int k, rows;                             // element of the next stage's copies; copies of rows that exist
+  __device__ __forceinline__ StageCopy(const T* base, uint32_t tile, int have, size_t ld, int k0) {
+    const int r = int(threadIdx.x) / StageTile<T>::kUnits, u = int(threadIdx.x) % StageTile<T>::kUnits;
+    k = k0 + u * (16 / int(sizeof(T)));
+    src = base + (r < have ? r : 0) * ld + k;
+    hop = kThreadRows * ld;
+    dst = tile + r * StageTile<T>::kRowBytes + StageTile<T>::swizzle(r, u) * 16;
+    rows = r < R ? (have - r + kThreadRows - 1) / kThreadRows : 0;
+    if (rows < 0) rows = 0;
+  }
+  // into the stage at `at` bytes; past `end` zeros
+  __device__ __forceinline__ void next(uint32_t at, int end) {
+    const bool in = k < end;
+    const T* from = in ? src : src - k;    // an address that may be read
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      if (R >= kThreadRows || int(threadIdx.x) < R * StageTile<T>::kUnits)
+        cp_async16(dst + at + i * kThreadRows * StageTile<T>::kRowBytes, i < rows ? from + i * hop : from, in && i < rows);
+    src += kShrinkChunk;
+    k += kShrinkChunk;
+  }
+};
+
+// stages: as many as half an SM's shared memory holds
+template <typename TX, typename TW, int MT>
+__host__ __device__ constexpr int shrink_stages() {
+  const int n = 110 * 1024 / (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
+  return n > 8 ? 8 : n;
+}
+
 template <typename TX, typename TW, int MT>
 constexpr int shrink_tile_smem() {
-  const int stages = kShrinkStages * (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
-  const int sums = kShrinkWarps * 16 * (16 * MT + 4) * 4;
+  const int stages = shrink_stages<TX, TW, MT>() * (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
+  const int sums = (kShrinkWarps * 16 * (16 * MT + 4) + kAdaptMaxRows * 16 * MT) * 4;
   return stages > sums ? stages : sums;
 }
 
@@ -337,31 +402,35 @@ template <typename TX, typename TW, int MT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(const AdaptParams P) {
   constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
-  constexpr int RC = 16 * MT, kStride = RC + 4, NT = 2;
+  constexpr int RC = 16 * MT, kStride = RC + 4, NT = 2, kShrinkStages = shrink_stages<TX, TW, MT>();
   constexpr int kBytesX = kAdaptMaxRows * StageTile<TX>::kRowBytes, kBytes = kBytesX + RC * StageTile<TW>::kRowBytes;
   extern __shared__ __align__(128) char stages[];
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int per = (P.T + kAdaptMaxRows - 1) / kAdaptMaxRows, s = blockIdx.x / per, first = (blockIdx.x - s * per) * kAdaptMaxRows;
+  const int tile = blockIdx.x / P.splits, split = blockIdx.x - tile * P.splits, mat = blockIdx.z;
+  const int per = (P.T + kAdaptMaxRows - 1) / kAdaptMaxRows, s = tile / per, first = (tile - s * per) * kAdaptMaxRows;
   const int count = min(kAdaptMaxRows, P.T - first), row0 = s * P.T + first, K = P.K, rank = P.rank;
   const long long asked = __ldg(P.ids + s);
-  if (asked < 0 || asked >= P.adapters) return;
-  const int mat = blockIdx.z / P.splits, split = blockIdx.z - mat * P.splits, j0 = blockIdx.y * RC, ranks = min(RC, rank - j0);
+  if (asked < 0 || asked >= P.adapters) return;            // the whole cluster
+  const int j0 = blockIdx.y * RC, ranks = min(RC, rank - j0);
   const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
   const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
   const int chunks = (K + kShrinkChunk - 1) / kShrinkChunk, c0 = int((long long)chunks * split / P.splits), c1 = int((long long)chunks * (split + 1) / P.splits);
   const uint32_t base = smem_u32(stages);
-  auto request = [&](int c) {
-    if (c < c1) {
-      const uint32_t at = base + (c - c0) % kShrinkStages * kBytes;
-      StageTile<TX>::template request<kAdaptMaxRows>(at, x, count, K, c * kShrinkChunk, K);
-      StageTile<TW>::template request<RC>(at + kBytesX, a, ranks, K, c * kShrinkChunk, K);
-    }
-    cp_async_commit();                     // a group per stage, also an empty one
+  StageCopy<TX, kAdaptMaxRows> copy_x(x, base, count, K, c0 * kShrinkChunk);
+  StageCopy<TW, RC> copy_a(a, base + kBytesX, ranks, K, c0 * kShrinkChunk);
+  const int end = min(K, c1 * kShrinkChunk);
+  uint32_t to = 0;                         // the stage that is filled next, in bytes
+  auto request = [&] {
+    copy_x.next(to, end);
+    copy_a.next(to, end);
+    cp_async_commit();
+    to = to == (kShrinkStages - 1) * kBytes ? 0 : to + kBytes;
   };
 #pragma unroll
-  for (int i = 0; i < kShrinkStages - 1; ++i) request(c0 + i);
+  for (int i = 0; i < kShrinkStages - 1; ++i) request();
   const int my_rows = (warp & 3) * 16, half = warp >> 2;
+  const char* from = stages;               // the stage that is read
   float sum[MT][NT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -369,59 +438,59 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(co
     for (int q = 0; q < NT; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
-  float part[MT][NT][4];                   // the tensor cores cut their sums off; the running sum rounds, every second stage
-#pragma unroll 2
-  for (int c = c0; c < c1; ++c) {
-    cp_async_wait<kShrinkStages - 2>();
-    __syncthreads();                       // the stage has arrived; everyone is done with the one that is requested next
-    request(c + kShrinkStages - 1);
-    const char* tx = stages + (c - c0) % kShrinkStages * kBytes;
-    const char* ta = tx + kBytesX;
-    const bool even = ((c - c0) & 1) == 0;
+  for (int c = c0; c < c1; c += 2) {       // two stages; one past the end holds zeros
+    float part[MT][NT][4];                 // the tensor cores cut their sums off; the running sum rounds
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int step = 2 * half + o;
-      uint32_t fx[NT][2][PX], fa[MT][PW][4];
+    for (int pair = 0; pair < 2; ++pair) {
+      cp_async_wait<kShrinkStages - 2>();
+      __syncthreads();                     // the stage has arrived; everyone is done with the one that is requested next
+      request();
+      const char *tx = from, *ta = from + kBytesX;
+      from = from == stages + (kShrinkStages - 1) * kBytes ? stages : from + kBytes;
 #pragma unroll
-      for (int q = 0; q < NT; ++q) {
-        AdaptRaw<TX, 4> f;
-        StageTile<TX>::read(tx, my_rows + q * 8 + g, step, t, f);
-        f.template pair<PX>(0, fx[q][0]);
-        f.template pair<PX>(1, fx[q][1]);
+      for (int o = 0; o < 2; ++o) {
+        const int step = 2 * half + o;
+        uint32_t fx[NT][2][PX], fa[MT][PW][4];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+          AdaptRaw<TX, 4> f;
+          StageTile<TX>::read(tx, my_rows + q * 8 + g, step, t, f);
+          f.template pair<PX>(0, fx[q][0]);
+          f.template pair<PX>(1, fx[q][1]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            AdaptRaw<TW, 4> f;
+            StageTile<TW>::read(ta, m * 16 + e * 8 + g, step, t, f);
+            uint32_t lo[PW], hi[PW];
+            f.template pair<PW>(0, lo);
+            f.template pair<PW>(1, hi);
+#pragma unroll
+            for (int i = 0; i < PW; ++i) { fa[m][i][e] = lo[i]; fa[m][i][2 + e] = hi[i]; }
+          }
+        bool first = pair == 0 && o == 0;
+#pragma unroll
+        for (int i = PW - 1; i >= 0; --i)
+#pragma unroll
+          for (int j = PX - 1; j >= 0; --j) {
+            if (i + j >= 3) continue;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int q = 0; q < NT; ++q)
+                mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
+            first = false;
+          }
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          AdaptRaw<TW, 4> f;
-          StageTile<TW>::read(ta, m * 16 + e * 8 + g, step, t, f);
-          uint32_t lo[PW], hi[PW];
-          f.template pair<PW>(0, lo);
-          f.template pair<PW>(1, hi);
-#pragma unroll
-          for (int i = 0; i < PW; ++i) { fa[m][i][e] = lo[i]; fa[m][i][2 + e] = hi[i]; }
-        }
-      bool first = even && o == 0;
-#pragma unroll
-      for (int i = PW - 1; i >= 0; --i)
-#pragma unroll
-        for (int j = PX - 1; j >= 0; --j) {
-          if (i + j >= 3) continue;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int q = 0; q < NT; ++q)
-              mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
-          first = false;
-        }
     }
-    if (!even || c + 1 == c1)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int q = 0; q < NT; ++q)
+      for (int q = 0; q < NT; ++q)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
+        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
   }
   cp_async_wait<0>();
   __syncthreads();                         // the stages become the table of sums
@@ -433,11 +502,16 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(co
 #pragma unroll
       for (int i = 0; i < 4; ++i) red[(warp * 16 + q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = sum[m][q][i];
   __syncthreads();
-  float* h = P.h[mat] + (size_t(split) * P.R + row0) * rank + j0;
+  float* part_sums = red + kShrinkWarps * 16 * kStride;
   for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
     const int r = i / RC, j = i - r * RC;
-    if (j < ranks) h[size_t(r) * rank + j] = red[r * kStride + j] + red[(64 + r) * kStride + j];
+    part_sums[i] = red[r * kStride + j] + red[(64 + r) * kStride + j];
   }
+  float* h = P.h[mat] + size_t(row0) * rank + j0;
+  shrink_join(P, part_sums, count * RC, [&](int i, float v) {
+    const int r = i / RC, j = i - r * RC;
+    if (j < ranks) h[size_t(r) * rank + j] = v;
+  });
 }
 
 template <typename TY>
@@ -622,16 +696,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
       const int r = i / r4, j4 = i - r * r4, j = j4 * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < count && j < rank) {
-        const float* h = P.h[mat] + size_t(rows[r]) * rank + j;
-        const size_t part = size_t(P.R) * rank;
-        for (int p = 0; p < P.splits; p += 4) {            // four in flight, added in their order
-          float4 v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            v[k] = p + k < P.splits ? __ldcg(reinterpret_cast<const float4*>(h + (p + k) * part)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
-        }
+        s = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(rows[r]) * rank + j));
       }
       uint32_t lo[PH], hi[PH];
       split_pair<PH>(s.x * scale, s.y * scale, lo);
@@ -762,58 +827,73 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(co
   // meet no bank twice
   auto place_of = [](int c) { return (c & ~7) | (c & 1) | ((c >> 1) & 2) | ((c << 1) & 4); };
   auto turned = [](int place, int unit) { return KS == 4 ? unit ^ ((place & 3) << 1) : KS == 2 ? unit ^ (place & 2) : unit; };
-  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
   const bool wide = rank % 8 == 0;                         // rows of B start on 16 bytes, else on 8
+  // what a thread copies each step: a 16-byte unit (KS 1: for half of the threads) of one column of B, or of two, and four units of y
+  constexpr int kUnitsB = KS * 2, kColsAtOnce = KS == 3 ? 32 : kExpandThreads / kUnitsB < kExpandTileCols ? kExpandThreads / kUnitsB : kExpandTileCols;
+  const int bu = tid % kUnitsB, bc = tid / kUnitsB;
+  const bool b_mine = bc < kColsAtOnce && 8 * bu < rank;
+  const bool b_half = 8 * bu + 4 < rank;                   // not wide: the second half exists
+  const TW* bp = static_cast<const TW*>(P.b[mat]) + (size_t(id) * N + c_begin + (bc < kColsAtOnce ? bc : 0)) * rank + 8 * bu;
+  auto b_at = [&](int c) { return place_of(c) * kPitch + turned(place_of(c), bu) * 16; };
   auto y_unit = [](int row, int unit) { return row * 8 + (unit ^ (sizeof(TY) == 4 ? (row & 1) << 2 : (row & 2) << 1)); };
   const int yu = lane & 7, yr = lane >> 3;
-  const TY* yp = y + (row0 + my_rows + yr) * N + my_cols + 4 * yu;
-  auto request = [&](int stage, int c0) {
-    if (c0 < c_end) {
-      char* to = shared + stage * kStage;
-      for (int i = tid; i < kExpandTileCols * KS * 2; i += kExpandThreads) {
-        const int c = i / (KS * 2), u = i % (KS * 2), place = place_of(c);
-        if (c0 + c >= c_end) continue;
-        const uint32_t dst = smem_u32(to + place * kPitch + turned(place, u) * 16);
-        const TW* src = b + size_t(c0 + c) * rank + 8 * u;
-        if (wide) {
-          cp_async16(dst, 8 * u < rank ? src : b, 8 * u < rank);
-        } else {
-          cp_async8(dst, 8 * u < rank ? src : b, 8 * u < rank);
-          cp_async8(dst + 8, 8 * u + 4 < rank ? src + 4 : b, 8 * u + 4 < rank);
+  const TY* yp = y + (row0 + my_rows + (my_rows < count ? min(yr, count - 1 - my_rows) : -my_rows)) * N + c_begin + my_cols + 4 * yu;
+  const int y_rows = (count - my_rows - yr + 3) / 4;       // of the four
+  const size_t y_hop = size_t(4) * N;
+  const uint32_t base = smem_u32(shared), y_to = base + kBytesB + warp * kBytesY + y_unit(yr, yu) * kUnit;
+  // a row four further has the same place among the banks (fp32: rows mod 2, 16 bits: row & 2)
+  int ask = c_begin;                                       // the columns that are requested next
+  uint32_t to = 0;                                         // and the stage they go to, in bytes
+  auto request = [&] {
+    if (ask < c_end) {
+#pragma unroll
+      for (int k = 0; k < kExpandTileCols / kColsAtOnce; ++k) {
+        const int c = bc + k * kColsAtOnce;
+        if (b_mine && ask + c < c_end) {
+          const uint32_t dst = base + to + b_at(c);
+          const TW* src = bp + size_t(k * kColsAtOnce) * rank;
+          if (wide) {
+            cp_async16(dst, src, true);
+          } else {
+            cp_async8(dst, src, true);
+            cp_async8(dst + 8, b_half ? src + 4 : src, b_half);
+          }
         }
       }
-      const uint32_t dst = smem_u32(to + kBytesB + warp * kBytesY);
+      if (ask + my_cols + 4 * yu < c_end) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (my_rows + yr + 4 * k < count && c0 + my_cols + 4 * yu < c_end) {
-          if constexpr (sizeof(TY) == 4) cp_async16(dst + y_unit(yr + 4 * k, yu) * kUnit, yp + size_t(4 * k) * N + c0, true);
-          else cp_async8(dst + y_unit(yr + 4 * k, yu) * kUnit, yp + size_t(4 * k) * N + c0, true);
-        }
+        for (int k = 0; k < 4; ++k)
+          if (k < y_rows) {
+            if constexpr (sizeof(TY) == 4) cp_async16(y_to + to + k * 4 * 8 * kUnit, yp + k * y_hop, true);
+            else cp_async8(y_to + to + k * 4 * 8 * kUnit, yp + k * y_hop, true);
+          }
+      }
+      ask += kExpandTileCols;
+      bp += size_t(kExpandTileCols) * rank;
+      yp += kExpandTileCols;
     }
     cp_async_commit();                                     // a group per step, also an empty one
+    to = to == (kExpandTileStages - 1) * kStage ? 0 : to + kStage;
   };
+  if (rank < 16 * KS && 8 * bu >= rank && bc < kColsAtOnce)   // ranks that do not exist: zeros, once
 #pragma unroll
-  for (int i = 0; i < kExpandTileStages - 1; ++i) request(i, c_begin + i * kExpandTileCols);   // none of it comes from the first launch
+    for (int k = 0; k < kExpandTileCols / kColsAtOnce; ++k)
+      for (int i = 0; i < kExpandTileStages; ++i)
+        *reinterpret_cast<uint4*>(shared + i * kStage + b_at(bc + k * kColsAtOnce)) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int i = 0; i < kExpandTileStages - 1; ++i) request();   // none of it comes from the first launch
   griddep_wait();
   uint32_t h[KS][PH][4];
   {
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
-    const size_t part = size_t(P.R) * rank;
     float4 sum[KS][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) sum[s][e] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < P.splits; ++p)
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = my_rows + e * 8 + g, j = s * 16 + 4 * t;
-          if (i >= count || j >= rank) continue;
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + p * part + (row0 + i) * rank + j));
-          sum[s][e].x += v.x; sum[s][e].y += v.y; sum[s][e].z += v.z; sum[s][e].w += v.w;
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int i = my_rows + e * 8 + g, j = s * 16 + 4 * t;
+        sum[s][e] = i < count && j < rank ? __ldcg(reinterpret_cast<const float4*>(P.h[mat] + (row0 + i) * rank + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -834,13 +914,11 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(co
     op[e] = out + (row0 + (row_ok[e] ? i : 0)) * N + my_cols + 4 * t;
   }
   const int place = place_of(4 * (g >> 1) + (g & 1));      // of a lane's column of product 0; that of product n: + (n / 2) * 16 + (n % 2) * 4
-  int stage = 0;
+  const char* from = shared;
   for (int c0 = c_begin; c0 < c_end; c0 += kExpandTileCols) {
     cp_async_wait<kExpandTileStages - 2>();
     __syncthreads();                                       // the stage has arrived; everyone is done with the one that is requested next
-    const int ahead = stage == 0 ? kExpandTileStages - 1 : stage - 1;
-    request(ahead, c0 + (kExpandTileStages - 1) * kExpandTileCols);
-    const char* from = shared + stage * kStage;
+    request();
     float acc[4][4];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -876,7 +954,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(co
           const float d[4] = {acc[2 * q][2 * e], acc[2 * q][2 * e + 1], acc[2 * q + 1][2 * e], acc[2 * q + 1][2 * e + 1]};
           four.add_store(op[e] + c0 + q * 16, d);
         }
-    stage = stage == kExpandTileStages - 1 ? 0 : stage + 1;
+    from = from == shared + (kExpandTileStages - 1) * kStage ? shared : from + kStage;
   }
   cp_async_wait<0>();
 }
@@ -887,7 +965,7 @@ struct AdaptShape {
 };
 
 // Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
-// Splits of K: as many as make two CTAs per SM (one wave), with 256 or more k each.  Columns of a CTA of the second launch: a
+// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a
 // multiple of what its warps take at a time, the more the more tiles there are.
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
   AdaptShape s;
@@ -900,9 +978,8 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.ks = rank <= 16 ? 1 : rank <= 32 || w_pieces > 2 ? 2 : 4;
   const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
-  long long splits = 2LL * sms / ctas;
-  if (splits > K / 256) splits = K / 256;
-  s.splits = int(splits < 1 ? 1 : splits > 16 ? 16 : splits);
+  s.splits = 1;
+  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
   s.tiled = s.rt == kAdaptMaxRows && w_pieces < 3 && rank <= 64;
   const int unit = s.tiled ? kExpandTileCols : kExpandWarps / (s.rt / 16) * 8 * expand_nb(s.ks, w_pieces);
   long long units = 0;

@@ -735,8 +735,8 @@ static cudaError_t launch_sample(const float* x, int rows, int n, long long ldx,
 // ---------------------------------------------------------------------------------------- adapters, verification
 template <typename TX, typename TW, int MT>
 static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  const dim3 grid(sh.tiles, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat * P.splits);
-  if (sh.rt == 16) return launch_chained(adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), 0, stream, P);
+  const dim3 grid(sh.tiles * P.splits, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat);
+  if (sh.rt == 16) return launch_clustered(P.splits, adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), 0, stream, P);
   static bool configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -748,7 +748,7 @@ static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_chained(adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), smem, stream, P);
+  return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), smem, stream, P);
 }
 
 template <typename TX, typename TW>
@@ -2013,9 +2013,8 @@ static AdaptShape adapt_shape_of(int nmat, const b200rwkv_adapters* banks, int n
 
 size_t b200rwkv_adapt_rows_workspace_bytes(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype,
                                            int streams, int tokens_per_stream) {
-  if (adapt_problem(nmat, banks, n_adapters, rank, k_in, streams, tokens_per_stream) || !dense_elem_bytes(dtype) || device_sms() < 1) return 0;
-  const AdaptShape sh = adapt_shape_of(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
-  return size_t(nmat) * align256(size_t(sh.splits) * streams * tokens_per_stream * rank * 4);
+  if (adapt_problem(nmat, banks, n_adapters, rank, k_in, streams, tokens_per_stream) || !dense_elem_bytes(dtype)) return 0;
+  return size_t(nmat) * align256(size_t(streams) * tokens_per_stream * rank * 4);
 }
 
 int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, const void* const* x,

@@ -283,7 +283,7 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     banks_c, pointers = struct.pack("=" + "QQQi4x" * n, *packed), "=%dQ" % n
     shape = (count, rank, k_in, _DENSE_DTYPES[dt])
     with _on(index):
-        ws = torch.empty(_adapt_workspace(index, tuple(n_out), *shape, streams, rows // streams), dtype=torch.uint8, device=a0.device)
+        ws = torch.empty(_adapt_workspace(tuple(n_out), *shape, streams, rows // streams), dtype=torch.uint8, device=a0.device)
         _lib.check(_lib.lib().b200rwkv_adapt_rows(n, banks_c, *shape, struct.pack(pointers, *px), struct.pack(pointers, *py),
                                                   struct.pack(pointers, *po), _DENSE_DTYPES[row_dt], ids.data_ptr(), streams,
                                                   rows // streams, ws.data_ptr(), ws.numel(), _raw_stream(index)))
@@ -291,9 +291,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
 
 
 @lru_cache(maxsize=1024)
-def _adapt_workspace(index: int, n_out: Tuple[int, ...], count: int, rank: int, k_in: int, dtype: int, streams: int, tokens: int) -> int:
-    """Bytes of scratch for a call of this shape on this device (the current one); a refused shape gets a few, for the call to
-    say why."""
+def _adapt_workspace(n_out: Tuple[int, ...], count: int, rank: int, k_in: int, dtype: int, streams: int, tokens: int) -> int:
+    """Bytes of scratch for a call of this shape; a refused shape gets a few, for the call to say why."""
     banks = (_lib.Adapters * len(n_out))(*[_lib.Adapters(None, None, None, o) for o in n_out])
     return max(256, int(_lib.lib().b200rwkv_adapt_rows_workspace_bytes(len(n_out), banks, count, rank, k_in, dtype, streams, tokens)))
 
