@@ -179,8 +179,9 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
 
 // h[row][j] = sum_k x[row][k] A[id][j][k].  Grid (tiles * splits of K, rank chunks of 16 * MT, matrices); the CTAs of a tile's
 // splits are a cluster, whose sums meet in shared memory, in the order of the splits.
-// For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter: from global memory to
-// registers.  A warp takes every eighth block of 32 k of the split.
+// For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter.  A warp takes every eighth
+// block of 32 k of the split; a lane copies its own 16-byte fragments of A and x into slots of its own, several blocks ahead, so
+// that nothing but the end of the sums needs the other warps.
 template <typename Put>
 __device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_sums, int n, Put put) {
   const int S = P.splits;
@@ -206,32 +207,57 @@ __device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_su
   cluster.sync();                          // the tables are read before their CTAs leave
 }
 
+// 16-byte units of a lane and block, and blocks in flight: as many as half an SM's shared memory holds.
+template <typename TX, typename TW, int MT>
+struct ShrinkRing {
+  static constexpr int kA = int(sizeof(TW)) / 2, kX = int(sizeof(TX)) / 2, kUnits = MT * 2 * kA + 2 * kX, kStage = kUnits * 512;
+  static constexpr int kFit = 104 * 1024 / (kShrinkWarps * kStage), kStages = kFit > 6 ? 6 : kFit, kBytes = kShrinkWarps * kStages * kStage;
+  static constexpr int kSums = (kShrinkWarps * 16 * (16 * MT + 4) + 16 * 16 * MT) * 4, kSmem = kBytes > kSums ? kBytes : kSums;
+  static_assert(kStages >= 2, "a block ahead of the one in use");
+};
+
 template <typename TX, typename TW, int MT, int NT>
 __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int mat, int split, int chunk, const int* rows,
-                                            int count, float* red, float* part_sums) {
+                                            int count, char* shared) {
+  using Ring = ShrinkRing<TX, TW, MT>;
   constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
-  constexpr int RC = 16 * MT, kStride = RC + 4;
+  constexpr int RC = 16 * MT, kStride = RC + 4, kStages = Ring::kStages;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int K = P.K, rank = P.rank;
+  const int blocks = (K + 31) / 32, b0 = int((long long)blocks * split / P.splits), b1 = int((long long)blocks * (split + 1) / P.splits);
   const TX* xp[NT];
-  bool xok[NT];
+  uint32_t xok = 0;
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
     const int i = q * 8 + g;
-    xok[q] = i < count;
-    xp[q] = x + size_t(xok[q] ? rows[i] : 0) * K + 8 * t;
+    if (i < count) xok |= 1u << q;
+    xp[q] = x + size_t(rows[i < count ? i : 0]) * K + 8 * t;
   }
-  const TW* ap[MT][2];
-  bool aok[MT][2];
+  const TW* ap = a + size_t(chunk * RC + (chunk * RC + g < rank ? g : 0)) * K + 8 * t;
+  const int have = (rank - chunk * RC - g + 7) / 8;        // of the lane's 2 MT rows of A, those that exist
+  const size_t hop = size_t(8) * K;
+  char* slots = shared + warp * (kStages * Ring::kStage) + lane * 16;
+  const uint32_t slots_at = smem_u32(slots);
+  int ask = b0 + warp;
+  uint32_t to = 0;
+  auto request = [&] {
+    const int k = ask * 32;
+    const bool in = ask < b1 && k + 8 * t < K;             // K is a multiple of 8
+    const int at = in ? k : 0;
+    uint32_t dst = slots_at + to;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < 2 * MT; ++m)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int j = chunk * RC + m * 16 + e * 8 + g;
-      aok[m][e] = j < rank;
-      ap[m][e] = a + size_t(aok[m][e] ? j : 0) * K + 8 * t;
-    }
+      for (int u = 0; u < Ring::kA; ++u, dst += 512) cp_async16(dst, (m < have ? ap + m * hop : ap) + at + u * 4, in && m < have);
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int u = 0; u < Ring::kX; ++u, dst += 512) cp_async16(dst, xp[q] + at + u * 4, in && (xok >> q & 1));
+    cp_async_commit();                                     // a group per block, also an empty one
+    ask += kShrinkWarps;
+    to = to == (kStages - 1) * Ring::kStage ? 0 : to + Ring::kStage;
+  };
   float sum[MT][NT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -239,58 +265,61 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
     for (int q = 0; q < NT; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
-  const int blocks = (K + 31) / 32, b0 = int((long long)blocks * split / P.splits), b1 = int((long long)blocks * (split + 1) / P.splits);
-  for (int kb = b0 + warp; kb < b1; kb += 2 * kShrinkWarps) {
-    // two blocks of 32 k: all loads first
-    AdaptRaw<TX, 8> rx[2][NT];
-    AdaptRaw<TW, 8> ra[2][MT][2];
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) request();
+  const char* from = slots;
+  auto take = [&](auto& raw, const char* at) {             // 8 elements
+    constexpr int n = sizeof(raw.w) / 16;
+#pragma unroll
+    for (int u = 0; u < n; ++u) {
+      const uint4 v = *reinterpret_cast<const uint4*>(at + u * 512);
+      raw.w[4 * u] = v.x; raw.w[4 * u + 1] = v.y; raw.w[4 * u + 2] = v.z; raw.w[4 * u + 3] = v.w;
+    }
+  };
+  for (int kb = b0 + warp; kb < b1; kb += 2 * kShrinkWarps) {   // two blocks; one past the end holds zeros
+    float part[MT][NT][4];                                 // the tensor cores cut their sums off; the running sum rounds
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      const int k = (kb + o * kShrinkWarps) * 32;
-      const bool in = kb + o * kShrinkWarps < b1 && k + 8 * t < K;  // K is a multiple of 8
+      request();
+      cp_async_wait<kStages - 1>();
+      AdaptRaw<TX, 8> rx[NT];
+      AdaptRaw<TW, 8> ra[MT][2];
 #pragma unroll
-      for (int q = 0; q < NT; ++q) rx[o][q].load(xp[q] + k, in && xok[q]);
+      for (int m = 0; m < 2 * MT; ++m) take(ra[m >> 1][m & 1], from + m * Ring::kA * 512);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int q = 0; q < NT; ++q) take(rx[q], from + (2 * MT * Ring::kA + q * Ring::kX) * 512);
+      from = from == slots + (kStages - 1) * Ring::kStage ? slots : from + Ring::kStage;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) ra[o][m][e].load(ap[m][e] + k, in && aok[m][e]);
-    }
-    float part[MT][NT][4];                               // the tensor cores cut their sums off; the running sum rounds
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < NT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[m][q][i] = 0.f;
-#pragma unroll
-    for (int o = 0; o < 2; ++o)
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {             // elements 4 step .. 4 step + 3 of every lane
-        uint32_t fx[NT][2][PX];
+      for (int step = 0; step < 2; ++step) {               // elements 4 step .. 4 step + 3 of every lane
+        uint32_t fx[NT][2][PX], fa[MT][PW][4];
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) rx[o][q].template pair<PX>(2 * step + i, fx[q][i]);
+          for (int i = 0; i < 2; ++i) rx[q].template pair<PX>(2 * step + i, fx[q][i]);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          uint32_t fa[4][PW];
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ra[o][m][i & 1].template pair<PW>(2 * step + (i >> 1), fa[i]);
+          for (int i = 0; i < 4; ++i) {
+            uint32_t f[PW];
+            ra[m][i & 1].template pair<PW>(2 * step + (i >> 1), f);
 #pragma unroll
-          for (int i = PW - 1; i >= 0; --i) {
-            const uint32_t f[4] = {fa[0][i], fa[1][i], fa[2][i], fa[3][i]};
-#pragma unroll
-            for (int j = PX - 1; j >= 0; --j) {
-              if (i + j >= 3) continue;
-#pragma unroll
-              for (int q = 0; q < NT; ++q) {
-                if constexpr (std::is_same<TX, __half>::value && kSame) mma_f16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
-                else mma_bf16(part[m][q], f, fx[q][0][j], fx[q][1][j]);
-              }
-            }
+            for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
           }
-        }
+        bool first = o == 0 && step == 0;
+#pragma unroll
+        for (int i = PW - 1; i >= 0; --i)
+#pragma unroll
+          for (int j = PX - 1; j >= 0; --j) {
+            if (i + j >= 3) continue;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int q = 0; q < NT; ++q)
+                mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
+            first = false;
+          }
       }
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -298,6 +327,9 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
   }
+  cp_async_wait<0>();
+  __syncthreads();                                         // the slots become the table of sums
+  float *red = reinterpret_cast<float*>(shared), *part_sums = red + kShrinkWarps * 16 * kStride;
   // products' rows are ranks (g, g + 8), their columns rows of x (2t, 2t + 1)
   float* mine = red + warp * (16 * kStride);
 #pragma unroll
@@ -320,9 +352,8 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 }
 
 template <typename TX, typename TW, int MT>
-__global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const AdaptParams P) {
-  __shared__ float red[kShrinkWarps * 16 * (16 * MT + 4)];
-  __shared__ float part_sums[16 * 16 * MT];
+__global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_kernel(const AdaptParams P) {
+  extern __shared__ __align__(16) char shared[];
   __shared__ int rows[kAdaptMaxRows];
   __shared__ uint32_t mask[kAdaptWindow / 32];
   griddep_launch_dependents();
@@ -332,8 +363,8 @@ __global__ void __launch_bounds__(kShrinkThreads) adapt_shrink_kernel(const Adap
   if (count == 0 || id < 0) return;        // the whole cluster
   const TX* x = static_cast<const TX*>(P.x[mat]);
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
-  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, red, part_sums);
-  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, red, part_sums);
+  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
+  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
 }
 
 // The same for tiles of 64 rows of one stream: x and A are staged in shared memory, 64 k at a time, several stages ahead of

@@ -736,19 +736,20 @@ static cudaError_t launch_sample(const float* x, int rows, int n, long long ldx,
 template <typename TX, typename TW, int MT>
 static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
   const dim3 grid(sh.tiles * P.splits, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat);
-  if (sh.rt == 16) return launch_clustered(P.splits, adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), 0, stream, P);
+  constexpr int few = ShrinkRing<TX, TW, MT>::kSmem, many = shrink_tile_smem<TX, TW, MT>();
   static bool configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  constexpr int smem = shrink_tile_smem<TX, TW, MT>();
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_shrink_tile_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(adapt_shrink_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, few);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(adapt_shrink_tile_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, many);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), smem, stream, P);
+  if (sh.rt == 16) return launch_clustered(P.splits, adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), few, stream, P);
+  return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), many, stream, P);
 }
 
 template <typename TX, typename TW>
