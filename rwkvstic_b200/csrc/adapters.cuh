@@ -625,33 +625,185 @@ __device__ __forceinline__ void adapt_copy(const TY* y, TY* out, const int* rows
   }
 }
 
-// Products of 8 columns that a warp forms at a time: more where a column has few bytes, so that its loads are as many.
-__host__ __device__ constexpr int expand_nb(int ks, int w_pieces) { return ks < 4 && w_pieces < 3 ? 8 : 4; }
-constexpr int kExpandStages = 2;           // of y, per warp
-// Shared memory: h in the fragments' own order, [row tile][step of 16 ranks][piece][lane] of 16 bytes; then per warp the stages of
-// y, or the table in which odd rows are turned.
+// The second launch, for tiles of up to 16 rows.  Shared memory: h in the fragments' own order, [8 rows][step of 16 ranks][piece]
+// [lane] of 8 bytes; then per warp the stages of B and the table in which its sums are turned.
+// KC: ranks of B per stage.
+template <typename TY, typename TW, int KC>
+struct ExpandRing {
+  static constexpr int MT = sizeof(TW) == 2 ? 4 : 2, kCols = 16 * MT;        // products of 16 columns that a warp forms at a time
+  static constexpr int kLane = KC / 4 * int(sizeof(TW)), kUnit = kLane < 16 ? kLane : 16, kParts = kLane / kUnit;
+  static constexpr int kStage = MT * 2 * 32 * kLane, kPitch = kCols + 4, kTurn = 16 * kPitch * 4;
+  static constexpr int kStages = KC == 16 ? 4 : sizeof(TW) == 2 ? 2 : 3, kWarp = kStages * kStage + kTurn;
+};
 template <typename TY>
-__host__ __device__ constexpr int expand_h_bytes(int row_tiles, int rank) { return row_tiles * ((rank + 15) / 16) * (sizeof(TY) == 2 ? 2 : 3) * 512; }
-template <typename TY, int NB, bool VEC>
-__host__ __device__ constexpr int expand_warp_bytes() { return VEC ? kExpandStages * 16 * 8 * NB * int(sizeof(TY)) : 16 * (8 * NB + 1) * 4; }
+__host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * ((rank + kc - 1) / kc * (kc / 16)) * (sizeof(TY) == 2 ? 2 : 3) * 256; }
 
-// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles, column chunks of all matrices).
-// A warp has 16 rows and takes 8 * NB columns at a time; the columns of two products are dealt out so that a lane ends up with
-// four consecutive ones of two rows.  In a tile of 64 rows four warps take the same columns, in one of 16 all take their own.
-// Fragments of B for the next columns are requested in front of the stores of the present ones; a lane's y comes by asynchronous
-// copies into slots of its own, one step ahead.  h is scaled, and the sum with y rounded once to TY; two pieces of h carry 16
-// bits, enough for a 16-bit y.  Rows that do not start on boundaries of four elements (an odd number of columns) are turned in
-// shared memory, so that a warp's access is one line of a row instead of quarters of eight.
-// KS: steps of 16 ranks whose fragments are held (with more, all are fetched in KS at a time); VEC: all rows of y and out start
-// on boundaries of four elements.
-template <typename TY, typename TW, int KS, bool VEC>
-__global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const AdaptParams P) {
+// NT: products of 8 rows; stage_h() puts the tile's h into shared memory.
+template <typename TY, typename TW, int KC, bool VEC, int NT, typename StageH>
+__device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b, const TY* y, TY* out, int N, int c0, int c_end, const int* rows,
+                                               int count, const char* shared, char* slots, StageH stage_h) {
+  using Ring = ExpandRing<TY, TW, KC>;
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
-  constexpr int NB = expand_nb(KS, PW), COLS = 8 * NB;
+  constexpr int MT = Ring::MT, COLS = Ring::kCols, kStages = Ring::kStages, kStep = kExpandWarps * COLS;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);
+  const uint2* hf = reinterpret_cast<const uint2*>(shared) + lane;
+  float* turn = reinterpret_cast<float*>(slots + kStages * Ring::kStage);
+  // a lane's columns of product m are 16 m + g and 16 m + g + 8, its ranks of a stage KC / 4 * t ..
+  const bool wide = rank * int(sizeof(TW)) % 16 == 0;      // rows of B start on 16 bytes, else on 8
+  const size_t hop = size_t(8) * rank;
+  const uint32_t slots_at = smem_u32(slots) + lane * Ring::kUnit;
+  int ask = c0, ask_k = 0;                                 // columns and rank that are requested next
+  const TW* bp = b + size_t(c0 + g) * rank + KC / 4 * t;
+  uint32_t to = 0;
+  auto request = [&] {
+    if (ask < c_end) {
+      const int j = ask_k + KC / 4 * t;                    // the lane's first rank
+      const TW* src = bp;
+      uint32_t dst = slots_at + to;
+#pragma unroll
+      for (int u = 0; u < 2 * MT; ++u, src += hop) {
+        const bool in = ask + 8 * u + g < c_end;
+#pragma unroll
+        for (int e = 0; e < Ring::kParts; ++e, dst += 32 * Ring::kUnit) {
+          constexpr int n = Ring::kUnit / int(sizeof(TW));
+          const bool ok = in && j + e * n < rank;
+          const TW* at = ok ? src + e * n : b;
+          if (Ring::kUnit == 16 && wide) {
+            cp_async16(dst, at, ok);
+          } else {
+            cp_async8(dst, at, ok);
+            if constexpr (Ring::kUnit == 16) {
+              const bool second = in && j + e * n + n / 2 < rank;
+              cp_async8(dst + 8, second ? src + e * n + n / 2 : b, second);
+            }
+          }
+        }
+      }
+      ask_k += KC;
+      bp += KC;
+      if (ask_k >= rank) { bp += size_t(kStep) * rank - ask_k; ask_k = 0; ask += kStep; }
+    }
+    cp_async_commit();                                     // a group per stage, also an empty one
+    to = to == (kStages - 1) * Ring::kStage ? 0 : to + Ring::kStage;
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) request();         // weights: no part of what the first launch writes
+  stage_h();
+  // sums go out row by row: VEC, half a warp per row, four columns per lane; else a warp per row, a column per lane
+  constexpr int kPass = VEC ? 4 * NT : 8 * NT, kLanes = COLS / 4, kRowsAtOnce = VEC ? 32 / kLanes : 1, kPasses = VEC ? (8 * NT + kRowsAtOnce - 1) / kRowsAtOnce : kPass;
+  const int my_row = VEC ? lane / kLanes : 0, my_col = VEC ? lane % kLanes * 4 : lane;
+  const char* from = slots;
+  for (; c0 < c_end; c0 += kStep) {
+    AdaptFour<TY> four[VEC ? kPasses : 1];
+    TY line[VEC ? 1 : kPasses][VEC ? 1 : COLS / 32];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      if (i * kRowsAtOnce >= count) break;
+      const int r = i * kRowsAtOnce + my_row;
+      const TY* p = y + size_t(rows[r < count ? r : 0]) * N + c0 + my_col;
+      if constexpr (VEC) {
+        if (r < count && c0 + my_col < c_end) four[i].load(p);
+      } else {
+#pragma unroll
+        for (int q = 0; q < COLS / 32; ++q)
+          if (c0 + q * 32 + my_col < c_end) line[i][q] = p[q * 32];
+      }
+    }
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+    for (int k0 = 0; k0 < rank; k0 += KC) {
+      request();
+      cp_async_wait<kStages - 1>();
+      AdaptRaw<TW, KC / 4> raw[MT][2];
+#pragma unroll
+      for (int u = 0; u < 2 * MT; ++u)
+#pragma unroll
+        for (int e = 0; e < Ring::kParts; ++e) {
+          const char* at = from + (u * Ring::kParts + e) * 32 * Ring::kUnit + lane * Ring::kUnit;
+          uint32_t* w = raw[u >> 1][u & 1].w;
+          if constexpr (Ring::kUnit == 16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            w[4 * e] = v.x; w[4 * e + 1] = v.y; w[4 * e + 2] = v.z; w[4 * e + 3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            w[0] = v.x; w[1] = v.y;
+          }
+        }
+      from = from == slots + (kStages - 1) * Ring::kStage ? slots : from + Ring::kStage;
+#pragma unroll
+      for (int s = 0; s < KC / 16; ++s) {
+        uint32_t fa[MT][PW][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t f[PW];
+            raw[m][i & 1].template pair<PW>(2 * s + (i >> 1), f);
+#pragma unroll
+            for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
+          }
+#pragma unroll
+        for (int p = PH - 1; p >= 0; --p)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 h = hf[((n * ksteps + k0 / 16 + s) * PH + p) * 32];
+#pragma unroll
+            for (int w = PW - 1; w >= 0; --w) {
+              if (p + w >= PH) continue;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) mma_bf16(acc[m][n], fa[m][w], h.x, h.y);
+            }
+          }
+      }
+    }
+    __syncwarp();                                          // the table has been read
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn[(n * 8 + 2 * t + (i & 1)) * Ring::kPitch + m * 16 + (i >> 1) * 8 + g] = acc[m][n][i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      if (i * kRowsAtOnce >= count) break;
+      const int r = i * kRowsAtOnce + my_row;
+      TY* p = out + size_t(rows[r < count ? r : 0]) * N + c0 + my_col;
+      if constexpr (VEC) {
+        if (r < count && c0 + my_col < c_end) {
+          const float4 v = *reinterpret_cast<const float4*>(turn + r * Ring::kPitch + my_col);
+          const float d[4] = {v.x, v.y, v.z, v.w};
+          four[i].add_store(p, d);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < COLS / 32; ++q)
+          if (c0 + q * 32 + my_col < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[r * Ring::kPitch + q * 32 + my_col]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles of up to 16 rows, column chunks of all matrices).
+// Columns are the rows of the products and rows, 8 at a time, their columns, so that a tile of one row, the common one of a
+// decoding step, wastes little.  A lane's fragments of B come by asynchronous copies into slots of its own, some stages ahead;
+// sums are turned in the warp's table and leave in lines of a row.  h is scaled, and the sum with y rounded once to TY; two
+// pieces of h carry 16 bits, enough for a 16-bit y.  VEC: all rows of y and out start on boundaries of four elements.
+template <typename TY, typename TW, int KC, bool VEC>
+__global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const AdaptParams P) {
+  using Ring = ExpandRing<TY, TW, KC>;
+  constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
   extern __shared__ __align__(16) char shared[];
-  __shared__ int rows[kAdaptMaxRows];
+  __shared__ int rows[16];
   __shared__ uint32_t mask[kAdaptWindow / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5;
   int id = -1;
   const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
   int mat = 0;
@@ -665,159 +817,31 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
     if (y != out) adapt_copy<TY, VEC>(y, out, rows, count, N, c_begin, c_end);
     return;
   }
-  const int rank = P.rank, ksteps = (rank + 15) / 16;
-  const bool held = ksteps <= KS;
-  const int row_ways = P.rt / 16, my_rows = warp % row_ways * 16, step = kExpandWarps / row_ways * COLS;
-  int c0 = c_begin + warp / row_ways * COLS;
-  const bool mine = my_rows < count && c0 < c_end;         // this warp has anything to do
-  // a lane's column of product n is col + (n / 2) * 16 + (n % 2) * 2, its ranks of a step 4 t .. 4 t + 3
-  const int col = 4 * (g >> 1) + (g & 1);
-  const TW* b = static_cast<const TW*>(P.b[mat]) + (size_t(id) * N + col) * rank + 4 * t;
-  const bool tail = (ksteps - 1) * 16 + 4 * t < rank;      // the lane's ranks of the last step exist (rank is a multiple of four)
-  AdaptRaw<TW, 4> raw[NB][KS];
-  auto fetch = [&](int c, int k0) {
-    const TW* at = b + size_t(c) * rank + k0 * 16;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int off = (n >> 1) * 16 + (n & 1) * 2;
-      const bool in = c + col + off < c_end;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        raw[n][s].load(at + off * rank + s * 16, in && (k0 + s < ksteps - 1 || (k0 + s == ksteps - 1 && tail)));
-    }
-  };
-  // y: rows g and g + 8 of the warp's, columns c + 16 q + 4 t .. + 3
-  const TY* yp[2];
-  TY* op[2];
-  bool row_ok[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int i = my_rows + e * 8 + g;
-    row_ok[e] = i < count;
-    const size_t at = size_t(row_ok[e] ? rows[i] : rows[0]) * N + 4 * t;
-    yp[e] = y + at; op[e] = out + at;
-  }
-  char* slots = shared + expand_h_bytes<TY>(row_ways, rank) + warp * expand_warp_bytes<TY, NB, VEC>();
-  constexpr int kUnit = 4 * sizeof(TY), kStage = NB * 32 * kUnit;
-  auto request = [&](int stage, int c) {
-    if constexpr (VEC) {
-      if (c < c_end) {
-        const uint32_t dst = smem_u32(slots) + stage * kStage + lane * kUnit;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int q = 0; q < NB / 2; ++q)
-            if (row_ok[e] && c + q * 16 + 4 * t < c_end) {
-              if constexpr (sizeof(TY) == 4) cp_async16(dst + (e * (NB / 2) + q) * 32 * kUnit, yp[e] + c + q * 16, true);
-              else cp_async8(dst + (e * (NB / 2) + q) * 32 * kUnit, yp[e] + c + q * 16, true);
-            }
-      }
-      cp_async_commit();                                   // a group per step, also an empty one
-    }
-  };
-  if (mine) {                                              // neither weights nor y come from the first launch
-    if (held) fetch(c0, 0);
-    request(0, c0);
-  }
-  griddep_wait();
-  {
+  const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);
+  auto stage_h = [&] {
+    griddep_wait();
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
-    const int r4 = ksteps * 4, padded = (count + 15) / 16 * 16;      // groups of four ranks; rows
+    const int r4 = ksteps * 4, padded = (count + 7) / 8 * 8;         // groups of four ranks; rows
     for (int i = tid; i < padded * r4; i += kExpandThreads) {
       const int r = i / r4, j4 = i - r * r4, j = j4 * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < count && j < rank) {
-        s = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(rows[r]) * rank + j));
-      }
+      if (r < count && j < rank) s = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(rows[r]) * rank + j));
       uint32_t lo[PH], hi[PH];
       split_pair<PH>(s.x * scale, s.y * scale, lo);
       split_pair<PH>(s.z * scale, s.w * scale, hi);
-      uint32_t* f = reinterpret_cast<uint32_t*>(shared) + (((r >> 4) * ksteps + (j4 >> 2)) * PH * 32 + (r & 7) * 4 + (j4 & 3)) * 4 + ((r >> 3) & 1);
+      // ranks of a step and lane: 16 step + 4 t .. + 3, or with 32 ranks a stage 32 (step / 2) + 8 t + 4 (step % 2) .. + 3
+      const int ks = KC == 16 ? j4 >> 2 : (j4 >> 3) * 2 + (j4 & 1), t = KC == 16 ? j4 & 3 : (j4 >> 1) & 3;
+      uint2* f = reinterpret_cast<uint2*>(shared) + ((r >> 3) * ksteps + ks) * PH * 32 + (r & 7) * 4 + t;
 #pragma unroll
-      for (int p = 0; p < PH; ++p) { f[p * 128] = lo[p]; f[p * 128 + 2] = hi[p]; }
+      for (int p = 0; p < PH; ++p) f[p * 32] = make_uint2(lo[p], hi[p]);
     }
-  }
-  __syncthreads();
-  if (!mine) return;
-  const uint4* hf = reinterpret_cast<const uint4*>(shared) + (my_rows / 16 * ksteps) * PH * 32 + lane;
-  for (int stage = 0; c0 < c_end; c0 += step, stage ^= 1) {
-    TY line[VEC ? 1 : 16][VEC ? 1 : COLS / 32];            // not VEC: rows i, columns c0 + 32 q + lane
-    if constexpr (VEC) {
-      request(stage ^ 1, c0 + step);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (my_rows + i < count) {
-          const TY* p = y + size_t(rows[my_rows + i]) * N + c0 + lane;
-#pragma unroll
-          for (int q = 0; q < COLS / 32; ++q)
-            if (c0 + q * 32 + lane < c_end) line[i][q] = p[q * 32];
-        }
-    }
-    float acc[NB][4];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-    for (int k0 = 0; k0 < ksteps; k0 += KS) {
-      if (!held) fetch(c0, k0);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        if (k0 + s >= ksteps) break;
-        uint32_t fb[NB][2][PW];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          raw[n][s].template pair<PW>(0, fb[n][0]);
-          raw[n][s].template pair<PW>(1, fb[n][1]);
-        }
-#pragma unroll
-        for (int p = PH - 1; p >= 0; --p) {
-          const uint4 v = hf[((k0 + s) * PH + p) * 32];
-          const uint32_t f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int w = PW - 1; w >= 0; --w) {
-            if (p + w >= PH) continue;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) mma_bf16(acc[n], f, fb[n][0][w], fb[n][1][w]);
-          }
-        }
-      }
-    }
-    if (held && c0 + step < c_end) fetch(c0 + step, 0);
-    if constexpr (VEC) {
-      cp_async_wait<1>();
-      const char* from = slots + stage * kStage + lane * kUnit;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (!row_ok[e]) continue;
-#pragma unroll
-        for (int q = 0; q < NB / 2; ++q)
-          if (c0 + q * 16 + 4 * t < c_end) {
-            AdaptFour<TY> four;
-            four.load(reinterpret_cast<const TY*>(from + (e * (NB / 2) + q) * 32 * kUnit));
-            const float d[4] = {acc[2 * q][2 * e], acc[2 * q][2 * e + 1], acc[2 * q + 1][2 * e], acc[2 * q + 1][2 * e + 1]};
-            four.add_store(op[e] + c0 + q * 16, d);
-          }
-      }
-    } else {
-      float* turn = reinterpret_cast<float*>(slots);       // [16][COLS + 1]
-      __syncwarp();
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) turn[((i >> 1) * 8 + g) * (COLS + 1) + (n >> 1) * 16 + 4 * t + 2 * (n & 1) + (i & 1)] = acc[n][i];
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (my_rows + i < count) {
-          TY* p = out + size_t(rows[my_rows + i]) * N + c0 + lane;
-#pragma unroll
-          for (int q = 0; q < COLS / 32; ++q)
-            if (c0 + q * 32 + lane < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[i * (COLS + 1) + q * 32 + lane]);
-        }
-    }
-  }
-  if constexpr (VEC) cp_async_wait<0>();
+    __syncthreads();
+  };
+  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  char* slots = shared + expand_h_bytes<TY>(rank, KC) + warp * Ring::kWarp;
+  const int c0 = c_begin + warp * Ring::kCols;
+  if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, N, c0, c_end, rows, count, shared, slots, stage_h);
+  else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, N, c0, c_end, rows, count, shared, slots, stage_h);
 }
 
 // The same for tiles of 64 rows of one stream, 16-bit weights, ranks up to 64 and rows on boundaries of four elements.  What
@@ -991,31 +1015,36 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(co
 }
 
 struct AdaptShape {
-  bool tiled;                              // the second launch may take its form for 64 rows
-  int rt, tiles, splits, mt, ks, chunk_cols, chunks;   // mt: ranks of a CTA of the first launch, ks: of fragments held in the second, in 16
+  int rt, tiles, splits, mt;               // first launch: rows of a tile, tiles, splits of K, ranks of a CTA in 16
+  bool tiled;                              // second launch: the form for 64 rows, else for 16
+  int tiles2, kc, chunk_cols, chunks;      // its tiles, ranks per stage, columns of a CTA
 };
 
-// Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16.  Tiles that a launch has at most.
-// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.  Columns of a CTA of the second launch: a
-// multiple of what its warps take at a time, the more the more tiles there are.
-inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
+inline int adapt_tiles(int streams, int T, int rt) { return T < rt ? streams : streams * ((T + rt - 1) / rt); }
+
+// Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16; the second launch has its form for
+// 64 rows for 16-bit weights, ranks up to 64 and rows that start on boundaries of four elements (`vec`).
+// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.  Columns of a CTA of
+// the second launch: a multiple of what its warps take at a time, the more the more tiles there are.
+inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool vec, int sms) {
   AdaptShape s;
   s.rt = T >= kAdaptMaxRows ? kAdaptMaxRows : 16;
-  const bool gathered = T < s.rt;
-  s.tiles = gathered ? streams : streams * ((T + s.rt - 1) / s.rt);
-  const long long rows = (long long)streams * T;
-  long long busy = s.tiles;                              // tiles that lead rows
-  if (gathered && adapters + rows / s.rt + 1 < busy) busy = adapters + rows / s.rt + 1;
+  s.tiled = s.rt == kAdaptMaxRows && w_pieces < 3 && rank <= 64 && vec;
+  s.tiles = adapt_tiles(streams, T, s.rt);
+  s.tiles2 = adapt_tiles(streams, T, s.tiled ? kAdaptMaxRows : 16);
+  auto busy = [&](int tiles, int rt) {                   // tiles that lead rows
+    const long long most = adapters + (long long)streams * T / rt + 1;
+    return T < rt && most < tiles ? most : (long long)tiles;
+  };
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
-  s.ks = rank <= 16 ? 1 : rank <= 32 || w_pieces > 2 ? 2 : 4;
-  const long long ctas = busy * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
+  s.kc = rank <= 16 ? 16 : 32;
+  const long long ctas = busy(s.tiles, s.rt) * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
   s.splits = 1;
   while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
-  s.tiled = s.rt == kAdaptMaxRows && w_pieces < 3 && rank <= 64;
-  const int unit = s.tiled ? kExpandTileCols : kExpandWarps / (s.rt / 16) * 8 * expand_nb(s.ks, w_pieces);
+  const int unit = s.tiled ? kExpandTileCols : kExpandWarps * (w_pieces < 3 ? 64 : 32);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  long long per = units * busy / (6LL * sms);            // column units a CTA takes for six CTAs per SM
+  long long per = units * busy(s.tiles2, s.tiled ? kAdaptMaxRows : 16) / (6LL * sms);   // column units a CTA takes for six CTAs per SM
   s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
   s.chunks = 0;
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;

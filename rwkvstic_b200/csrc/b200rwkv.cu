@@ -760,27 +760,22 @@ static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& s
   return cudaErrorInvalidValue;
 }
 
-template <typename TY, typename TW, int KS, bool VEC>
+template <typename TY, typename TW, int KC, bool VEC>
 static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  constexpr int warps = kExpandWarps * expand_warp_bytes<TY, expand_nb(KS, AdaptType<TW>::kPieces), VEC>();
+  constexpr int warps = kExpandWarps * ExpandRing<TY, TW, KC>::kWarp;
   static bool configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KS, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             warps + expand_h_bytes<TY>(kAdaptMaxRows / 16, kAdaptMaxRank));
+    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KC, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             warps + expand_h_bytes<TY>(kAdaptMaxRank, KC));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_chained(adapt_expand_kernel<TY, TW, KS, VEC>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads),
-                        size_t(warps) + expand_h_bytes<TY>(P.rt / 16, P.rank), stream, P);
-}
-
-template <typename TY, typename TW, int KS>
-static cudaError_t launch_adapt_expand_ks(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
-  return vec ? launch_adapt_expand_as<TY, TW, KS, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, KS, false>(P, sh, stream);
+  return launch_chained(adapt_expand_kernel<TY, TW, KC, VEC>, dim3(sh.tiles2, sh.chunks), dim3(kExpandThreads),
+                        size_t(warps) + expand_h_bytes<TY>(P.rank, KC), stream, P);
 }
 
 template <typename TY, typename TW, int KS>
@@ -796,28 +791,28 @@ static cudaError_t launch_adapt_expand_tile(const AdaptParams& P, const AdaptSha
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_chained(adapt_expand_tile_kernel<TY, TW, KS>, dim3(sh.tiles, sh.chunks), dim3(kExpandThreads), smem, stream, P);
+  return launch_chained(adapt_expand_tile_kernel<TY, TW, KS>, dim3(sh.tiles2, sh.chunks), dim3(kExpandThreads), smem, stream, P);
 }
 
 template <typename TY, typename TW>
 static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   if constexpr (sizeof(TW) == 2)
-    if (sh.tiled && vec) switch ((P.rank + 15) / 16) {
+    if (sh.tiled) switch ((P.rank + 15) / 16) {
       case 1: return launch_adapt_expand_tile<TY, TW, 1>(P, sh, stream);
       case 2: return launch_adapt_expand_tile<TY, TW, 2>(P, sh, stream);
       case 3: return launch_adapt_expand_tile<TY, TW, 3>(P, sh, stream);
       default: return launch_adapt_expand_tile<TY, TW, 4>(P, sh, stream);
     }
-  if (sh.ks == 1) return launch_adapt_expand_ks<TY, TW, 1>(P, sh, vec, stream);
-  if (sh.ks == 2) return launch_adapt_expand_ks<TY, TW, 2>(P, sh, vec, stream);
-  if constexpr (AdaptType<TW>::kPieces < 3) return launch_adapt_expand_ks<TY, TW, 4>(P, sh, vec, stream);
-  return cudaErrorInvalidValue;
+  if (sh.kc == 16) return vec ? launch_adapt_expand_as<TY, TW, 16, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 16, false>(P, sh, stream);
+  return vec ? launch_adapt_expand_as<TY, TW, 32, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 32, false>(P, sh, stream);
 }
 
 template <typename TY, typename TW>
-static cudaError_t launch_adapt(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+static cudaError_t launch_adapt(AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   g_chain_launch = false;        // the first launch waits for the work in front of the call, which may still write its inputs
+  P.rt = sh.rt;
   cudaError_t e = launch_adapt_shrink<TY, TW>(P, sh, stream);
+  P.rt = sh.tiled ? kAdaptMaxRows : 16;
   return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, vec, stream) : e;
 }
 
@@ -2006,12 +2001,6 @@ static const char* adapt_problem(int nmat, const b200rwkv_adapters* banks, int n
   return nullptr;
 }
 
-static AdaptShape adapt_shape_of(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, int streams, int T) {
-  int n_out[kAdaptMaxMats] = {0, 0, 0};
-  for (int i = 0; i < nmat; ++i) n_out[i] = banks[i].n_out;
-  return adapt_shape(nmat, n_out, n_adapters, rank, k_in, streams, T, adapt_weight_pieces(dtype), device_sms());
-}
-
 size_t b200rwkv_adapt_rows_workspace_bytes(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype,
                                            int streams, int tokens_per_stream) {
   if (adapt_problem(nmat, banks, n_adapters, rank, k_in, streams, tokens_per_stream) || !dense_elem_bytes(dtype)) return 0;
@@ -2031,11 +2020,9 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
   if (device_sms() < 1) return fail(B200RWKV_ECUDA, "adapt_rows: no CUDA device");
   const size_t need = b200rwkv_adapt_rows_workspace_bytes(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
   if (workspace_bytes < need) return fail(B200RWKV_EINVAL, "adapt_rows: workspace %zu < %zu bytes", workspace_bytes, need);
-  const AdaptShape sh = adapt_shape_of(nmat, banks, n_adapters, rank, k_in, dtype, streams, tokens_per_stream);
   const size_t eb = size_t(dense_elem_bytes(row_dtype));
   AdaptParams P;
   memset(&P, 0, sizeof(P));
-  int chunks = 0;
   bool vec = true;               // rows of y and out start on boundaries of four elements
   for (int i = 0; i < nmat; ++i) {
     const b200rwkv_adapters& m = banks[i];
@@ -2044,12 +2031,12 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
     P.a[i] = m.a; P.b[i] = m.b; P.scale[i] = m.scale; P.x[i] = x[i]; P.y[i] = y[i]; P.out[i] = out[i]; P.n_out[i] = m.n_out;
     P.h[i] = reinterpret_cast<float*>(static_cast<char*>(workspace) + size_t(i) * (need / nmat));
     vec = vec && m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
-    chunks += (m.n_out + sh.chunk_cols - 1) / sh.chunk_cols;
-    P.chunk_end[i] = chunks;
   }
+  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), vec, device_sms());
+  for (int i = 0; i < nmat; ++i) P.chunk_end[i] = (i ? P.chunk_end[i - 1] : 0) + (P.n_out[i] + sh.chunk_cols - 1) / sh.chunk_cols;
   P.ids = reinterpret_cast<const long long*>(ids);
   P.nmat = nmat; P.adapters = n_adapters; P.rank = rank; P.K = k_in; P.R = streams * tokens_per_stream; P.T = tokens_per_stream;
-  P.streams = streams; P.rt = sh.rt; P.splits = sh.splits; P.chunk_cols = sh.chunk_cols;
+  P.streams = streams; P.splits = sh.splits; P.chunk_cols = sh.chunk_cols;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == B200RWKV_F32) e = launch_adapt<float, float>(P, sh, vec, s);
