@@ -598,29 +598,30 @@ struct AdaptFour {
   }
 };
 
-// Columns c_begin .. c_end of `count` rows, eight accesses of a thread in flight.
+// Columns c_begin .. c_end of `count` rows: a warp per row, several accesses of a lane in flight.
 template <typename TY, bool VEC>
 __device__ __forceinline__ void adapt_copy(const TY* y, TY* out, const int* rows, int count, int N, int c_begin, int c_end) {
-  constexpr int W = VEC ? 4 : 1, U = 8;
-  const int wide = (c_end - c_begin) / W, items = count * wide;
-  for (int first = threadIdx.x; first < items; first += U * kExpandThreads) {
-    AdaptFour<TY> four[U];
-    TY one[U];
-    size_t at[U];
+  constexpr int W = VEC ? 4 : 1, U = VEC ? 8 : 16;
+  const int lane = threadIdx.x & 31, n = c_end - c_begin;
+  for (int i = threadIdx.x >> 5; i < count; i += kExpandWarps) {
+    const size_t at = size_t(rows[i]) * N + c_begin;
+    const TY* from = y + at;
+    TY* to = out + at;
+    for (int c = lane * W; c < n; c += U * 32 * W) {
+      AdaptFour<TY> four[VEC ? U : 1];
+      TY one[VEC ? 1 : U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = first + k * kExpandThreads;
-      if (i >= items) continue;
-      const int r = i / wide;
-      at[k] = size_t(rows[r]) * N + c_begin + size_t(i - r * wide) * W;
-      if constexpr (VEC) four[k].load(y + at[k]);
-      else one[k] = y[at[k]];
-    }
+      for (int k = 0; k < U; ++k)
+        if (c + k * 32 * W < n) {
+          if constexpr (VEC) four[k].load(from + c + k * 32 * W);
+          else one[k] = from[c + k * 32];
+        }
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (first + k * kExpandThreads >= items) continue;
-      if constexpr (VEC) four[k].store(out + at[k]);
-      else out[at[k]] = one[k];
+      for (int k = 0; k < U; ++k)
+        if (c + k * 32 * W < n) {
+          if constexpr (VEC) four[k].store(to + c + k * 32 * W);
+          else to[c + k * 32] = one[k];
+        }
     }
   }
 }
@@ -640,7 +641,7 @@ __host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * 
 
 // NT: products of 8 rows; stage_h() puts the tile's h into shared memory.
 template <typename TY, typename TW, int KC, bool VEC, int NT, typename StageH>
-__device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b, const TY* y, TY* out, int N, int c0, int c_end, const int* rows,
+__device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b, const TY* y, TY* out, int c0, int c_end, const size_t* row_at,
                                                int count, const char* shared, char* slots, StageH stage_h) {
   using Ring = ExpandRing<TY, TW, KC>;
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
@@ -701,7 +702,7 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
     for (int i = 0; i < kPasses; ++i) {
       if (i * kRowsAtOnce >= count) break;
       const int r = i * kRowsAtOnce + my_row;
-      const TY* p = y + size_t(rows[r < count ? r : 0]) * N + c0 + my_col;
+      const TY* p = y + row_at[r] + c0 + my_col;
       if constexpr (VEC) {
         if (r < count && c0 + my_col < c_end) four[i].load(p);
       } else {
@@ -774,7 +775,7 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
     for (int i = 0; i < kPasses; ++i) {
       if (i * kRowsAtOnce >= count) break;
       const int r = i * kRowsAtOnce + my_row;
-      TY* p = out + size_t(rows[r < count ? r : 0]) * N + c0 + my_col;
+      TY* p = out + row_at[r] + c0 + my_col;
       if constexpr (VEC) {
         if (r < count && c0 + my_col < c_end) {
           const float4 v = *reinterpret_cast<const float4*>(turn + r * Ring::kPitch + my_col);
@@ -802,6 +803,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
   extern __shared__ __align__(16) char shared[];
   __shared__ int rows[16];
+  __shared__ size_t row_at[16];                            // where they start in y and out
   __shared__ uint32_t mask[kAdaptWindow / 32];
   const int tid = threadIdx.x, warp = tid >> 5;
   int id = -1;
@@ -818,6 +820,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
     return;
   }
   const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);
+  if (tid < 16) row_at[tid] = size_t(rows[tid < count ? tid : 0]) * N;
   auto stage_h = [&] {
     griddep_wait();
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
@@ -840,8 +843,8 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
   char* slots = shared + expand_h_bytes<TY>(rank, KC) + warp * Ring::kWarp;
   const int c0 = c_begin + warp * Ring::kCols;
-  if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, N, c0, c_end, rows, count, shared, slots, stage_h);
-  else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, N, c0, c_end, rows, count, shared, slots, stage_h);
+  if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
+  else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
 }
 
 // The same for tiles of 64 rows of one stream, 16-bit weights, ranks up to 64 and rows on boundaries of four elements.  What
@@ -1024,8 +1027,10 @@ inline int adapt_tiles(int streams, int T, int rt) { return T < rt ? streams : s
 
 // Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16; the second launch has its form for
 // 64 rows for 16-bit weights, ranks up to 64 and rows that start on boundaries of four elements (`vec`).
-// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.  Columns of a CTA of
-// the second launch: a multiple of what its warps take at a time, the more the more tiles there are.
+// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.
+// Columns of a CTA of the second launch: what its warps take at a time, times what leaves three CTAs per SM (gathered tiles: each
+// starts with a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40) or six (tiles of 64 rows,
+// whose last wave costs more; 3B ffn for 8192 rows 222, 217, 204).
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool vec, int sms) {
   AdaptShape s;
   s.rt = T >= kAdaptMaxRows ? kAdaptMaxRows : 16;
@@ -1044,7 +1049,7 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   const int unit = s.tiled ? kExpandTileCols : kExpandWarps * (w_pieces < 3 ? 64 : 32);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  long long per = units * busy(s.tiles2, s.tiled ? kAdaptMaxRows : 16) / (6LL * sms);   // column units a CTA takes for six CTAs per SM
+  long long per = units * busy(s.tiles2, s.tiled ? kAdaptMaxRows : 16) / ((s.tiled ? 6LL : 3LL) * sms);
   s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
   s.chunks = 0;
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
