@@ -14,6 +14,8 @@
 
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "common.cuh"
 
 namespace b200 {
@@ -41,7 +43,7 @@ __device__ __forceinline__ int verify_length(const VerifyParams& P, int b) {
   return n < 0 ? 0 : n > P.K ? P.K : int(n);
 }
 // a weight counts where it is above zero (so not where it is NaN)
-__device__ __forceinline__ double verify_weight(float w) { return w > 0.f ? double(w) : 0.0; }
+__device__ __forceinline__ double verify_weight(float w) { return double(fmaxf(w, 0.f)); }
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -63,11 +65,11 @@ __global__ void __launch_bounds__(kVerifySumWarps * 32) verify_sums_kernel(const
   float w[kVerifySeg / 32];
 #pragma unroll
   for (int i = 0; i < kVerifySeg / 32; ++i) w[i] = i * 32 + lane < n ? __ldg(row + first + i * 32 + lane) : 0.f;
-  double s = 0.0;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};                            // four chains: an addition waits long for the one before
 #pragma unroll
-  for (int i = 0; i < kVerifySeg / 32; ++i) s += verify_weight(w[i]);
-  s = warp_sum_f64(s);
-  if (lane == 0) P.sums[row_id * P.segs + seg] = s;
+  for (int i = 0; i < kVerifySeg / 32; ++i) s[i & 3] += verify_weight(w[i]);
+  const double all = warp_sum_f64((s[0] + s[1]) + (s[2] + s[3]));
+  if (lane == 0) P.sums[row_id * P.segs + seg] = all;
 }
 
 struct VerifyShared {
@@ -78,11 +80,19 @@ struct VerifyShared {
   int any;                                 // the distribution has a weight above zero
 };
 
-// The sum of one row's segments, by a warp.
-__device__ __forceinline__ double verify_row_sum(const double* s, int segs) {
-  double v = 0.0;
-  for (int i = threadIdx.x & 31; i < segs; i += 32) v += __ldcg(s + i);
-  return warp_sum_f64(v);
+// The sums of the segments of one row, or of two (b may be null), by a warp.
+__device__ __forceinline__ double2 verify_row_sums(const double* a, const double* b, int segs) {
+  double2 v = make_double2(0.0, 0.0);
+  for (int i = threadIdx.x & 31; i < segs; i += 32) {
+    const double p = __ldcg(a + i), q = b ? __ldcg(b + i) : 0.0;
+    v.x += p; v.y += q;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double p = __shfl_xor_sync(0xffffffffu, v.x, o), q = __shfl_xor_sync(0xffffffffu, v.y, o);
+    v.x += p; v.y += q;
+  }
+  return v;
 }
 
 __device__ __forceinline__ double warp_inclusive_f64(double v) {
@@ -95,10 +105,63 @@ __device__ __forceinline__ double warp_inclusive_f64(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const VerifyParams P) {
+// The distribution that a stream's token is drawn from.  One form per kind, without branches per weight: the 50 segments of a
+// vocabulary of 50277 are some 3000 weights a warp and stream, and instructions are what this costs.
+enum { VERIFY_TARGET, VERIFY_OTHERS, VERIFY_LEFT };        // the row itself; without the refused token; what the draft leaves of it
+struct VerifyRow {
+  const float *p, *q;
+  double Ps, Qs;
+  int V, refused;                                          // VERIFY_OTHERS: the refused token, or -1
+};
+template <int KIND>
+__device__ __forceinline__ double verify_value(float p, float q, const VerifyRow& R) {
+  const double pd = verify_weight(p);
+  if (KIND != VERIFY_LEFT) return pd;
+  const double v = pd * R.Qs - verify_weight(q) * R.Ps;
+  const int hi = __double2hiint(v), keep = ~(hi >> 31);    // zero where negative
+  return __hiloint2double(hi & keep, __double2loint(v) & keep);
+}
+// put(i, value) for the 32 weights i * 32 + lane of a segment, 16 requested at a time
+template <int KIND, typename Put>
+__device__ __forceinline__ void verify_segment(const VerifyRow& R, int seg, Put put) {
+  constexpr int kPer = kVerifySeg / 32, kHalf = kPer / 2;
+  const int lane = threadIdx.x & 31, first = seg * kVerifySeg, m = R.V - first;
+  const float *pr = R.p + first + lane, *qr = KIND == VERIFY_LEFT ? R.q + first + lane : nullptr;
+  const int gone = KIND == VERIFY_OTHERS && (R.refused & 31) == lane ? (R.refused - first) >> 5 : -1;   // the lane's weight that does not count
+#pragma unroll
+  for (int h = 0; h < kPer; h += kHalf) {
+    float p[kHalf], q[kHalf];
+    if (m >= kVerifySeg) {
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        p[i] = __ldg(pr + (h + i) * 32);
+        q[i] = KIND == VERIFY_LEFT ? __ldg(qr + (h + i) * 32) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        const bool in = (h + i) * 32 + lane < m;
+        p[i] = in ? __ldg(pr + (h + i) * 32) : 0.f;
+        q[i] = KIND == VERIFY_LEFT && in ? __ldg(qr + (h + i) * 32) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) put(h + i, verify_value<KIND>(KIND == VERIFY_OTHERS && h + i == gone ? 0.f : p[i], q[i], R));
+  }
+}
+template <int KIND>
+__device__ __forceinline__ double verify_segment_sum(const VerifyRow& R, int seg) {
+  double c[4] = {0.0, 0.0, 0.0, 0.0};                      // four chains: an addition waits long for the one before
+  verify_segment<KIND>(R, seg, [&](int i, double v) { c[i & 3] += v; });
+  return warp_sum_f64((c[0] + c[1]) + (c[2] + c[3]));
+}
+
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const VerifyParams P) {
   namespace cg = cooperative_groups;
   __shared__ VerifyShared S;
+  if (threadIdx.x == 0) S.any = 0;
   const cg::cluster_group cluster = cg::this_cluster();
+  auto started = cluster.barrier_arrive();                         // met before the first access to another CTA's memory
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank()), b = int(blockIdx.x) / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = P.K, V = P.V, segs = P.segs;
   const int rows = K + 1 + (P.draft ? K : 0), len = verify_length(P, b);
@@ -106,7 +169,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
   const long long* tokens = P.tokens + (long long)b * K;
   const float* u = P.u + (long long)b * (K + 1);
   const double* sums = P.sums + (long long)b * rows * segs;
-  if (tid == 0) S.any = 0;
   // what was drafted, before the dependency: none of it comes from the first launch
   double pd = 0.0, qd = 1.0, ut = 0.0;
   if (warp < len) {
@@ -118,8 +180,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
   }
   griddep_wait();
   for (int r = warp; r <= len; r += kVerifyWarps) {
-    const double p = verify_row_sum(sums + (long long)r * segs, segs);
-    const double q = draft && r < len ? verify_row_sum(sums + (long long)(K + 1 + r) * segs, segs) : 1.0;
+    const bool drafted = draft && r < len;
+    const double2 both = verify_row_sums(sums + (long long)r * segs, drafted ? sums + (long long)(K + 1 + r) * segs : nullptr, segs);
+    const double p = both.x, q = drafted ? both.y : 1.0;
     if (r > warp && r < len) {                                     // beyond the first: rare, many drafts
       const long long d = __ldg(tokens + r);
       const bool known = d >= 0 && d < V;
@@ -138,38 +201,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
   __syncthreads();
   int n = 0;
   while (n < len && S.ok[n]) ++n;
-  // the distribution: 0 the row itself, 1 without the refused token, 2 what the draft leaves of it
-  int kind = n == len ? 0 : draft ? 2 : 1;
-  const float *pr = target + n * P.target_row, *qr = kind == 2 ? draft + n * P.draft_row : pr;
-  const double Ps = S.p_sum[n], Qs = kind == 2 ? S.q_sum[n] : 1.0;
-  const long long refused = kind ? __ldg(tokens + n) : -1;
-  auto weight = [&](float pf, float qf, int i) -> double {
-    const double p = verify_weight(pf);
-    if (kind == 0) return p;
-    if (kind == 1) return i == refused ? 0.0 : p;
-    return fmax(p * Qs - verify_weight(qf) * Ps, 0.0);
-  };
-  constexpr int kPer = kVerifySeg / 32;
+  int kind = n == len ? VERIFY_TARGET : draft ? VERIFY_LEFT : VERIFY_OTHERS;
+  VerifyRow R;
+  R.p = target + n * P.target_row; R.q = kind == VERIFY_LEFT ? draft + n * P.draft_row : nullptr;
+  R.Ps = S.p_sum[n]; R.Qs = kind == VERIFY_LEFT ? S.q_sum[n] : 1.0; R.V = V;
+  const long long d = kind == VERIFY_OTHERS ? __ldg(tokens + n) : -1;
+  R.refused = d >= 0 && d < V ? int(d) : -1;
   VerifyShared* S0 = cluster.map_shared_rank(&S, 0);
-  cluster.sync();                                                  // all CTAs run, so their shared memory exists
+  cluster.barrier_wait(std::move(started));                        // all CTAs run, so their shared memory exists, and S.any is set
   for (;;) {                                                       // a second time where the first distribution is empty
     for (int s = rank * kVerifyWarps + warp; s < segs; s += C * kVerifyWarps) {
-      const int first = s * kVerifySeg, m = V - first;
-      double v = 0.0;
-      if (kind == 0) {                                             // the first launch has these
-        v = lane == 0 ? __ldcg(sums + (long long)n * segs + s) : 0.0;
-      } else {
-        float p[kPer], q[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int at = i * 32 + lane;
-          p[i] = at < m ? __ldg(pr + first + at) : 0.f;
-          q[i] = kind == 2 && at < m ? __ldg(qr + first + at) : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) v += weight(p[i], q[i], first + i * 32 + lane);
-        v = warp_sum_f64(v);
-      }
+      const double v = kind == VERIFY_TARGET ? __ldcg(sums + (long long)n * segs + s)     // the first launch has these
+                       : kind == VERIFY_LEFT ? verify_segment_sum<VERIFY_LEFT>(R, s) : verify_segment_sum<VERIFY_OTHERS>(R, s);
       if (lane == 0) {
         S0->seg[s] = v;
         if (v > 0.0)
@@ -177,8 +220,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
       }
     }
     cluster.sync();
-    if (kind == 0 || S.any) break;                                 // the same in all CTAs
-    kind = 0;
+    if (kind == VERIFY_TARGET || S.any) break;                     // the same in all CTAs
+    kind = VERIFY_TARGET;
     cluster.sync();
   }
   if (rank != 0 || warp != 0) return;
@@ -199,26 +242,22 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
     const int w0 = who * per;
     const double seg = lane < per && w0 + lane < segs ? S.seg[w0 + lane] : 0.0;
     const double seg_upto = warp_inclusive_f64(seg) + run;
-    const int at = choose(seg > 0.0, seg_upto >= aim), first = (w0 + at) * kVerifySeg, m = V - first;
+    const int at = choose(seg > 0.0, seg_upto >= aim);
     run = __shfl_sync(0xffffffffu, seg_upto - seg, at);
-    float p[kPer], q[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int j = i * 32 + lane;
-      p[i] = j < m ? __ldg(pr + first + j) : 0.f;
-      q[i] = kind == 2 && j < m ? __ldg(qr + first + j) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) S.turn[i][lane] = weight(p[i], q[i], first + i * 32 + lane);
+    auto put = [&](int i, double v) { S.turn[i][lane] = v; };
+    if (kind == VERIFY_TARGET) verify_segment<VERIFY_TARGET>(R, w0 + at, put);
+    else if (kind == VERIFY_LEFT) verify_segment<VERIFY_LEFT>(R, w0 + at, put);
+    else verify_segment<VERIFY_OTHERS>(R, w0 + at, put);
     __syncwarp();
-    double sum = 0.0;                                              // of the lane's 32 consecutive weights
+    double c[4] = {0.0, 0.0, 0.0, 0.0};                            // of the lane's 32 consecutive weights
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += S.turn[lane][i];
+    for (int i = 0; i < kVerifySeg / 32; ++i) c[i & 3] += S.turn[lane][i];
+    const double sum = (c[0] + c[1]) + (c[2] + c[3]);
     const double sum_upto = warp_inclusive_f64(sum) + run;
     const int group = choose(sum > 0.0, sum_upto >= aim);
     run = __shfl_sync(0xffffffffu, sum_upto - sum, group);
     const double w = S.turn[group][lane], w_upto = warp_inclusive_f64(w) + run;
-    pick = first + group * 32 + choose(w > 0.0, w_upto >= aim);
+    pick = (long long)(w0 + at) * kVerifySeg + group * 32 + choose(w > 0.0, w_upto >= aim);
   }
   for (int i = lane; i <= K; i += 32) P.out[(long long)b * (K + 1) + i] = i < n ? __ldg(tokens + i) : i == n ? pick : -1;
   if (lane == 0) P.accepted[b] = n;
@@ -226,10 +265,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(const Verif
 
 inline int verify_segs(int V) { return (V + kVerifySeg - 1) / kVerifySeg; }
 
-// CTAs per stream: as many as leave an SM to each, and at most one warp per segment.
+// CTAs per stream: as many as run at once, two per SM, and at most a warp per segment.
 inline int verify_cluster(int B, int segs, int sms) {
   int c = 1;
-  while (c < kVerifyMaxCluster && (long long)B * 2 * c <= sms && segs > c * kVerifyWarps) c *= 2;
+  while (c < kVerifyMaxCluster && (long long)B * c <= sms && segs > c * kVerifyWarps) c *= 2;
   return c;
 }
 
