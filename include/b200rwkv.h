@@ -293,6 +293,16 @@ int b200rwkv_forward_rows(const b200rwkv_model* m, const int64_t* tokens, int st
                           size_t workspace_bytes, void* stream);
 
 /*
+ * b200rwkv_forward_rows for a step whose tokens are drafted and may be refused: the logits of EVERY row, device f32
+ * [streams][tokens_per_stream][n_vocab], and in `trace`, device f32 [n_layer][4][streams][tokens_per_stream][n_embd], 16-byte
+ * aligned, what b200rwkv_advance_state needs to move the state in front of the step on by the accepted tokens only.  `state`
+ * is advanced by all tokens: pass a copy.  Same workspace and results as b200rwkv_forward_rows.
+ */
+int b200rwkv_forward_rows_draft(const b200rwkv_model* m, const int64_t* tokens, int streams, int tokens_per_stream,
+                                float* state, int64_t state_stride, float* logits, float* trace, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/*
  * One pipeline stage of b200rwkv_forward_rows for a model whose blocks are partitioned
  * contiguously over several GPUs (the layer split: each GPU holds the blocks of its stage, as the
  * reference's TORCH_SPLIT strategy places whole layers on devices).  `m` describes THIS stage:

@@ -23,7 +23,7 @@ EXPORTS = (
     "b200rwkv_gemm_plan", "b200rwkv_gemm_workspace_bytes", "b200rwkv_gemm_u8", "b200rwkv_rows_workspace_bytes", "b200rwkv_forward_rows", "b200rwkv_forward_rows_stage", "b200rwkv_argmax",
     "b200rwkv_sample_typical", "b200rwkv_gemv_dense",
     "b200rwkv_adapt_rows_workspace_bytes", "b200rwkv_adapt_rows", "b200rwkv_verify_drafts_workspace_bytes", "b200rwkv_verify_drafts",
-    "b200rwkv_advance_state",
+    "b200rwkv_advance_state", "b200rwkv_forward_rows_draft",
     "b200rwkv_dense_workspace_bytes", "b200rwkv_dense_step", "b200rwkv_dense_rows_workspace_bytes", "b200rwkv_dense_forward_rows",
     "b200rwkv_dense_step_layers", "b200rwkv_dense_forward_rows_layers", "b200rwkv_wait_selftest", "b200rwkv_debug_expire_waits",
     "b200rwkv_step_plan_bytes", "b200rwkv_step_plan_init", "b200rwkv_decode_step_persistent", "b200rwkv_step_geometry",
@@ -137,6 +137,9 @@ def lib() -> C.CDLL:
     L.b200rwkv_forward_rows_stage.restype = C.c_int
     L.b200rwkv_forward_rows_stage.argtypes = [C.POINTER(Model), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
                                               C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.b200rwkv_forward_rows_draft.restype = C.c_int
+    L.b200rwkv_forward_rows_draft.argtypes = [C.POINTER(Model), C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                              C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     L.b200rwkv_argmax.restype = C.c_int
     L.b200rwkv_argmax.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                   C.c_void_p]

@@ -442,11 +442,11 @@ static cudaError_t launch_chained(Kernel kernel, dim3 grid, dim3 block, size_t s
 }
 
 // WKV over T rows of B streams in one launch (wkv_rows.cuh); st: the block's state rows of stream 0.
-static cudaError_t launch_wkv(int B, int T, int C, const float* w, const float* u, float* k, const float* v, const float* gate, float* st,
-                              long long state_stride, unsigned short* out16, int is_bf16, cudaStream_t stream) {
+static cudaError_t launch_wkv(int B, int T, int C, const float* w, const float* u, const float* k, const float* v, const float* gate, float* y,
+                              float* st, long long state_stride, unsigned short* out16, int is_bf16, cudaStream_t stream) {
   WkvParams P;
   memset(&P, 0, sizeof(P));
-  P.w = w; P.u = u; P.k = k; P.v = v; P.gate = gate;
+  P.w = w; P.u = u; P.k = k; P.v = v; P.gate = gate; P.y = y;
   P.aa = st + 2 * size_t(C); P.bb = st + 3 * size_t(C); P.pp = st + 4 * size_t(C);
   P.state_stride = state_stride; P.out16 = out16; P.is_bf16 = is_bf16; P.T = T; P.C = C;
   if (T == 1) return launch_chained(wkv_step_kernel, dim3((B * C + 127) / 128), dim3(128), 0, stream, P, B * C);
@@ -1808,12 +1808,15 @@ size_t b200rwkv_rows_workspace_bytes(const b200rwkv_model* m, int streams, int t
 
 // tokens != null: embedding + ln0 produce the rows; else the rows arrive in x_ext.  x_ext != null: the
 // residual stream lives there (and is left there for the next pipeline stage) instead of the workspace.
+// trace != null: a step with drafted tokens; of every block the rows in front of ln1 and ln2, the keys and the values stay in
+// trace [layers][4][rows][D], and the logits are those of every row.
 static int forward_rows_impl(const b200rwkv_model* m, const int64_t* tokens, float* x_ext, int streams, int tokens_per_stream,
-                             float* state, int64_t state_stride, float* logits, void* workspace, size_t workspace_bytes,
+                             float* state, int64_t state_stride, float* logits, float* trace, void* workspace, size_t workspace_bytes,
                              void* stream) {
   if (!m || !state || !workspace || !m->layers || (!tokens && !x_ext) || (tokens && !m->emb))
     return fail(B200RWKV_EINVAL, "forward_rows: null argument");
   if (x_ext && !aligned16(x_ext)) return fail(B200RWKV_EINVAL, "forward_rows: x must be 16-byte aligned");
+  if (trace && !aligned16(trace)) return fail(B200RWKV_EINVAL, "forward_rows: trace must be 16-byte aligned");
   const int D = m->n_embd, F = m->n_ffn, V = m->n_vocab, L = m->n_layer, B = streams, T = tokens_per_stream;
   if (D <= 0 || (D % 128) != 0 || F <= 0 || (F % 128) != 0 || L <= 0 || ((tokens || logits) && V <= 0))
     return fail(B200RWKV_EINVAL, "forward_rows: n_embd=%d n_ffn=%d must be positive multiples of 128", D, F);
@@ -1835,6 +1838,10 @@ static int forward_rows_impl(const b200rwkv_model* m, const int64_t* tokens, flo
   // 4096 rows a call, 71868 -> 71569, within the noise).
   g_chain_launch = false;
   if (x_ext) ws.xa = x_ext;
+  // with a trace a block's rows live there: its input, the ffn's input, keys and values; the WKV output keeps the workspace
+  float *const wkv_out = ws.kb, *const x_out = ws.xa;
+  auto traced = [&](int l, int which) { return trace + (size_t(l) * 4 + which) * R * D; };
+  if (trace) ws.xa = traced(0, 0);
   if (tokens) {
     e = launch_chained(embed_ln0_rows_kernel, dim3(R), dim3(256), 0, s, m->emb, reinterpret_cast<const long long*>(tokens), D, V,
                        m->ln0_w, m->ln0_b, ws.xa);
@@ -1870,6 +1877,11 @@ static int forward_rows_impl(const b200rwkv_model* m, const int64_t* tokens, flo
         return fail(B200RWKV_EINVAL, "forward_rows: layer %d matrix %d is %dx%d, expected %dx%d", l, i, chk[i]->n_out,
                     chk[i]->k_in, want_n[i], want_k[i]);
     }
+    float* x_next = ws.xa;          // the block's output, over its input
+    if (trace) {
+      ws.xa = traced(l, 0); ws.xb = traced(l, 1); ws.kb = traced(l, 2); ws.vb = traced(l, 3);
+      x_next = l + 1 < L ? traced(l + 1, 0) : x_out;
+    }
     // 1. ln1 + token-shift mix -> key, value, sigmoid(receptance)
     memset(&Q, 0, sizeof(Q));
     fill_prep_seg(Q.seg[0], ly.att_key, ly.att_mix_k, nullptr);
@@ -1886,13 +1898,13 @@ static int forward_rows_impl(const b200rwkv_model* m, const int64_t* tokens, flo
     gemm_common(3, D);
     { const b200rwkv_matrix* mp[3] = {&ly.att_key, &ly.att_value, &ly.att_receptance};
       if ((e = launch_tile_gemm(P, mp, ws.digits, s, &why)) != cudaSuccess) goto launch_failed; }
-    // 2. WKV recurrence over each stream's rows; kb <- sigmoid(r) * wkv
+    // 2. WKV recurrence over each stream's rows; kb (of the workspace) <- sigmoid(r) * wkv
     why = "wkv launch failed";
-    e = launch_wkv(B, T, D, ly.time_decay, ly.time_first, ws.kb, ws.vb, ws.rb, st, state_stride, nullptr, 0, s);
+    e = launch_wkv(B, T, D, ly.time_decay, ly.time_first, ws.kb, ws.vb, ws.rb, wkv_out, st, state_stride, nullptr, 0, s);
     if (e != cudaSuccess) goto launch_failed;
     // 3. attention output projection + residual -> xb
     memset(&Q, 0, sizeof(Q));
-    fill_prep_seg(Q.seg[0], ly.att_output, nullptr, ws.kb);
+    fill_prep_seg(Q.seg[0], ly.att_output, nullptr, wkv_out);
     prep_common(1, D, ROWS_PLAIN, nullptr, nullptr, nullptr, nullptr, wants_sums(ly.att_output));
     commit_carry(st);                 // ln1 output of each stream's last row -> state row 0
     if ((e = launch_rows_prep(Q, s, &why)) != cudaSuccess) goto launch_failed;
@@ -1923,26 +1935,27 @@ static int forward_rows_impl(const b200rwkv_model* m, const int64_t* tokens, flo
     commit_carry(st + size_t(D));     // ln2 output of each stream's last row -> state row 1
     if ((e = launch_rows_prep(Q, s, &why)) != cudaSuccess) goto launch_failed;
     memset(&P, 0, sizeof(P));
-    fill_gemm_seg(P.seg[0], ly.ffn_value, ws.scal, ws.xa, D);
+    fill_gemm_seg(P.seg[0], ly.ffn_value, ws.scal, x_next, D);
     P.seg[0].res = ws.xb; P.seg[0].ldres = D; P.seg[0].gate = ws.rb; P.seg[0].ldgate = D;
     gemm_common(1, F);
     { const b200rwkv_matrix* mp[1] = {&ly.ffn_value};
       if ((e = launch_tile_gemm(P, mp, ws.digits, s, &why)) != cudaSuccess) goto launch_failed; }
   }
   if (logits) {
-    // ln_out + head on the last row of every stream (opt.py:73-75)
+    // ln_out + head on the last row of every stream (opt.py:73-75), on every row of a step with drafted tokens
     if (int rc = check_matrix(m->head, "forward_rows head")) return rc;
     if (m->head.n_out != V || m->head.k_in != D) return fail(B200RWKV_EINVAL, "forward_rows: head is %dx%d", m->head.n_out, m->head.k_in);
-    const int Bpad = gemm_padded_rows(B);
+    if (trace) ws.xa = x_out;
+    const int H = trace ? R : B, Hpad = gemm_padded_rows(H);
     memset(&Q, 0, sizeof(Q));
     fill_prep_seg(Q.seg[0], m->head, nullptr, nullptr);
-    Q.nseg = 1; Q.K = D; Q.R = B; Q.T = 1; Q.Rpad = Bpad; Q.mode = ROWS_LN; Q.need_sums = wants_sums(m->head) ? 1 : 0;
-    Q.ldx = (long long)T * D; Q.ln_x = ws.xa + size_t(T - 1) * D; Q.ln_w = m->ln_out_w; Q.ln_b = m->ln_out_b;
+    Q.nseg = 1; Q.K = D; Q.R = H; Q.T = 1; Q.Rpad = Hpad; Q.mode = ROWS_LN; Q.need_sums = wants_sums(m->head) ? 1 : 0;
+    Q.ldx = trace ? D : (long long)T * D; Q.ln_x = trace ? ws.xa : ws.xa + size_t(T - 1) * D; Q.ln_w = m->ln_out_w; Q.ln_b = m->ln_out_b;
     Q.digits = ws.digits; Q.scal = ws.scal;
     if ((e = launch_rows_prep(Q, s, &why)) != cudaSuccess) goto launch_failed;
     memset(&P, 0, sizeof(P));
     fill_gemm_seg(P.seg[0], m->head, ws.scal, logits, V);
-    P.nseg = 1; P.K = D; P.R = B; P.Rpad = Bpad; P.status = ws.status; P.sk_acc = ws.sk_acc; P.sk_count = ws.sk_count;
+    P.nseg = 1; P.K = D; P.R = H; P.Rpad = Hpad; P.status = ws.status; P.sk_acc = ws.sk_acc; P.sk_count = ws.sk_count;
     { const b200rwkv_matrix* mp[1] = {&m->head};
       if ((e = launch_tile_gemm(P, mp, ws.digits, s, &why)) != cudaSuccess) goto launch_failed; }
   }
@@ -1954,7 +1967,14 @@ launch_failed:
 int b200rwkv_forward_rows(const b200rwkv_model* m, const int64_t* tokens, int streams, int tokens_per_stream, float* state,
                           int64_t state_stride, float* logits, void* workspace, size_t workspace_bytes, void* stream) {
   if (!tokens) return fail(B200RWKV_EINVAL, "forward_rows: null tokens");
-  return forward_rows_impl(m, tokens, nullptr, streams, tokens_per_stream, state, state_stride, logits, workspace,
+  return forward_rows_impl(m, tokens, nullptr, streams, tokens_per_stream, state, state_stride, logits, nullptr, workspace,
+                           workspace_bytes, stream);
+}
+
+int b200rwkv_forward_rows_draft(const b200rwkv_model* m, const int64_t* tokens, int streams, int tokens_per_stream, float* state,
+                                int64_t state_stride, float* logits, float* trace, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!tokens || !trace || !logits) return fail(B200RWKV_EINVAL, "forward_rows_draft: null tokens, logits or trace");
+  return forward_rows_impl(m, tokens, nullptr, streams, tokens_per_stream, state, state_stride, logits, trace, workspace,
                            workspace_bytes, stream);
 }
 
@@ -1962,8 +1982,8 @@ int b200rwkv_forward_rows_stage(const b200rwkv_model* m, const int64_t* tokens, 
                                 float* state, int64_t state_stride, float* logits, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   if (!x) return fail(B200RWKV_EINVAL, "forward_rows_stage: null x");
-  return forward_rows_impl(m, tokens, x, streams, tokens_per_stream, state, state_stride, logits, workspace, workspace_bytes,
-                           stream);
+  return forward_rows_impl(m, tokens, x, streams, tokens_per_stream, state, state_stride, logits, nullptr, workspace,
+                           workspace_bytes, stream);
 }
 
 int b200rwkv_argmax(const float* x, int rows, int n, int64_t ldx, int64_t* out, int64_t* history, int* history_count,
@@ -2238,7 +2258,7 @@ int b200rwkv_dense_forward_rows_layers(const b200rwkv_dense_model* m, int layer_
       B200_DR_CHECK(launch_dense_gemm(P, w, x, D, Rpad, s, &why), "key/value/receptance"); }
     // 2. WKV recurrence over each stream's rows; t0 <- T(sigmoid(r) * wkv)
     why = "wkv launch";
-    B200_DR_CHECK(launch_wkv(B, T, D, ly.time_decay, ly.time_first, ws.kb, ws.vb, ws.rb, st, state_stride, ws.t0, bf, s), "wkv");
+    B200_DR_CHECK(launch_wkv(B, T, D, ly.time_decay, ly.time_first, ws.kb, ws.vb, ws.rb, nullptr, st, state_stride, ws.t0, bf, s), "wkv");
     // 3. attention output + residual -> xb
     memset(&P, 0, sizeof(P));
     P.nseg = 1; P.R = R; P.is_bf16 = bf; P.status = ws.status; P.sk_part = R <= kDgSplitMaxRows ? ws.sk_part : nullptr; P.sk_count = ws.sk_count;

@@ -1,6 +1,6 @@
 // WKV-4 over rows laid out [stream][T][C] for the many-rows paths: max-trick state rows of stream s at
-// aa / bb / pp + s * state_stride, advanced in place; y = gate * wkv goes over k (fp32) or, rounded to the
-// matrices' 16-bit type, to out16.
+// aa / bb / pp + s * state_stride, advanced in place; y = gate * wkv goes over k or to rows of its own (fp32) or,
+// rounded to the matrices' 16-bit type, to out16.
 //
 // The recurrence is sequential in t, but it is a scan whose state composes: after n steps without input
 // the state (aa, bb, pp) is (aa, bb, pp + n*w), and two states add after bringing them to a common
@@ -32,11 +32,12 @@ __device__ __forceinline__ unsigned short to_bits16(float v, int is_bf16) {
 
 struct WkvParams {
   const float *w, *u;               // [C] decay (negative), first
-  float* k;                         // [streams][T][C]
+  const float* k;                   // [streams][T][C]
   const float *v, *gate;
   float *aa, *bb, *pp;
   long long state_stride;
-  unsigned short* out16;            // null: y over k
+  float* y;                         // may be k
+  unsigned short* out16;            // not null: y goes here instead
   int is_bf16;
   int T, C, steps;                  // steps per warp, 1..kWkvSteps
 };
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kWkvWarpsMax * 32, 1) wkv_span_kernel(const Wk
       if (warp > g0) advance(a, b, p, g0, warp - g0);
       auto put = [&](int t, float y) {
         if (P.out16) P.out16[row + unsigned(t) * uC] = to_bits16(y, P.is_bf16);
-        else P.k[row + unsigned(t) * uC] = y;
+        else P.y[row + unsigned(t) * uC] = y;
       };
       int t = 0;
       for (; t + U <= len; t += U) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(128) wkv_step_kernel(const WkvParams P, int n)
   const float k = __ldcg(P.k + idx), v = __ldcg(P.v + idx), g = __ldcg(P.gate + idx);
   const float y = g * wkv_step(k, v, wv, uv, a, b, p);
   if (P.out16) P.out16[idx] = to_bits16(y, P.is_bf16);
-  else P.k[idx] = y;
+  else P.y[idx] = y;
   P.aa[so] = a; P.bb[so] = b; P.pp[so] = p;
 }
 

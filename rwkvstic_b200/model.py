@@ -413,6 +413,44 @@ class B200RWKV:
             self._queue_rows_status(ws)
         return out
 
+    # ------------------------------------------------------------------ steps with drafted tokens
+    def forward_draft(self, tokens: torch.Tensor, state: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """A step whose later tokens are drafted and may be refused: ``tokens [B,T]`` (each stream's last sure token and T-1
+        drafted ones), ``state [B,L,5,D]`` as ``forward_rows`` takes it, left as it is.  One rows call; returns the logits
+        after every token ``[B,T,V]`` and the trace ``[L,4,B,T,D]`` that ``accept`` needs.  At most ``rows_per_call`` rows."""
+        if tokens.dim() != 2 or tokens.numel() == 0:
+            raise ValueError("forward_draft needs tokens [B,T] with at least one token")
+        B, T = tokens.shape
+        if (state.dtype != torch.float32 or state.device != self.device or not state.is_contiguous()
+                or tuple(state.shape) != (B, self.n_layer, 5, self.n_embd)):
+            raise ValueError(f"forward_draft needs a contiguous fp32 state [{B},{self.n_layer},5,{self.n_embd}] on the model's device")
+        if B * T > min(self.rows_per_call, 65535):
+            raise ValueError(f"forward_draft: at most {min(self.rows_per_call, 65535)} rows per call")
+        if self.w.emb is None or self.w.head is None:
+            raise ValueError("forward_draft needs a whole model, not a pipeline stage")
+        self._raise_rows_status()
+        logits = torch.empty(B, T, self.n_vocab, dtype=torch.float32, device=self.device)
+        trace = torch.empty(self.n_layer, 4, B, T, self.n_embd, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            toks = tokens.to(device=self.device, dtype=torch.int64).contiguous()
+            ws, scratch = self._rows_workspace(B, T), state.clone()
+            _lib.check(self._L.b200rwkv_forward_rows_draft(
+                C.byref(self._cmodel), toks.data_ptr(), B, T, scratch.data_ptr(), scratch.stride(0), logits.data_ptr(), trace.data_ptr(),
+                ws.data_ptr(), ws.numel(), torch.cuda.current_stream(self.device).cuda_stream))
+            self.launch_count += self._rows_launches() + 3
+            self._queue_rows_status(ws)
+        return logits, trace
+
+    def accept(self, state: torch.Tensor, trace: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+        """Move ``state [B,L,5,D]`` on, in place, by the first ``counts[b]`` (int64, device) of the tokens that
+        ``forward_draft`` was given: the sure one and the accepted ones (``ops.verify_drafts``'s count plus one)."""
+        from . import ops
+        if getattr(self, "_advance_params", None) is None:
+            names = ("ln1.weight", "ln1.bias", "ln2.weight", "ln2.bias", "att.time_decay")
+            self._advance_params = torch.stack([torch.stack([ly.vec[k].reshape(-1) for k in names]) for ly in self.w.layers])
+        self.launch_count += 1
+        return ops.advance_state(state, counts, trace, self._advance_params)
+
     def _rows_workspace(self, B: int, tp: int) -> torch.Tensor:
         ws = self._rows_ws.get((B, tp))
         if ws is None:
