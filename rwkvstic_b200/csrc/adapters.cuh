@@ -31,10 +31,9 @@ namespace b200 {
 constexpr int kAdaptMaxMats = 3;
 constexpr int kAdaptWindow = 1024;         // streams
 constexpr int kAdaptMaxRank = 256;
-constexpr int kAdaptMaxRows = 64;          // of a tile
+constexpr int kAdaptRows = 16;             // of a gathered tile
 constexpr int kAdaptMaxSplits = 8;         // of K: a cluster of CTAs
 constexpr int kShrinkThreads = 256, kShrinkWarps = kShrinkThreads / 32;
-constexpr int kShrinkChunk = 64;           // k of a stage of the tiled form
 constexpr int kExpandThreads = 256, kExpandWarps = kExpandThreads / 32;
 
 struct AdaptParams {
@@ -45,7 +44,7 @@ struct AdaptParams {
   int n_out[kAdaptMaxMats];
   int chunk_end[kAdaptMaxMats];            // second launch: column chunks of the matrices up to and including this one
   const long long* ids;
-  int nmat, adapters, rank, K, R, T, streams, rt, splits, chunk_cols;
+  int nmat, adapters, rank, K, R, T, streams, splits, chunk_cols, stages;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -133,7 +132,8 @@ struct AdaptRaw {
 // The rows of tile `tile` into rows[0..count): returns count, 0 where this CTA leads none.  *id: their adapter, -1: none.
 // All threads of the CTA take part; mask: kAdaptWindow / 32 words of shared memory.
 __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* rows, uint32_t* mask, int* id) {
-  const int tid = threadIdx.x, nt = blockDim.x, T = P.T, rt = P.rt;
+  constexpr int rt = kAdaptRows;
+  const int tid = threadIdx.x, nt = blockDim.x, T = P.T;
   auto id_of = [&](int s) {
     const long long v = __ldg(P.ids + s);
     return v >= 0 && v < P.adapters ? int(v) : -1;
@@ -182,12 +182,13 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
 // For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter.  A warp takes every eighth
 // block of 32 k of the split; a lane copies its own 16-byte fragments of A and x into slots of its own, several blocks ahead, so
 // that nothing but the end of the sums needs the other warps.
-template <typename Put>
-__device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_sums, int n, Put put) {
-  const int S = P.splits;
+// put(i, sum over the cluster's CTAs of part_sums[place(i)]) for i < n
+template <typename Place, typename Put>
+__device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_sums, int n, Place place, Put put) {
+  const int S = P.splits, nt = blockDim.x;
   if (S == 1) {
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kShrinkThreads) put(i, part_sums[i]);
+    for (int i = threadIdx.x; i < n; i += nt) put(i, part_sums[place(i)]);
     return;
   }
   namespace cg = cooperative_groups;
@@ -195,10 +196,10 @@ __device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_su
   const int rank = int(cluster.block_rank());
   cluster.sync();
   // every CTA adds up a part of the table; all of a thread's remote reads are in flight at once
-  for (int i = rank * kShrinkThreads + threadIdx.x; i < n; i += S * kShrinkThreads) {
+  for (int i = rank * nt + threadIdx.x; i < n; i += S * nt) {
     float v[kAdaptMaxSplits];
 #pragma unroll
-    for (int c = 0; c < kAdaptMaxSplits; ++c) v[c] = c < S ? *cluster.map_shared_rank(part_sums + i, c) : 0.f;
+    for (int c = 0; c < kAdaptMaxSplits; ++c) v[c] = c < S ? *cluster.map_shared_rank(part_sums + place(i), c) : 0.f;
     float s = v[0];
 #pragma unroll
     for (int c = 1; c < kAdaptMaxSplits; ++c) s += v[c];
@@ -345,7 +346,7 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
     for (int w = 0; w < kShrinkWarps; ++w) s += red[(w * 16 + r) * kStride + j];
     part_sums[i] = s;
   }
-  shrink_join(P, part_sums, count * RC, [&](int i, float s) {
+  shrink_join(P, part_sums, count * RC, [](int i) { return i; }, [&](int i, float s) {
     const int r = i / RC, j = chunk * RC + i - r * RC;
     if (j < rank) P.h[mat][size_t(rows[r]) * rank + j] = s;
   });
@@ -354,7 +355,7 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
 template <typename TX, typename TW, int MT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_kernel(const AdaptParams P) {
   extern __shared__ __align__(16) char shared[];
-  __shared__ int rows[kAdaptMaxRows];
+  __shared__ int rows[kAdaptRows];
   __shared__ uint32_t mask[kAdaptWindow / 32];
   griddep_launch_dependents();
   int id = -1;
@@ -365,184 +366,6 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_kernel(const A
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
   if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
   else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
-}
-
-// The same for tiles of 64 rows of one stream: x and A are staged in shared memory, 64 k at a time, several stages ahead of
-// the products.  Four warps take 16 rows each, for one half of a stage's k; four more the other half.
-template <typename T>
-struct StageTile {                         // 64 elements of each row, in 16-byte units dealt out so that fragment reads meet no bank twice
-  static constexpr int kUnits = kShrinkChunk * int(sizeof(T)) / 16, kRowBytes = kUnits * 16;
-  __device__ static __forceinline__ int swizzle(int row, int unit) { return sizeof(T) == 2 ? unit ^ ((row & 3) << 1) : unit ^ ((row & 1) << 2); }
-  // elements 16 step + 4 t .. + 3 of a row
-  __device__ static __forceinline__ void read(const char* tile, int row, int step, int t, AdaptRaw<T, 4>& f) {
-    if constexpr (sizeof(T) == 2) {
-      const uint2 v = *reinterpret_cast<const uint2*>(tile + row * kRowBytes + swizzle(row, 2 * step + (t >> 1)) * 16 + (t & 1) * 8);
-      f.w[0] = v.x; f.w[1] = v.y;
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(tile + row * kRowBytes + swizzle(row, 4 * step + t) * 16);
-      f.w[0] = v.x; f.w[1] = v.y; f.w[2] = v.z; f.w[3] = v.w;
-    }
-  }
-};
-
-// What one thread copies of every stage of R rows: the same units of rows kThreadRows apart, 64 elements further each time.
-template <typename T, int R>
-struct StageCopy {
-  static constexpr int kThreadRows = kShrinkThreads / StageTile<T>::kUnits, kCopies = R / kThreadRows > 0 ? R / kThreadRows : 1;
-  const T* src;                            // of the first copy, in the next stage
-  size_t hop;                              // kThreadRows rows
-  uint32_t dst;                            // in stage 0 (the swizzle of a row kThreadRows further is the same)
-  int k, rows;                             // element of the next stage's copies; copies of rows that exist
-  __device__ __forceinline__ StageCopy(const T* base, uint32_t tile, int have, size_t ld, int k0) {
-    const int r = int(threadIdx.x) / StageTile<T>::kUnits, u = int(threadIdx.x) % StageTile<T>::kUnits;
-    k = k0 + u * (16 / int(sizeof(T)));
-    src = base + (r < have ? r : 0) * ld + k;
-    hop = kThreadRows * ld;
-    dst = tile + r * StageTile<T>::kRowBytes + StageTile<T>::swizzle(r, u) * 16;
-    rows = r < R ? (have - r + kThreadRows - 1) / kThreadRows : 0;
-    if (rows < 0) rows = 0;
-  }
-  // into the stage at `at` bytes; past `end` zeros
-  __device__ __forceinline__ void next(uint32_t at, int end) {
-    const bool in = k < end;
-    const T* from = in ? src : src - k;    // an address that may be read
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      if (R >= kThreadRows || int(threadIdx.x) < R * StageTile<T>::kUnits)
-        cp_async16(dst + at + i * kThreadRows * StageTile<T>::kRowBytes, i < rows ? from + i * hop : from, in && i < rows);
-    src += kShrinkChunk;
-    k += kShrinkChunk;
-  }
-};
-
-// stages: as many as half an SM's shared memory holds
-template <typename TX, typename TW, int MT>
-__host__ __device__ constexpr int shrink_stages() {
-  const int n = 110 * 1024 / (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
-  return n > 8 ? 8 : n;
-}
-
-template <typename TX, typename TW, int MT>
-constexpr int shrink_tile_smem() {
-  const int stages = shrink_stages<TX, TW, MT>() * (kAdaptMaxRows * StageTile<TX>::kRowBytes + 16 * MT * StageTile<TW>::kRowBytes);
-  const int sums = (kShrinkWarps * 16 * (16 * MT + 4) + kAdaptMaxRows * 16 * MT) * 4;
-  return stages > sums ? stages : sums;
-}
-
-template <typename TX, typename TW, int MT>
-__global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_tile_kernel(const AdaptParams P) {
-  constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
-  constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
-  constexpr int RC = 16 * MT, kStride = RC + 4, NT = 2, kShrinkStages = shrink_stages<TX, TW, MT>();
-  constexpr int kBytesX = kAdaptMaxRows * StageTile<TX>::kRowBytes, kBytes = kBytesX + RC * StageTile<TW>::kRowBytes;
-  extern __shared__ __align__(128) char stages[];
-  griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x / P.splits, split = blockIdx.x - tile * P.splits, mat = blockIdx.z;
-  const int per = (P.T + kAdaptMaxRows - 1) / kAdaptMaxRows, s = tile / per, first = (tile - s * per) * kAdaptMaxRows;
-  const int count = min(kAdaptMaxRows, P.T - first), row0 = s * P.T + first, K = P.K, rank = P.rank;
-  const long long asked = __ldg(P.ids + s);
-  if (asked < 0 || asked >= P.adapters) return;            // the whole cluster
-  const int j0 = blockIdx.y * RC, ranks = min(RC, rank - j0);
-  const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
-  const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
-  const int chunks = (K + kShrinkChunk - 1) / kShrinkChunk, c0 = int((long long)chunks * split / P.splits), c1 = int((long long)chunks * (split + 1) / P.splits);
-  const uint32_t base = smem_u32(stages);
-  StageCopy<TX, kAdaptMaxRows> copy_x(x, base, count, K, c0 * kShrinkChunk);
-  StageCopy<TW, RC> copy_a(a, base + kBytesX, ranks, K, c0 * kShrinkChunk);
-  const int end = min(K, c1 * kShrinkChunk);
-  uint32_t to = 0;                         // the stage that is filled next, in bytes
-  auto request = [&] {
-    copy_x.next(to, end);
-    copy_a.next(to, end);
-    cp_async_commit();
-    to = to == (kShrinkStages - 1) * kBytes ? 0 : to + kBytes;
-  };
-#pragma unroll
-  for (int i = 0; i < kShrinkStages - 1; ++i) request();
-  const int my_rows = (warp & 3) * 16, half = warp >> 2;
-  const char* from = stages;               // the stage that is read
-  float sum[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[m][q][i] = 0.f;
-  for (int c = c0; c < c1; c += 2) {       // two stages; one past the end holds zeros
-    float part[MT][NT][4];                 // the tensor cores cut their sums off; the running sum rounds
-#pragma unroll
-    for (int pair = 0; pair < 2; ++pair) {
-      cp_async_wait<kShrinkStages - 2>();
-      __syncthreads();                     // the stage has arrived; everyone is done with the one that is requested next
-      request();
-      const char *tx = from, *ta = from + kBytesX;
-      from = from == stages + (kShrinkStages - 1) * kBytes ? stages : from + kBytes;
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int step = 2 * half + o;
-        uint32_t fx[NT][2][PX], fa[MT][PW][4];
-#pragma unroll
-        for (int q = 0; q < NT; ++q) {
-          AdaptRaw<TX, 4> f;
-          StageTile<TX>::read(tx, my_rows + q * 8 + g, step, t, f);
-          f.template pair<PX>(0, fx[q][0]);
-          f.template pair<PX>(1, fx[q][1]);
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            AdaptRaw<TW, 4> f;
-            StageTile<TW>::read(ta, m * 16 + e * 8 + g, step, t, f);
-            uint32_t lo[PW], hi[PW];
-            f.template pair<PW>(0, lo);
-            f.template pair<PW>(1, hi);
-#pragma unroll
-            for (int i = 0; i < PW; ++i) { fa[m][i][e] = lo[i]; fa[m][i][2 + e] = hi[i]; }
-          }
-        bool first = pair == 0 && o == 0;
-#pragma unroll
-        for (int i = PW - 1; i >= 0; --i)
-#pragma unroll
-          for (int j = PX - 1; j >= 0; --j) {
-            if (i + j >= 3) continue;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int q = 0; q < NT; ++q)
-                mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
-            first = false;
-          }
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < NT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
-  }
-  cp_async_wait<0>();
-  __syncthreads();                         // the stages become the table of sums
-  float* red = reinterpret_cast<float*>(stages);
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[(warp * 16 + q * 8 + 2 * t + (i & 1)) * kStride + m * 16 + (i >> 1) * 8 + g] = sum[m][q][i];
-  __syncthreads();
-  float* part_sums = red + kShrinkWarps * 16 * kStride;
-  for (int i = threadIdx.x; i < count * RC; i += kShrinkThreads) {
-    const int r = i / RC, j = i - r * RC;
-    part_sums[i] = red[r * kStride + j] + red[(64 + r) * kStride + j];
-  }
-  float* h = P.h[mat] + size_t(row0) * rank + j0;
-  shrink_join(P, part_sums, count * RC, [&](int i, float v) {
-    const int r = i / RC, j = i - r * RC;
-    if (j < ranks) h[size_t(r) * rank + j] = v;
-  });
 }
 
 template <typename TY>
@@ -802,7 +625,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   using Ring = ExpandRing<TY, TW, KC>;
   constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
   extern __shared__ __align__(16) char shared[];
-  __shared__ int rows[16];
+  __shared__ int rows[kAdaptRows];
   __shared__ size_t row_at[16];                            // where they start in y and out
   __shared__ uint32_t mask[kAdaptWindow / 32];
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -845,215 +668,6 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   const int c0 = c_begin + warp * Ring::kCols;
   if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
   else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
-}
-
-// The same for tiles of 64 rows of one stream, 16-bit weights, ranks up to 64 and rows on boundaries of four elements.  What
-// bounds it then is the traffic of the SM's L1 (272 clocks per 16 x 32 values of the form above, of which fragments of B from
-// global memory 128 and those of h 48): so a warp keeps its 16 rows' fragments of h in registers, and B and y pass through
-// shared memory, copied in whole lines, 64 columns a step and two steps ahead.
-// KS: steps of 16 ranks.
-constexpr int kExpandTileStages = 3, kExpandTileCols = 64;
-template <typename TY, int KS>
-__host__ __device__ constexpr int expand_tile_smem() {
-  return kExpandTileStages * (kExpandTileCols * KS * 32 + kExpandWarps * 16 * 32 * int(sizeof(TY)));
-}
-
-template <typename TY, typename TW, int KS>
-__global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_tile_kernel(const AdaptParams P) {
-  constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
-  constexpr int kPitch = KS * 32, kBytesB = kExpandTileCols * kPitch, kUnit = 4 * int(sizeof(TY)), kBytesY = 16 * 8 * kUnit;
-  constexpr int kStage = kBytesB + kExpandWarps * kBytesY;
-  extern __shared__ __align__(128) char shared[];
-  __shared__ int rows[kAdaptMaxRows];
-  __shared__ uint32_t mask[kAdaptWindow / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  int id = -1;
-  const int count = adapt_tile(P, blockIdx.x, rows, mask, &id);
-  int mat = 0;
-  while (mat < P.nmat - 1 && int(blockIdx.y) >= P.chunk_end[mat]) ++mat;
-  const int N = P.n_out[mat], chunk = int(blockIdx.y) - (mat ? P.chunk_end[mat - 1] : 0), rank = P.rank;
-  const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
-  const TY* y = static_cast<const TY*>(P.y[mat]);
-  TY* out = static_cast<TY*>(P.out[mat]);
-  if (id < 0) {
-    if (y != out) adapt_copy<TY, true>(y, out, rows, count, N, c_begin, c_end);
-    return;
-  }
-  const int my_rows = (warp & 3) * 16, my_cols = (warp >> 2) * 32;
-  const size_t row0 = rows[0];
-  // B: a column is a row of kPitch bytes at place_of(column), so that fragment reads (columns 0, 1, 4, 5 of eight by half a warp)
-  // meet no bank twice
-  auto place_of = [](int c) { return (c & ~7) | (c & 1) | ((c >> 1) & 2) | ((c << 1) & 4); };
-  auto turned = [](int place, int unit) { return KS == 4 ? unit ^ ((place & 3) << 1) : KS == 2 ? unit ^ (place & 2) : unit; };
-  const bool wide = rank % 8 == 0;                         // rows of B start on 16 bytes, else on 8
-  // what a thread copies each step: a 16-byte unit (KS 1: for half of the threads) of one column of B, or of two, and four units of y
-  constexpr int kUnitsB = KS * 2, kColsAtOnce = KS == 3 ? 32 : kExpandThreads / kUnitsB < kExpandTileCols ? kExpandThreads / kUnitsB : kExpandTileCols;
-  const int bu = tid % kUnitsB, bc = tid / kUnitsB;
-  const bool b_mine = bc < kColsAtOnce && 8 * bu < rank;
-  const bool b_half = 8 * bu + 4 < rank;                   // not wide: the second half exists
-  const TW* bp = static_cast<const TW*>(P.b[mat]) + (size_t(id) * N + c_begin + (bc < kColsAtOnce ? bc : 0)) * rank + 8 * bu;
-  auto b_at = [&](int c) { return place_of(c) * kPitch + turned(place_of(c), bu) * 16; };
-  auto y_unit = [](int row, int unit) { return row * 8 + (unit ^ (sizeof(TY) == 4 ? (row & 1) << 2 : (row & 2) << 1)); };
-  const int yu = lane & 7, yr = lane >> 3;
-  const TY* yp = y + (row0 + my_rows + (my_rows < count ? min(yr, count - 1 - my_rows) : -my_rows)) * N + c_begin + my_cols + 4 * yu;
-  const int y_rows = (count - my_rows - yr + 3) / 4;       // of the four
-  const size_t y_hop = size_t(4) * N;
-  const uint32_t base = smem_u32(shared), y_to = base + kBytesB + warp * kBytesY + y_unit(yr, yu) * kUnit;
-  // a row four further has the same place among the banks (fp32: rows mod 2, 16 bits: row & 2)
-  int ask = c_begin;                                       // the columns that are requested next
-  uint32_t to = 0;                                         // and the stage they go to, in bytes
-  auto request = [&] {
-    if (ask < c_end) {
-#pragma unroll
-      for (int k = 0; k < kExpandTileCols / kColsAtOnce; ++k) {
-        const int c = bc + k * kColsAtOnce;
-        if (b_mine && ask + c < c_end) {
-          const uint32_t dst = base + to + b_at(c);
-          const TW* src = bp + size_t(k * kColsAtOnce) * rank;
-          if (wide) {
-            cp_async16(dst, src, true);
-          } else {
-            cp_async8(dst, src, true);
-            cp_async8(dst + 8, b_half ? src + 4 : src, b_half);
-          }
-        }
-      }
-      if (ask + my_cols + 4 * yu < c_end) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < y_rows) {
-            if constexpr (sizeof(TY) == 4) cp_async16(y_to + to + k * 4 * 8 * kUnit, yp + k * y_hop, true);
-            else cp_async8(y_to + to + k * 4 * 8 * kUnit, yp + k * y_hop, true);
-          }
-      }
-      ask += kExpandTileCols;
-      bp += size_t(kExpandTileCols) * rank;
-      yp += kExpandTileCols;
-    }
-    cp_async_commit();                                     // a group per step, also an empty one
-    to = to == (kExpandTileStages - 1) * kStage ? 0 : to + kStage;
-  };
-  if (rank < 16 * KS && 8 * bu >= rank && bc < kColsAtOnce)   // ranks that do not exist: zeros, once
-#pragma unroll
-    for (int k = 0; k < kExpandTileCols / kColsAtOnce; ++k)
-      for (int i = 0; i < kExpandTileStages; ++i)
-        *reinterpret_cast<uint4*>(shared + i * kStage + b_at(bc + k * kColsAtOnce)) = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-  for (int i = 0; i < kExpandTileStages - 1; ++i) request();   // none of it comes from the first launch
-  griddep_wait();
-  uint32_t h[KS][PH][4];
-  {
-    const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
-    float4 sum[KS][2];
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = my_rows + e * 8 + g, j = s * 16 + 4 * t;
-        sum[s][e] = i < count && j < rank ? __ldcg(reinterpret_cast<const float4*>(P.h[mat] + (row0 + i) * rank + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t lo[PH], hi[PH];
-        split_pair<PH>(sum[s][e].x * scale, sum[s][e].y * scale, lo);
-        split_pair<PH>(sum[s][e].z * scale, sum[s][e].w * scale, hi);
-#pragma unroll
-        for (int p = 0; p < PH; ++p) { h[s][p][e] = lo[p]; h[s][p][2 + e] = hi[p]; }
-      }
-  }
-  TY* op[2];
-  bool row_ok[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int i = my_rows + e * 8 + g;
-    row_ok[e] = i < count;
-    op[e] = out + (row0 + (row_ok[e] ? i : 0)) * N + my_cols + 4 * t;
-  }
-  const int place = place_of(4 * (g >> 1) + (g & 1));      // of a lane's column of product 0; that of product n: + (n / 2) * 16 + (n % 2) * 4
-  const char* from = shared;
-  for (int c0 = c_begin; c0 < c_end; c0 += kExpandTileCols) {
-    cp_async_wait<kExpandTileStages - 2>();
-    __syncthreads();                                       // the stage has arrived; everyone is done with the one that is requested next
-    request();
-    float acc[4][4];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      uint32_t fb[4][2][PW];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int at = place + (n >> 1) * 16 + (n & 1) * 4 + my_cols;
-        const uint2 v = *reinterpret_cast<const uint2*>(from + at * kPitch + turned(at, 2 * s + (t >> 1)) * 16 + (t & 1) * 8);
-        AdaptRaw<TW, 4> raw;
-        raw.w[0] = v.x; raw.w[1] = v.y;
-        raw.template pair<PW>(0, fb[n][0]);
-        raw.template pair<PW>(1, fb[n][1]);
-      }
-      bool first = s == 0;
-#pragma unroll
-      for (int p = PH - 1; p >= 0; --p)
-#pragma unroll
-        for (int w = PW - 1; w >= 0; --w) {
-          if (p + w >= PH) continue;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) mma_to<false>(first, acc[n], h[s][p], fb[n][0][w], fb[n][1][w]);
-          first = false;
-        }
-    }
-    const char* mine = from + kBytesB + warp * kBytesY;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (row_ok[e] && c0 + my_cols + q * 16 + 4 * t < c_end) {
-          AdaptFour<TY> four;
-          four.load(reinterpret_cast<const TY*>(mine + y_unit(e * 8 + g, 4 * q + t) * kUnit));
-          const float d[4] = {acc[2 * q][2 * e], acc[2 * q][2 * e + 1], acc[2 * q + 1][2 * e], acc[2 * q + 1][2 * e + 1]};
-          four.add_store(op[e] + c0 + q * 16, d);
-        }
-    from = from == shared + (kExpandTileStages - 1) * kStage ? shared : from + kStage;
-  }
-  cp_async_wait<0>();
-}
-
-struct AdaptShape {
-  int rt, tiles, splits, mt;               // first launch: rows of a tile, tiles, splits of K, ranks of a CTA in 16
-  bool tiled;                              // second launch: the form for 64 rows, else for 16
-  int tiles2, kc, chunk_cols, chunks;      // its tiles, ranks per stage, columns of a CTA
-};
-
-inline int adapt_tiles(int streams, int T, int rt) { return T < rt ? streams : streams * ((T + rt - 1) / rt); }
-
-// Rows of a tile: 64 where streams have that many (a tile reads its adapter once), else 16; the second launch has its form for
-// 64 rows for 16-bit weights, ranks up to 64 and rows that start on boundaries of four elements (`vec`).
-// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.
-// Columns of a CTA of the second launch: what its warps take at a time, times what leaves three CTAs per SM (gathered tiles: each
-// starts with a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40) or six (tiles of 64 rows,
-// whose last wave costs more; 3B ffn for 8192 rows 222, 217, 204).
-inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool vec, int sms) {
-  AdaptShape s;
-  s.rt = T >= kAdaptMaxRows ? kAdaptMaxRows : 16;
-  s.tiled = s.rt == kAdaptMaxRows && w_pieces < 3 && rank <= 64 && vec;
-  s.tiles = adapt_tiles(streams, T, s.rt);
-  s.tiles2 = adapt_tiles(streams, T, s.tiled ? kAdaptMaxRows : 16);
-  auto busy = [&](int tiles, int rt) {                   // tiles that lead rows
-    const long long most = adapters + (long long)streams * T / rt + 1;
-    return T < rt && most < tiles ? most : (long long)tiles;
-  };
-  s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
-  s.kc = rank <= 16 ? 16 : 32;
-  const long long ctas = busy(s.tiles, s.rt) * nmat * ((rank + 16 * s.mt - 1) / (16 * s.mt));
-  s.splits = 1;
-  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
-  const int unit = s.tiled ? kExpandTileCols : kExpandWarps * (w_pieces < 3 ? 64 : 32);
-  long long units = 0;
-  for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  long long per = units * busy(s.tiles2, s.tiled ? kAdaptMaxRows : 16) / ((s.tiled ? 6LL : 3LL) * sms);
-  s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
-  s.chunks = 0;
-  for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
-  return s;
 }
 
 }  // namespace b200

@@ -1,0 +1,491 @@
+// The two launches of adapters.cuh for streams of many rows, on the 5th-generation tensor cores: tiles of 128 rows of one
+// stream, whose adapter is read once per tile.
+//
+// The operands are the same bfloat16 pieces (or values of one 16-bit type), cut by the threads that bring them and laid out
+// in shared memory as the MMAs want them: rows of 64 elements, 128-byte swizzle.  At rank 64 and fp32 rows the pieces are
+// 26 multiplications a byte, which mma.sync just about kept up with (and less under the power cap); tcgen05 leaves the
+// memory as the bound.  Every wait is bounded; where one runs out the rows concerned come out as NaN.
+#pragma once
+
+#include "adapters.cuh"
+#include "dense_gemm.cuh"
+
+namespace b200 {
+
+constexpr int kAdaptTile = 128;            // rows of a tile; columns of a step of the second launch
+constexpr int kTileBytes = kAdaptTile * 128;         // 128 rows of 64 elements
+constexpr int kTileRankMax = 128;          // of the second launch: two times 64 ranks
+
+__device__ __forceinline__ void fence_smem_to_mma() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int COLS>
+__device__ __forceinline__ void tmem_alloc_cols(uint32_t slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "n"(COLS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int COLS>
+__device__ __forceinline__ void tmem_free_cols(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
+}
+// 16 consecutive columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Where unit `u` (16 bytes) of a row lies in a tile of 128-byte rows.
+__device__ __forceinline__ int tile_unit(int row, int u) { return row * 128 + ((u ^ (row & 7)) << 4); }
+
+// Barriers and flags at the front of dynamic shared memory (1024 bytes, so that the tiles behind are aligned).
+struct TileControl {
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], h_full;
+  int abort;
+  uint32_t tmem;
+};
+__device__ __forceinline__ TileControl* tile_control(char* shared) { return reinterpret_cast<TileControl*>(shared); }
+
+// ---------------------------------------------------------------------------------------------- the first launch
+// h[row][j] = sum_k x[row][k] A[id][j][k] for 128 rows (the MMAs' M, a TMEM lane each) and up to 64 ranks (their N).  Eight warps
+// bring 64 k of x and A at a time, requested one stage ahead, cut them into pieces and store them; one warp issues the MMAs.
+// Two stages make a sum: its 24 additions are cut off by the tensor cores (rank 64, fp32 x, bf16 A: 12 MMAs each), so the eight
+// warps add it up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
+constexpr int kShrinkTileWorkers = 256, kShrinkTileThreads = kShrinkTileWorkers + 32, kShrinkTileRanks = 64;
+
+template <typename TX, typename TW>
+struct ShrinkTile {
+  static constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
+  static constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
+  static constexpr int kBytesX = PX * kTileBytes, kStage = kBytesX + PW * kTileBytes / 2;
+  static constexpr int kStages = kStage <= 28 * 1024 ? 4 : kStage <= 56 * 1024 ? 2 : kStage <= 64 * 1024 ? 3 : 2;
+  static constexpr int kPitch = kShrinkTileRanks + 1, kTable = kAdaptTile * kPitch * 4;
+  static constexpr int kSmem = 1024 + (kStages * kStage > kTable ? kStages * kStage : kTable);
+  // loads of a thread: 16 bytes each
+  static constexpr int kUnitX = 16 / int(sizeof(TX)), kRowX = 64 / kUnitX, kHopX = kShrinkTileWorkers / kRowX, kLoadX = kAdaptTile / kHopX;
+  static constexpr int kUnitW = 16 / int(sizeof(TW)), kRowW = 64 / kUnitW, kHopW = kShrinkTileWorkers / kRowW, kLoadW = kShrinkTileRanks / kHopW;
+};
+
+// One 16-byte load of T as P pieces into tiles `hop` bytes apart: eight elements are a unit, four (fp32) half of one.
+template <typename T, int P>
+__device__ __forceinline__ void tile_put(char* tile, int hop, int row, int load, uint4 v) {
+  if constexpr (P == 1) {
+    *reinterpret_cast<uint4*>(tile + tile_unit(row, load)) = v;
+  } else if constexpr (sizeof(T) == 4) {
+    uint32_t a[P], b[P];
+    split_pair<P>(__uint_as_float(v.x), __uint_as_float(v.y), a);
+    split_pair<P>(__uint_as_float(v.z), __uint_as_float(v.w), b);
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<uint2*>(tile + p * hop + tile_unit(row, load >> 1) + (load & 1) * 8) = make_uint2(a[p], b[p]);
+  } else {
+    uint32_t f[4][P];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      split_pair<P>(x.x, x.y, f[i]);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(tile + p * hop + tile_unit(row, load)) = make_uint4(f[0][p], f[1][p], f[2][p], f[3][p]);
+  }
+}
+
+template <typename TX, typename TW>
+__global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem <= 113 * 1024 ? 2 : 1) adapt_shrink_tile_kernel(const AdaptParams P) {
+  using S = ShrinkTile<TX, TW>;
+  extern __shared__ __align__(1024) char shared[];
+  TileControl& C = *tile_control(shared);
+  char* stages = shared + 1024;
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  const int tile = blockIdx.x / P.splits, split = blockIdx.x - tile * P.splits, mat = blockIdx.z;
+  const int per = (P.T + kAdaptTile - 1) / kAdaptTile, s = tile / per, first = (tile - s * per) * kAdaptTile;
+  const int count = min(kAdaptTile, P.T - first), row0 = s * P.T + first, K = P.K, rank = P.rank;
+  const long long asked = __ldg(P.ids + s);
+  if (asked < 0 || asked >= P.adapters) return;            // the whole cluster
+  const int j0 = blockIdx.y * kShrinkTileRanks, ranks = min(kShrinkTileRanks, rank - j0), n16 = (ranks + 15) / 16 * 16;
+  const int chunks = (K + 63) / 64, c0 = int((long long)chunks * split / P.splits), c1 = int((long long)chunks * (split + 1) / P.splits);
+  const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty);
+  volatile int* abort_flag = &C.abort;
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) { mbar_init(full + 8 * i, kShrinkTileWorkers); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kShrinkTileWorkers / 32); }
+    C.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kShrinkTileWorkers / 32) tmem_alloc_cols<128>(smem_u32(&C.tmem));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
+  griddep_launch_dependents();                             // only now: the second launch takes tensor memory too
+  float sum[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sum[i] = 0.f;
+  const int q = warp & 3, half = warp >> 2;                // workers: TMEM lanes 32 q .., ranks 32 half ..
+  if (warp < kShrinkTileWorkers / 32) {
+    const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
+    const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
+    const int ux = tid % S::kRowX, rx = tid / S::kRowX, uw = tid % S::kRowW, rw = tid / S::kRowW;
+    uint4 vx[S::kLoadX], vw[S::kLoadW];
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    auto load = [&](int c) {
+      const int kx = c * 64 + ux * S::kUnitX, kw = c * 64 + uw * S::kUnitW;
+#pragma unroll
+      for (int i = 0; i < S::kLoadX; ++i) {
+        const int r = rx + i * S::kHopX;
+        vx[i] = r < count && kx < K ? __ldg(reinterpret_cast<const uint4*>(x + size_t(r) * K + kx)) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < S::kLoadW; ++i) {
+        const int r = rw + i * S::kHopW;
+        vw[i] = r < ranks && kw < K ? __ldg(reinterpret_cast<const uint4*>(a + size_t(r) * K + kw)) : zero;
+      }
+    };
+    bool ok = true;
+    auto flush = [&](int g) {                              // the sum of stages 2 g and 2 g + 1
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * (g & 1), uint32_t(g >> 1) & 1u, abort_flag));
+      if (!ok) return;
+      tc_fence_after();
+      if (half * 32 < n16) {
+        float v[2][16];
+        const uint32_t at = tmem + (uint32_t(q * 32) << 16) + uint32_t((g & 1) * 64 + half * 32);
+        tmem_ld16(at, v[0]);
+        if (half * 32 + 16 < n16) tmem_ld16(at + 16, v[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i] += v[0][i];
+        if (half * 32 + 16 < n16)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[16 + i] += v[1][i];
+      }
+      tc_fence_before();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * (g & 1));
+    };
+    load(c0);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int c = c0; c < c1 && ok; ++c) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag));
+      if (!ok) break;
+      char* to = stages + slot * S::kStage;
+#pragma unroll
+      for (int i = 0; i < S::kLoadX; ++i) tile_put<TX, S::PX>(to, kTileBytes, rx + i * S::kHopX, ux, vx[i]);
+#pragma unroll
+      for (int i = 0; i < S::kLoadW; ++i) tile_put<TW, S::PW>(to + S::kBytesX, kTileBytes / 2, rw + i * S::kHopW, uw, vw[i]);
+      if (c + 1 < c1) load(c + 1);
+      fence_smem_to_mma();
+      mbar_arrive(full + 8 * slot);
+      if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
+      const int n = c - c0;
+      if (n >= 2 && (n & 1) == 0) flush(n / 2 - 1);
+    }
+    if (ok) flush((c1 - c0 + 1) / 2 - 1);                  // the others have been
+    if (!ok)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum[i] = NAN;
+  } else {
+    const uint32_t idesc = umma_idesc_f16(kAdaptTile, n16, !(S::kSame && std::is_same<TX, __half>::value));
+    const uint32_t base = smem_u32(stages);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int c = c0; c < c1; ++c) {
+      const int n = c - c0, g = n >> 1;
+      if ((n & 1) == 0 && !warp_wait(acc_empty + 8 * (g & 1), (uint32_t(g >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0)) break;
+      if (!warp_wait(full + 8 * slot, phase, abort_flag, nullptr, 0)) break;
+      if (elect_one()) {
+        tc_fence_after();
+        const uint32_t at = base + slot * S::kStage, d = tmem + uint32_t((g & 1) * 64);
+        uint32_t more = (n & 1) != 0;
+#pragma unroll
+        for (int i = S::PW - 1; i >= 0; --i)
+#pragma unroll
+          for (int j = S::PX - 1; j >= 0; --j) {
+            if (i + j >= 3) continue;
+            const uint64_t ad = umma_desc(at + j * kTileBytes), bd = umma_desc(at + S::kBytesX + i * (kTileBytes / 2));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              umma_f16<false>(d, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc, more);
+              more = 1u;
+            }
+          }
+        umma_commit<false>(empty + 8 * slot);
+        if ((n & 1) != 0 || c + 1 == c1) umma_commit<false>(acc_full + 8 * (g & 1));
+      }
+      __syncwarp();
+      if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
+    }
+  }
+  // every MMA is over (the workers saw the last sum): the stages become the table of sums
+  float* table = reinterpret_cast<float*>(stages);
+  if (warp < kShrinkTileWorkers / 32) {
+    float* mine = table + (q * 32 + lane) * S::kPitch + half * 32;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mine[i] = sum[i];
+  }
+  tc_fence_before();
+  float* h = P.h[mat] + size_t(row0) * rank + j0;
+  shrink_join(P, table, count * kShrinkTileRanks, [&](int i) { return i / kShrinkTileRanks * S::kPitch + i % kShrinkTileRanks; },
+              [&](int i, float v) {
+                const int r = i / kShrinkTileRanks, j = i % kShrinkTileRanks;
+                if (j < ranks) h[size_t(r) * rank + j] = v;
+              });
+  if (warp == kShrinkTileWorkers / 32) {
+    tc_fence_after();
+    tmem_free_cols<128>(tmem);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- the second launch
+// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j] for 128 rows (the MMAs' N) and 128 columns a step (their M, a TMEM
+// lane each), so that a warp's access to y and out is one line of a row whatever its length.  Four warps bring B and cut it into
+// pieces, one issues the MMAs, eight hold y of 16 rows at a time in registers, requested in front of the accumulator, add and
+// store; two accumulators.  The pieces of h are laid out once.
+constexpr int kExpandTileLoaders = 128, kExpandTileAdders = 256, kExpandTileThreads = kExpandTileLoaders + kExpandTileAdders + 32;
+
+template <typename TY, typename TW>
+struct ExpandTile {
+  static constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  // for `halves` times 64 ranks: as many stages as leave room for two CTAs, else two
+  __host__ __device__ static constexpr int stages(int halves) {
+    const int n = (113 * 1024 - 1024 - PH * halves * kTileBytes) / (PW * halves * kTileBytes);
+    return n > 4 ? 4 : n < 2 ? (1024 + (PH + 2 * PW) * halves * kTileBytes <= 226 * 1024 ? 2 : 1) : n;
+  }
+  __host__ __device__ static constexpr int smem(int halves) { return 1024 + (PH + stages(halves) * PW) * halves * kTileBytes; }
+};
+
+template <typename TY, typename TW>
+__global__ void __launch_bounds__(kExpandTileThreads, 2) adapt_expand_tile_kernel(const AdaptParams P) {
+  using S = ExpandTile<TY, TW>;
+  constexpr int PH = S::PH, PW = S::PW;
+  extern __shared__ __align__(1024) char shared[];
+  TileControl& C = *tile_control(shared);
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  const int per = (P.T + kAdaptTile - 1) / kAdaptTile, s = blockIdx.x / per, first = (int(blockIdx.x) - s * per) * kAdaptTile;
+  const int count = min(kAdaptTile, P.T - first), row0 = s * P.T + first;
+  int mat = 0;
+  while (mat < P.nmat - 1 && int(blockIdx.y) >= P.chunk_end[mat]) ++mat;
+  const int N = P.n_out[mat], chunk = int(blockIdx.y) - (mat ? P.chunk_end[mat - 1] : 0), rank = P.rank;
+  const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
+  const TY* y = static_cast<const TY*>(P.y[mat]);
+  TY* out = static_cast<TY*>(P.out[mat]);
+  const long long asked = __ldg(P.ids + s);
+  if (asked < 0 || asked >= P.adapters) {                  // no adapter: only a copy, where out is not y
+    if (y == out) return;
+    for (int r = warp; r < count; r += kExpandTileThreads / 32) {
+      const size_t at = size_t(row0 + r) * N;
+      for (int c = c_begin + lane; c < c_end; c += 32 * 16) {
+        TY v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (c + 32 * k < c_end) v[k] = y[at + c + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (c + 32 * k < c_end) out[at + c + 32 * k] = v[k];
+      }
+    }
+    return;
+  }
+  const int ksteps = (rank + 15) / 16, halves = (rank + 63) / 64, NS = P.stages, h_piece = halves * kTileBytes, stage_bytes = PW * h_piece;
+  char *h_tiles = shared + 1024, *stages = h_tiles + PH * h_piece;
+  const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty), h_full = smem_u32(&C.h_full);
+  volatile int* abort_flag = &C.abort;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) { mbar_init(full + 8 * i, kExpandTileLoaders); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kExpandTileAdders / 32); }
+    mbar_init(h_full, kExpandTileAdders);
+    C.abort = 0;
+    fence_mbar_init();
+  }
+  constexpr int kMmaWarp = (kExpandTileLoaders + kExpandTileAdders) / 32;
+  if (warp == kMmaWarp) tmem_alloc_cols<256>(smem_u32(&C.tmem));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
+  const int steps = (c_end - c_begin + kAdaptTile - 1) / kAdaptTile;
+  if (warp < kExpandTileLoaders / 32) {
+    // ---- B: units of eight ranks of a column; neither it nor y comes from the first launch
+    const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(asked) * N * rank;
+    const int units = halves * 8, u = tid % units, hop = kExpandTileLoaders / units, j = u * 8;
+    const bool wide = rank * int(sizeof(TW)) % 16 == 0, used = u < 2 * ksteps;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int it = 0; it < steps; ++it) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag))) break;
+      char* to = stages + slot * stage_bytes + (u >> 3) * kTileBytes;
+      const int c0 = c_begin + it * kAdaptTile;
+      if (used)
+        for (int c = tid / units; c < kAdaptTile; c += 4 * hop) {
+          uint4 v[4][sizeof(TW) / 2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const TW* src = b + size_t(c0 + c + i * hop) * rank + j;
+            const bool in = c + i * hop < kAdaptTile && c0 + c + i * hop < c_end;
+            if constexpr (sizeof(TW) == 4) {
+              v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
+              v[i][1] = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint4*>(src) + 1) : zero;
+            } else if (wide) {
+              v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
+            } else {
+              const uint2 lo = in && j < rank ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
+              const uint2 hi = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint2*>(src) + 1) : make_uint2(0u, 0u);
+              v[i][0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i * hop < kAdaptTile) {
+              if constexpr (sizeof(TW) == 4) {
+                tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2, v[i][0]);
+                tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2 + 1, v[i][1]);
+              } else {
+                tile_put<TW, PW>(to, h_piece, c + i * hop, u & 7, v[i][0]);
+              }
+            }
+        }
+      fence_smem_to_mma();
+      mbar_arrive(full + 8 * slot);
+      if (++slot == NS) { slot = 0; phase ^= 1u; }
+    }
+  } else if (warp < kMmaWarp) {
+    const int q = warp & 3, part = (warp - kExpandTileLoaders / 32) >> 2;      // TMEM lanes 32 q .., every second 16 rows
+    griddep_wait();
+    {
+      const float scale = P.scale[mat] ? __ldg(P.scale[mat] + asked) : 1.f;
+      const int r4 = ksteps * 4, n16 = (count + 15) / 16 * 16;                 // groups of four ranks; rows
+      for (int i = tid - kExpandTileLoaders; i < n16 * r4; i += kExpandTileAdders) {
+        const int r = i / r4, j4 = i - r * r4, jj = j4 * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < count && jj < rank) v = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(row0 + r) * rank + jj));
+        uint32_t lo[PH], hi[PH];
+        split_pair<PH>(v.x * scale, v.y * scale, lo);
+        split_pair<PH>(v.z * scale, v.w * scale, hi);
+        char* at = h_tiles + (j4 >> 4) * kTileBytes + tile_unit(r, (j4 & 15) >> 1) + (j4 & 1) * 8;
+#pragma unroll
+        for (int p = 0; p < PH; ++p) *reinterpret_cast<uint2*>(at + p * h_piece) = make_uint2(lo[p], hi[p]);
+      }
+      fence_smem_to_mma();
+      mbar_arrive(h_full);
+    }
+    const int groups = (count + 15) / 16;
+    bool ok = true;
+    for (int it = 0; it < steps; ++it) {
+      const int n = c_begin + it * kAdaptTile + q * 32 + lane, buf = it & 1;
+      const bool in = n < c_end;
+      const TY* yp = y + size_t(row0) * N + (in ? n : c_begin);
+      TY* op = out + size_t(row0) * N + n;
+      TY v[16];
+      auto fetch = [&](int grp) {
+        const TY* p = yp + size_t(grp * 16) * N;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (grp * 16 + i < count) v[i] = *p;
+          p += N;
+        }
+      };
+      if (part < groups) fetch(part);
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * buf, uint32_t(it >> 1) & 1u, abort_flag));
+      tc_fence_after();
+      for (int grp = part; grp < groups; grp += 2) {
+        float d[16];
+        if (ok) {
+          tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * kAdaptTile + grp * 16), d);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d[i] = NAN;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] += adapt_float(v[i]);
+        if (grp + 2 < groups) fetch(grp + 2);
+        TY* p = op + size_t(grp * 16) * N;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (in && grp * 16 + i < count) adapt_store(p, d[i]);
+          p += N;
+        }
+      }
+      tc_fence_before();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+    }
+  } else {
+    const uint32_t idesc = umma_idesc_f16(kAdaptTile, (count + 15) / 16 * 16, 1);
+    const uint32_t h_at = smem_u32(h_tiles), base = smem_u32(stages);
+    bool ok = warp_wait(h_full, 0u, abort_flag, nullptr, 0);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int it = 0; it < steps && ok; ++it) {
+      const int buf = it & 1;
+      if (!warp_wait(acc_empty + 8 * buf, (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0)) break;
+      if (!warp_wait(full + 8 * slot, phase, abort_flag, nullptr, 0)) break;
+      if (elect_one()) {
+        tc_fence_after();
+        const uint32_t d = tmem + uint32_t(buf * kAdaptTile);
+        uint32_t more = 0u;
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = uint32_t((k >> 2) * kTileBytes + (k & 3) * 32);
+#pragma unroll
+          for (int p = PH - 1; p >= 0; --p)
+#pragma unroll
+            for (int w = PW - 1; w >= 0; --w) {
+              if (p + w >= PH) continue;
+              umma_f16<false>(d, umma_desc(base + slot * stage_bytes + w * h_piece + off), umma_desc(h_at + p * h_piece + off), idesc, more);
+              more = 1u;
+            }
+        }
+        umma_commit<false>(empty + 8 * slot);
+        umma_commit<false>(acc_full + 8 * buf);
+      }
+      __syncwarp();
+      if (++slot == NS) { slot = 0; phase ^= 1u; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_free_cols<256>(tmem);
+  }
+}
+
+struct AdaptShape {
+  bool tiles1, tiles2;                     // the forms for 128 rows of a stream, else for gathered tiles of 16
+  int n1, n2;                              // tiles that a launch has at most
+  int splits, mt;                          // first launch: CTAs that share K; gathered: ranks of a CTA in 16
+  int kc, chunk_cols, chunks;              // second launch: gathered: ranks per stage; columns of a CTA
+};
+
+// Streams of 64 rows or more are cut into tiles of 128 (ranks up to 128 in the second launch, whose h stays in shared memory);
+// shorter ones are gathered.  Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or
+// more k each.  Columns of a CTA of the second launch: what it takes at a time, times what leaves three CTAs per SM (gathered
+// tiles: each starts with a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40) or four.
+inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
+  AdaptShape s;
+  auto tiles = [&](int rows) { return T < rows ? streams : streams * ((T + rows - 1) / rows); };
+  auto cut = [&](int rows) { return streams * ((T + rows - 1) / rows); };
+  s.tiles1 = T >= 64;
+  s.tiles2 = T >= 64 && rank <= kTileRankMax;
+  s.n1 = s.tiles1 ? cut(kAdaptTile) : tiles(kAdaptRows);
+  s.n2 = s.tiles2 ? cut(kAdaptTile) : tiles(kAdaptRows);
+  auto busy = [&](int n, bool tiled) {                   // tiles that lead rows
+    const long long most = adapters + (long long)streams * T / kAdaptRows + 1;
+    return !tiled && T < kAdaptRows && most < n ? most : (long long)n;
+  };
+  s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
+  s.kc = rank <= 16 ? 16 : 32;
+  const int per_cta = s.tiles1 ? kShrinkTileRanks : 16 * s.mt;
+  const long long ctas = busy(s.n1, s.tiles1) * nmat * ((rank + per_cta - 1) / per_cta);
+  s.splits = 1;
+  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
+  const int unit = s.tiles2 ? kAdaptTile : kExpandWarps * (w_pieces < 3 ? 64 : 32);
+  long long units = 0;
+  for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
+  long long per = units * busy(s.n2, s.tiles2) / ((s.tiles2 ? 4LL : 3LL) * sms);
+  s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
+  s.chunks = 0;
+  for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
+  return s;
+}
+
+}  // namespace b200

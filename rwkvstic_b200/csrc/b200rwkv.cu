@@ -15,6 +15,7 @@
 #include "dense_step.cuh"
 #include "dense_gemm.cuh"
 #include "adapters.cuh"
+#include "adapters_tiles.cuh"
 #include "verify.cuh"
 #include "advance.cuh"
 
@@ -733,27 +734,41 @@ static cudaError_t launch_sample(const float* x, int rows, int n, long long ldx,
 }
 
 // ---------------------------------------------------------------------------------------- adapters, verification
-template <typename TX, typename TW, int MT>
-static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  const dim3 grid(sh.tiles * P.splits, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat);
-  constexpr int few = ShrinkRing<TX, TW, MT>::kSmem, many = shrink_tile_smem<TX, TW, MT>();
-  static bool configured[64];
+// Dynamic shared memory beyond 48 KB has to be asked for, once per kernel and device.
+template <typename Kernel>
+static cudaError_t allow_smem(Kernel kernel, int bytes, bool (&configured)[64]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_shrink_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, few);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(adapt_shrink_tile_kernel<TX, TW, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, many);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  if (sh.rt == 16) return launch_clustered(P.splits, adapt_shrink_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), few, stream, P);
-  return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW, MT>, grid, dim3(kShrinkThreads), many, stream, P);
+  return cudaSuccess;
+}
+
+template <typename TX, typename TW, int MT>
+static cudaError_t launch_adapt_shrink_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  static bool configured[64];
+  constexpr int smem = ShrinkRing<TX, TW, MT>::kSmem;
+  const cudaError_t e = allow_smem(adapt_shrink_kernel<TX, TW, MT>, smem, configured);
+  if (e != cudaSuccess) return e;
+  return launch_clustered(P.splits, adapt_shrink_kernel<TX, TW, MT>, dim3(sh.n1 * P.splits, (P.rank + 16 * MT - 1) / (16 * MT), P.nmat),
+                          dim3(kShrinkThreads), smem, stream, P);
 }
 
 template <typename TX, typename TW>
 static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
+  if (sh.tiles1) {
+    static bool configured[64];
+    constexpr int smem = ShrinkTile<TX, TW>::kSmem;
+    const cudaError_t e = allow_smem(adapt_shrink_tile_kernel<TX, TW>, smem, configured);
+    if (e != cudaSuccess) return e;
+    return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW>, dim3(sh.n1 * P.splits, (P.rank + kShrinkTileRanks - 1) / kShrinkTileRanks, P.nmat),
+                            dim3(kShrinkTileThreads), smem, stream, P);
+  }
   if (sh.mt == 1) return launch_adapt_shrink_as<TX, TW, 1>(P, sh, stream);
   if (sh.mt == 2) return launch_adapt_shrink_as<TX, TW, 2>(P, sh, stream);
   if constexpr (AdaptType<TW>::kPieces == 1) return launch_adapt_shrink_as<TX, TW, 4>(P, sh, stream);
@@ -764,45 +779,23 @@ template <typename TY, typename TW, int KC, bool VEC>
 static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
   constexpr int warps = kExpandWarps * ExpandRing<TY, TW, KC>::kWarp;
   static bool configured[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = allow_smem(adapt_expand_kernel<TY, TW, KC, VEC>, warps + expand_h_bytes<TY>(kAdaptMaxRank, KC), configured);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_expand_kernel<TY, TW, KC, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             warps + expand_h_bytes<TY>(kAdaptMaxRank, KC));
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  return launch_chained(adapt_expand_kernel<TY, TW, KC, VEC>, dim3(sh.tiles2, sh.chunks), dim3(kExpandThreads),
+  return launch_chained(adapt_expand_kernel<TY, TW, KC, VEC>, dim3(sh.n2, sh.chunks), dim3(kExpandThreads),
                         size_t(warps) + expand_h_bytes<TY>(P.rank, KC), stream, P);
 }
 
-template <typename TY, typename TW, int KS>
-static cudaError_t launch_adapt_expand_tile(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
-  constexpr int smem = expand_tile_smem<TY, KS>();
-  static bool configured[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    e = cudaFuncSetAttribute(adapt_expand_tile_kernel<TY, TW, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  return launch_chained(adapt_expand_tile_kernel<TY, TW, KS>, dim3(sh.tiles2, sh.chunks), dim3(kExpandThreads), smem, stream, P);
-}
-
 template <typename TY, typename TW>
-static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
-  if constexpr (sizeof(TW) == 2)
-    if (sh.tiled) switch ((P.rank + 15) / 16) {
-      case 1: return launch_adapt_expand_tile<TY, TW, 1>(P, sh, stream);
-      case 2: return launch_adapt_expand_tile<TY, TW, 2>(P, sh, stream);
-      case 3: return launch_adapt_expand_tile<TY, TW, 3>(P, sh, stream);
-      default: return launch_adapt_expand_tile<TY, TW, 4>(P, sh, stream);
-    }
+static cudaError_t launch_adapt_expand(AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+  if (sh.tiles2) {
+    using S = ExpandTile<TY, TW>;
+    static bool configured[64];
+    const int halves = (P.rank + 63) / 64;
+    const cudaError_t e = allow_smem(adapt_expand_tile_kernel<TY, TW>, S::smem(1) > S::smem(2) ? S::smem(1) : S::smem(2), configured);
+    if (e != cudaSuccess) return e;
+    P.stages = S::stages(halves);
+    return launch_chained(adapt_expand_tile_kernel<TY, TW>, dim3(sh.n2, sh.chunks), dim3(kExpandTileThreads), S::smem(halves), stream, P);
+  }
   if (sh.kc == 16) return vec ? launch_adapt_expand_as<TY, TW, 16, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 16, false>(P, sh, stream);
   return vec ? launch_adapt_expand_as<TY, TW, 32, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 32, false>(P, sh, stream);
 }
@@ -810,9 +803,7 @@ static cudaError_t launch_adapt_expand(const AdaptParams& P, const AdaptShape& s
 template <typename TY, typename TW>
 static cudaError_t launch_adapt(AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   g_chain_launch = false;        // the first launch waits for the work in front of the call, which may still write its inputs
-  P.rt = sh.rt;
   cudaError_t e = launch_adapt_shrink<TY, TW>(P, sh, stream);
-  P.rt = sh.tiled ? kAdaptMaxRows : 16;
   return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, vec, stream) : e;
 }
 
@@ -2052,7 +2043,7 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
     P.h[i] = reinterpret_cast<float*>(static_cast<char*>(workspace) + size_t(i) * (need / nmat));
     vec = vec && m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
   }
-  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), vec, device_sms());
+  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), device_sms());
   for (int i = 0; i < nmat; ++i) P.chunk_end[i] = (i ? P.chunk_end[i - 1] : 0) + (P.n_out[i] + sh.chunk_cols - 1) / sh.chunk_cols;
   P.ids = reinterpret_cast<const long long*>(ids);
   P.nmat = nmat; P.adapters = n_adapters; P.rank = rank; P.K = k_in; P.R = streams * tokens_per_stream; P.T = tokens_per_stream;
