@@ -44,7 +44,7 @@ struct AdaptParams {
   int n_out[kAdaptMaxMats];
   int chunk_end[kAdaptMaxMats];            // second launch: column chunks of the matrices up to and including this one
   const long long* ids;
-  int nmat, adapters, rank, K, R, T, streams, splits, chunk_cols, stages;
+  int nmat, adapters, rank, K, R, T, streams, splits, chunk_cols, stages, ring;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -141,6 +141,14 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
         vw[i] = r < ranks && kw < K ? __ldg(reinterpret_cast<const uint4*>(a + size_t(r) * K + kw)) : zero;
       }
     };
+    // ask L2 for the lines of x some stages further on: registers hold one stage, which is too little to keep HBM busy
+    constexpr int kLines = 64 * int(sizeof(TX)) / 128, kAhead = 4;
+    auto ask = [&](int c) {
+      const int r = tid / kLines, k = c * 64 + tid % kLines * (128 / int(sizeof(TX)));
+      if (c < c1 && r < count && k < K) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + size_t(r) * K + k));
+    };
+#pragma unroll
+    for (int i = 1; i < kAhead; ++i) ask(c0 + i);
     bool ok = true;
     auto flush = [&](int g) {                              // the sum of stages 2 g and 2 g + 1
       ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * (g & 1), uint32_t(g >> 1) & 1u, abort_flag));
@@ -173,6 +181,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
 #pragma unroll
       for (int i = 0; i < S::kLoadW; ++i) tile_put<TW, S::PW>(to + S::kBytesX, kTileBytes / 2, rw + i * S::kHopW, uw, vw[i]);
       if (c + 1 < c1) load(c + 1);
+      ask(c + kAhead);
       fence_smem_to_mma();
       mbar_arrive(full + 8 * slot);
       if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
@@ -236,209 +245,329 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
 }
 
 // ---------------------------------------------------------------------------------------------- the second launch
-// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j] for 128 rows (the MMAs' N) and 128 columns a step (their M, a TMEM
-// lane each), so that a warp's access to y and out is one line of a row whatever its length.  Four warps bring B and cut it into
-// pieces, one issues the MMAs, eight hold y of 16 rows at a time in registers, requested in front of the accumulator, add and
-// store; two accumulators.  The pieces of h are laid out once.
-constexpr int kExpandTileLoaders = 128, kExpandTileAdders = 256, kExpandTileThreads = kExpandTileLoaders + kExpandTileAdders + 32;
+// out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j] for tiles of 128 rows (the MMAs' N) and 128 columns a step (their M,
+// a TMEM lane each).  One persistent CTA per SM takes an equal share of all steps of all tiles and matrices, in order; a
+// segment is what it has of one tile and matrix, whose pieces of h it lays out once.
+//   warps 0..3   bring B and cut it into pieces, a step at a time
+//   warps 4..11  add: a warp has 32 columns (lanes) and every second 16 rows of a half step
+//   warp 12      issues the MMAs; two accumulators
+//   warp 13      requests y, 64 rows x 128 columns a half step, in TMA boxes of 16 rows, up to four half steps ahead
+// Sums are added in place in shared memory, with the lanes along a row, and leave in the same boxes (as bulk copies of single
+// rows, 512 bytes each, both ways took 215 us for 8192 rows of a 3B ffn).  What bounds it is memory: 128
+// bytes per 16 values pass the SM.  The same tiles with y through registers were bound by the L1 lines that loads in flight
+// occupy beside 226 KB of shared memory (3B ffn, 8192 rows: 190 us for 839 MB), mma.sync by its own rate under the power cap.
+// A tile without an adapter goes through unchanged, or is left out where out is y.
+constexpr int kExpandTileLoaders = 128, kExpandTileAdders = 256, kExpandTileThreads = kExpandTileLoaders + kExpandTileAdders + 64;
+constexpr int kExpandTileRing = 4, kExpandHalf = 64;       // half steps of y in shared memory, at most; rows of one
+
+struct ExpandTileControl {
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], h_full, y_full[kExpandTileRing], y_empty[kExpandTileRing];
+  int abort;
+  uint32_t tmem;
+};
 
 template <typename TY, typename TW>
 struct ExpandTile {
   static constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
-  // for `halves` times 64 ranks: as many stages as leave room for two CTAs, else two
-  __host__ __device__ static constexpr int stages(int halves) {
-    const int n = (113 * 1024 - 1024 - PH * halves * kTileBytes) / (PW * halves * kTileBytes);
-    return n > 4 ? 4 : n < 2 ? (1024 + (PH + 2 * PW) * halves * kTileBytes <= 226 * 1024 ? 2 : 1) : n;
+  static constexpr int kRow = kAdaptTile * int(sizeof(TY)), kHalfBytes = kExpandHalf * kRow;
+  // for `halves` times 64 ranks: half steps of y (2 to 4) that leave room for a stage of B beside h, 0 where none do; then stages
+  // of B, at most 4
+  __host__ __device__ static constexpr int room(int halves, int ring) { return 226 * 1024 - 1024 - ring * kHalfBytes - PH * halves * kTileBytes; }
+  __host__ __device__ static constexpr int ring(int halves) {
+    for (int n = kExpandTileRing; n >= 2; --n)
+      if (room(halves, n) >= PW * halves * kTileBytes) return n;
+    return 0;
   }
-  __host__ __device__ static constexpr int smem(int halves) { return 1024 + (PH + stages(halves) * PW) * halves * kTileBytes; }
+  __host__ __device__ static constexpr int stages(int halves) {
+    const int n = ring(halves) ? room(halves, ring(halves)) / (PW * halves * kTileBytes) : 0;
+    return n > 4 ? 4 : n;
+  }
+  __host__ __device__ static constexpr int smem(int halves) { return 1024 + ring(halves) * kHalfBytes + (PH + stages(halves) * PW) * halves * kTileBytes; }
 };
 
-template <typename TY, typename TW>
-__global__ void __launch_bounds__(kExpandTileThreads, 2) adapt_expand_tile_kernel(const AdaptParams P) {
-  using S = ExpandTile<TY, TW>;
-  constexpr int PH = S::PH, PW = S::PW;
-  extern __shared__ __align__(1024) char shared[];
-  TileControl& C = *tile_control(shared);
-  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-  const int per = (P.T + kAdaptTile - 1) / kAdaptTile, s = blockIdx.x / per, first = (int(blockIdx.x) - s * per) * kAdaptTile;
-  const int count = min(kAdaptTile, P.T - first), row0 = s * P.T + first;
-  int mat = 0;
-  while (mat < P.nmat - 1 && int(blockIdx.y) >= P.chunk_end[mat]) ++mat;
-  const int N = P.n_out[mat], chunk = int(blockIdx.y) - (mat ? P.chunk_end[mat - 1] : 0), rank = P.rank;
-  const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
-  const TY* y = static_cast<const TY*>(P.y[mat]);
-  TY* out = static_cast<TY*>(P.out[mat]);
-  const long long asked = __ldg(P.ids + s);
-  if (asked < 0 || asked >= P.adapters) {                  // no adapter: only a copy, where out is not y
-    if (y == out) return;
-    for (int r = warp; r < count; r += kExpandTileThreads / 32) {
-      const size_t at = size_t(row0 + r) * N;
-      for (int c = c_begin + lane; c < c_end; c += 32 * 16) {
-        TY v[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (c + 32 * k < c_end) v[k] = y[at + c + 32 * k];
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (c + 32 * k < c_end) out[at + c + 32 * k] = v[k];
-      }
-    }
-    return;
+// A CTA's share of the steps, segment by segment.
+struct ExpandSegment {
+  int tile, mat, step, steps;              // columns [step, step + steps) * 128 of a matrix for a tile
+  int row0, count, id;                     // id -1: none
+};
+struct ExpandWalk {
+  const AdaptParams& P;
+  int per, per_tile, at, end;
+  __device__ __forceinline__ explicit ExpandWalk(const AdaptParams& P_) : P(P_) {
+    per = (P.T + kAdaptTile - 1) / kAdaptTile;
+    per_tile = P.chunk_end[P.nmat - 1];                    // steps of all matrices
+    const long long all = (long long)P.streams * per * per_tile;
+    at = int(all * blockIdx.x / gridDim.x); end = int(all * (blockIdx.x + 1) / gridDim.x);
   }
-  const int ksteps = (rank + 15) / 16, halves = (rank + 63) / 64, NS = P.stages, h_piece = halves * kTileBytes, stage_bytes = PW * h_piece;
-  char *h_tiles = shared + 1024, *stages = h_tiles + PH * h_piece;
+  __device__ __forceinline__ bool next(ExpandSegment& S) {
+    if (at >= end) return false;
+    S.tile = at / per_tile;
+    const int in_tile = at - S.tile * per_tile;
+    S.mat = 0;
+    while (S.mat < P.nmat - 1 && in_tile >= P.chunk_end[S.mat]) ++S.mat;
+    S.step = in_tile - (S.mat ? P.chunk_end[S.mat - 1] : 0);
+    S.steps = min(P.chunk_end[S.mat] - in_tile, end - at);
+    at += S.steps;
+    const int stream = S.tile / per, first = (S.tile - stream * per) * kAdaptTile;
+    S.count = min(kAdaptTile, P.T - first);
+    S.row0 = stream * P.T + first;
+    const long long v = __ldg(P.ids + stream);
+    S.id = v >= 0 && v < P.adapters ? int(v) : -1;
+    return true;
+  }
+  // left out altogether: in place and without an adapter
+  __device__ __forceinline__ bool skipped(const ExpandSegment& S) const { return S.id < 0 && P.y[S.mat] == P.out[S.mat]; }
+};
+
+// y and out of every matrix as [rows][N], boxes of 16 rows x 128 columns.
+struct AdaptMaps {
+  CUtensorMap y[kAdaptMaxMats], out[kAdaptMaxMats];
+};
+constexpr int kExpandBox = 16;
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int col, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(col), "r"(row), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_rows(const CUtensorMap* map, int col, int row, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(col), "r"(row), "r"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+template <typename TY, typename TW>
+__global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kernel(const __grid_constant__ AdaptParams P, const __grid_constant__ AdaptMaps M) {
+  using E = ExpandTile<TY, TW>;
+  constexpr int PH = E::PH, PW = E::PW;
+  extern __shared__ __align__(1024) char shared[];
+  ExpandTileControl& C = *reinterpret_cast<ExpandTileControl*>(shared);
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  const int rank = P.rank, ksteps = (rank + 15) / 16, halves = (rank + 63) / 64, NS = P.stages, NR = P.ring, h_piece = halves * kTileBytes, stage_bytes = PW * h_piece;
+  char *ring = shared + 1024, *h_tiles = ring + NR * E::kHalfBytes, *stages = h_tiles + PH * h_piece;
   const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty), h_full = smem_u32(&C.h_full);
+  const uint32_t y_full = smem_u32(C.y_full), y_empty = smem_u32(C.y_empty);
   volatile int* abort_flag = &C.abort;
+  constexpr int kAddWarps = kExpandTileAdders / 32, kAdd0 = kExpandTileLoaders / 32, kMmaWarp = kAdd0 + kAddWarps;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(full + 8 * i, kExpandTileLoaders); mbar_init(empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kExpandTileAdders / 32); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kAddWarps); }
+    for (int i = 0; i < NR; ++i) { mbar_init(y_full + 8 * i, 1); mbar_init(y_empty + 8 * i, kAddWarps); }
     mbar_init(h_full, kExpandTileAdders);
     C.abort = 0;
     fence_mbar_init();
   }
-  constexpr int kMmaWarp = (kExpandTileLoaders + kExpandTileAdders) / 32;
   if (warp == kMmaWarp) tmem_alloc_cols<256>(smem_u32(&C.tmem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
-  const int steps = (c_end - c_begin + kAdaptTile - 1) / kAdaptTile;
-  if (warp < kExpandTileLoaders / 32) {
+  ExpandWalk walk(P);
+  ExpandSegment G;
+  if (warp < kAdd0) {
     // ---- B: units of eight ranks of a column; neither it nor y comes from the first launch
-    const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(asked) * N * rank;
     const int units = halves * 8, u = tid % units, hop = kExpandTileLoaders / units, j = u * 8;
     const bool wide = rank * int(sizeof(TW)) % 16 == 0, used = u < 2 * ksteps;
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
     int slot = 0;
     uint32_t phase = 0;
-    for (int it = 0; it < steps; ++it) {
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag))) break;
-      char* to = stages + slot * stage_bytes + (u >> 3) * kTileBytes;
-      const int c0 = c_begin + it * kAdaptTile;
-      if (used)
-        for (int c = tid / units; c < kAdaptTile; c += 4 * hop) {
-          uint4 v[4][sizeof(TW) / 2];
+    bool ok = true;
+    while (ok && walk.next(G)) {
+      if (G.id < 0) continue;
+      const int N = P.n_out[G.mat];
+      const TW* b = static_cast<const TW*>(P.b[G.mat]) + size_t(G.id) * N * rank + j;
+      for (int it = 0; it < G.steps; ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag));
+        if (!ok) break;
+        char* to = stages + slot * stage_bytes + (u >> 3) * kTileBytes;
+        const int c0 = (G.step + it) * kAdaptTile;
+        if (used)
+          for (int c = tid / units; c < kAdaptTile; c += 4 * hop) {
+            uint4 v[4][sizeof(TW) / 2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const TW* src = b + size_t(c0 + c + i * hop) * rank + j;
-            const bool in = c + i * hop < kAdaptTile && c0 + c + i * hop < c_end;
-            if constexpr (sizeof(TW) == 4) {
-              v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
-              v[i][1] = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint4*>(src) + 1) : zero;
-            } else if (wide) {
-              v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
-            } else {
-              const uint2 lo = in && j < rank ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
-              const uint2 hi = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint2*>(src) + 1) : make_uint2(0u, 0u);
-              v[i][0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + i * hop < kAdaptTile) {
+            for (int i = 0; i < 4; ++i) {
+              const TW* src = b + size_t(c0 + c + i * hop) * rank;
+              const bool in = c + i * hop < kAdaptTile && c0 + c + i * hop < N;
               if constexpr (sizeof(TW) == 4) {
-                tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2, v[i][0]);
-                tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2 + 1, v[i][1]);
+                v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
+                v[i][1] = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint4*>(src) + 1) : zero;
+              } else if (wide) {
+                v[i][0] = in && j < rank ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
               } else {
-                tile_put<TW, PW>(to, h_piece, c + i * hop, u & 7, v[i][0]);
+                const uint2 lo = in && j < rank ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
+                const uint2 hi = in && j + 4 < rank ? __ldg(reinterpret_cast<const uint2*>(src) + 1) : make_uint2(0u, 0u);
+                v[i][0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
               }
             }
-        }
-      fence_smem_to_mma();
-      mbar_arrive(full + 8 * slot);
-      if (++slot == NS) { slot = 0; phase ^= 1u; }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c + i * hop < kAdaptTile) {
+                if constexpr (sizeof(TW) == 4) {
+                  tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2, v[i][0]);
+                  tile_put<TW, PW>(to, h_piece, c + i * hop, (u & 7) * 2 + 1, v[i][1]);
+                } else {
+                  tile_put<TW, PW>(to, h_piece, c + i * hop, u & 7, v[i][0]);
+                }
+              }
+          }
+        fence_smem_to_mma();
+        mbar_arrive(full + 8 * slot);
+        if (++slot == NS) { slot = 0; phase ^= 1u; }
+      }
     }
   } else if (warp < kMmaWarp) {
-    const int q = warp & 3, part = (warp - kExpandTileLoaders / 32) >> 2;      // TMEM lanes 32 q .., every second 16 rows
+    const int w = warp - kAdd0, q = warp & 3, part = w >> 2;                  // TMEM lanes 32 q ..; 16-row groups part, part + 2 of a half step
     griddep_wait();
-    {
-      const float scale = P.scale[mat] ? __ldg(P.scale[mat] + asked) : 1.f;
-      const int r4 = ksteps * 4, n16 = (count + 15) / 16 * 16;                 // groups of four ranks; rows
-      for (int i = tid - kExpandTileLoaders; i < n16 * r4; i += kExpandTileAdders) {
-        const int r = i / r4, j4 = i - r * r4, jj = j4 * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < count && jj < rank) v = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(row0 + r) * rank + jj));
-        uint32_t lo[PH], hi[PH];
-        split_pair<PH>(v.x * scale, v.y * scale, lo);
-        split_pair<PH>(v.z * scale, v.w * scale, hi);
-        char* at = h_tiles + (j4 >> 4) * kTileBytes + tile_unit(r, (j4 & 15) >> 1) + (j4 & 1) * 8;
-#pragma unroll
-        for (int p = 0; p < PH; ++p) *reinterpret_cast<uint2*>(at + p * h_piece) = make_uint2(lo[p], hi[p]);
-      }
-      fence_smem_to_mma();
-      mbar_arrive(h_full);
-    }
-    const int groups = (count + 15) / 16;
     bool ok = true;
-    for (int it = 0; it < steps; ++it) {
-      const int n = c_begin + it * kAdaptTile + q * 32 + lane, buf = it & 1;
-      const bool in = n < c_end;
-      const TY* yp = y + size_t(row0) * N + (in ? n : c_begin);
-      TY* op = out + size_t(row0) * N + n;
-      TY v[16];
-      auto fetch = [&](int grp) {
-        const TY* p = yp + size_t(grp * 16) * N;
+    int slot = 0, uses = 0, last_slot = -1;                // uses: accumulators taken so far
+    uint32_t phase = 0;
+    while (walk.next(G)) {
+      if (walk.skipped(G)) continue;
+      const int N = P.n_out[G.mat], n16 = (G.count + 15) / 16 * 16;
+      if (G.id >= 0) {                                     // every MMA of the segment before is over: its sums have been read
+        const float scale = P.scale[G.mat] ? __ldg(P.scale[G.mat] + G.id) : 1.f;
+        const int r4 = ksteps * 4;                         // groups of four ranks
+        for (int i = tid - kExpandTileLoaders; i < n16 * r4; i += kExpandTileAdders) {
+          const int r = i / r4, j4 = i - r * r4, jj = j4 * 4;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < G.count && jj < rank) v = __ldcg(reinterpret_cast<const float4*>(P.h[G.mat] + size_t(G.row0 + r) * rank + jj));
+          uint32_t lo[PH], hi[PH];
+          split_pair<PH>(v.x * scale, v.y * scale, lo);
+          split_pair<PH>(v.z * scale, v.w * scale, hi);
+          char* at = h_tiles + (j4 >> 4) * kTileBytes + tile_unit(r, (j4 & 15) >> 1) + (j4 & 1) * 8;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (grp * 16 + i < count) v[i] = *p;
-          p += N;
+          for (int p = 0; p < PH; ++p) *reinterpret_cast<uint2*>(at + p * h_piece) = make_uint2(lo[p], hi[p]);
         }
-      };
-      if (part < groups) fetch(part);
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * buf, uint32_t(it >> 1) & 1u, abort_flag));
-      tc_fence_after();
-      for (int grp = part; grp < groups; grp += 2) {
-        float d[16];
-        if (ok) {
-          tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * kAdaptTile + grp * 16), d);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) d[i] = NAN;
+        fence_smem_to_mma();
+        mbar_arrive(h_full);
+      }
+      TY* out = static_cast<TY*>(P.out[G.mat]);
+      const int n_half = (G.count + kExpandHalf - 1) / kExpandHalf;
+      for (int it = 0; it < G.steps; ++it) {
+        const int c0 = (G.step + it) * kAdaptTile, bytes = min(kAdaptTile, N - c0) * int(sizeof(TY)), buf = uses & 1;
+        if (G.id >= 0) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * buf, uint32_t(uses >> 1) & 1u, abort_flag));
+          tc_fence_after();
         }
+        for (int hf = 0; hf < n_half; ++hf) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(y_full + 8 * slot, phase, abort_flag));
+          char* half = ring + slot * E::kHalfBytes;
+          const int rows = min(kExpandHalf, G.count - hf * kExpandHalf);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) d[i] += adapt_float(v[i]);
-        if (grp + 2 < groups) fetch(grp + 2);
-        TY* p = op + size_t(grp * 16) * N;
+          for (int e = 0; e < 2; ++e) {
+            const int r0 = (part + 2 * e) * 16;
+            if (r0 >= rows) break;
+            if (G.id >= 0) {
+              float d[16];
+              if (ok) {
+                tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * kAdaptTile + hf * kExpandHalf + r0), d);
+                tmem_ld_wait();
+              } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (in && grp * 16 + i < count) adapt_store(p, d[i]);
-          p += N;
+                for (int i = 0; i < 16; ++i) d[i] = NAN;
+              }
+              TY* mine = reinterpret_cast<TY*>(half + r0 * E::kRow) + q * 32 + lane;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) adapt_store(mine + i * kAdaptTile, adapt_float(mine[i * kAdaptTile]) + d[i]);
+              fence_smem_to_mma();
+            }
+            named_bar_sync(1 + part, 128);                 // the four warps of these 16 rows
+            const int row = G.row0 + hf * kExpandHalf;
+            if (r0 + kExpandBox <= rows) {
+              if (q == 0 && lane == 0) tma_store_rows(&M.out[G.mat], c0, row + r0, smem_u32(half + r0 * E::kRow));
+            } else {                                       // the last rows of a stream, one by one
+              const int r = r0 + q * 4 + lane;
+              if (lane < 4 && r < rows) bulk_s2g(out + size_t(row + r) * N + c0, smem_u32(half + r * E::kRow), uint32_t(bytes));
+            }
+          }
+          if (lane < 4) bulk_commit();
+          if (hf == n_half - 1 && G.id >= 0) {             // this warp has read the accumulator
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+            ++uses;
+          }
+          if (last_slot >= 0) {                            // the half step before has left shared memory
+            if (lane < 4) bulk_wait_read<1>();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(y_empty + 8 * last_slot);
+          }
+          last_slot = slot;
+          if (++slot == NR) { slot = 0; phase ^= 1u; }
         }
       }
-      tc_fence_before();
-      if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+    }
+    if (lane < 4) bulk_wait_all();                         // out is written when the kernel ends
+  } else if (warp == kMmaWarp) {
+    const uint32_t h_at = smem_u32(h_tiles), base = smem_u32(stages);
+    int slot = 0, uses = 0, segs = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    while (ok && walk.next(G)) {
+      if (G.id < 0) continue;
+      const uint32_t idesc = umma_idesc_f16(kAdaptTile, (G.count + 15) / 16 * 16, 1);
+      ok = warp_wait(h_full, uint32_t(segs) & 1u, abort_flag, nullptr, 0);
+      ++segs;
+      for (int it = 0; it < G.steps && ok; ++it, ++uses) {
+        const int buf = uses & 1;
+        ok = warp_wait(acc_empty + 8 * buf, (uint32_t(uses >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0) && warp_wait(full + 8 * slot, phase, abort_flag, nullptr, 0);
+        if (!ok) break;
+        if (elect_one()) {
+          tc_fence_after();
+          const uint32_t d = tmem + uint32_t(buf * kAdaptTile);
+          uint32_t more = 0u;
+          for (int k = 0; k < ksteps; ++k) {
+            const uint32_t off = uint32_t((k >> 2) * kTileBytes + (k & 3) * 32);
+#pragma unroll
+            for (int p = PH - 1; p >= 0; --p)
+#pragma unroll
+              for (int w = PW - 1; w >= 0; --w) {
+                if (p + w >= PH) continue;
+                umma_f16<false>(d, umma_desc(base + slot * stage_bytes + w * h_piece + off), umma_desc(h_at + p * h_piece + off), idesc, more);
+                more = 1u;
+              }
+          }
+          umma_commit<false>(empty + 8 * slot);
+          umma_commit<false>(acc_full + 8 * buf);
+        }
+        __syncwarp();
+        if (++slot == NS) { slot = 0; phase ^= 1u; }
+      }
     }
   } else {
-    const uint32_t idesc = umma_idesc_f16(kAdaptTile, (count + 15) / 16 * 16, 1);
-    const uint32_t h_at = smem_u32(h_tiles), base = smem_u32(stages);
-    bool ok = warp_wait(h_full, 0u, abort_flag, nullptr, 0);
     int slot = 0;
     uint32_t phase = 0;
-    for (int it = 0; it < steps && ok; ++it) {
-      const int buf = it & 1;
-      if (!warp_wait(acc_empty + 8 * buf, (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0)) break;
-      if (!warp_wait(full + 8 * slot, phase, abort_flag, nullptr, 0)) break;
-      if (elect_one()) {
-        tc_fence_after();
-        const uint32_t d = tmem + uint32_t(buf * kAdaptTile);
-        uint32_t more = 0u;
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = uint32_t((k >> 2) * kTileBytes + (k & 3) * 32);
-#pragma unroll
-          for (int p = PH - 1; p >= 0; --p)
-#pragma unroll
-            for (int w = PW - 1; w >= 0; --w) {
-              if (p + w >= PH) continue;
-              umma_f16<false>(d, umma_desc(base + slot * stage_bytes + w * h_piece + off), umma_desc(h_at + p * h_piece + off), idesc, more);
-              more = 1u;
-            }
+    bool ok = true;
+    while (ok && walk.next(G)) {
+      if (walk.skipped(G)) continue;
+      const int N = P.n_out[G.mat], n_half = (G.count + kExpandHalf - 1) / kExpandHalf;
+      const TY* y = static_cast<const TY*>(P.y[G.mat]) + size_t(G.row0) * N;
+      for (int it = 0; it < G.steps && ok; ++it) {
+        const int c0 = (G.step + it) * kAdaptTile, bytes = min(kAdaptTile, N - c0) * int(sizeof(TY));
+        for (int hf = 0; hf < n_half && ok; ++hf) {
+          ok = warp_wait(y_empty + 8 * slot, phase ^ 1u, abort_flag, nullptr, 0);
+          if (!ok) break;
+          const int rows = min(kExpandHalf, G.count - hf * kExpandHalf);
+          const int boxed = rows / kExpandBox * kExpandBox;          // the last rows of a stream come one by one
+          if (lane == 0) mbar_arrive_expect_tx(y_full + 8 * slot, uint32_t(boxed * E::kRow + (rows - boxed) * bytes));
+          __syncwarp();
+          const uint32_t to = smem_u32(ring + slot * E::kHalfBytes);
+          if (lane * kExpandBox < boxed)
+            tma_load_rows(to + lane * kExpandBox * E::kRow, &M.y[G.mat], c0, G.row0 + hf * kExpandHalf + lane * kExpandBox, y_full + 8 * slot);
+          else if (lane >= 16 && boxed + lane - 16 < rows)
+            bulk_g2s(to + (boxed + lane - 16) * E::kRow, y + size_t(hf * kExpandHalf + boxed + lane - 16) * N + c0, uint32_t(bytes), y_full + 8 * slot);
+          if (++slot == NR) { slot = 0; phase ^= 1u; }
         }
-        umma_commit<false>(empty + 8 * slot);
-        umma_commit<false>(acc_full + 8 * buf);
       }
-      __syncwarp();
-      if (++slot == NS) { slot = 0; phase ^= 1u; }
+    }
+    // after an abort copies may still be on their way into shared memory
+    if (*abort_flag) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < kWaitLimitNs / 100) {
+      }
     }
   }
   tc_fence_before();
@@ -451,23 +580,22 @@ __global__ void __launch_bounds__(kExpandTileThreads, 2) adapt_expand_tile_kerne
 
 struct AdaptShape {
   bool tiles1, tiles2;                     // the forms for 128 rows of a stream, else for gathered tiles of 16
-  int n1, n2;                              // tiles that a launch has at most
+  int n1, n2;                              // tiles that a launch has at most; CTAs of the second launch's form for tiles
   int splits, mt;                          // first launch: CTAs that share K; gathered: ranks of a CTA in 16
-  int kc, chunk_cols, chunks;              // second launch: gathered: ranks per stage; columns of a CTA
+  int kc, chunk_cols, chunks;              // second launch: ranks per stage (gathered), columns of a CTA or step, those of all matrices
 };
 
-// Streams of 64 rows or more are cut into tiles of 128 (ranks up to 128 in the second launch, whose h stays in shared memory);
-// shorter ones are gathered.  Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or
-// more k each.  Columns of a CTA of the second launch: what it takes at a time, times what leaves three CTAs per SM (gathered
-// tiles: each starts with a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40) or four.
-inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int sms) {
+// Streams of 64 rows or more are cut into tiles of 128; shorter ones are gathered.  The second launch has its form for tiles for
+// ranks up to 128 and rows that start on 16 bytes (`aligned`; y passes as bulk copies), one CTA per SM.
+// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.
+// Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves three CTAs per SM (each starts with
+// a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40).
+inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool aligned, int sms) {
   AdaptShape s;
-  auto tiles = [&](int rows) { return T < rows ? streams : streams * ((T + rows - 1) / rows); };
-  auto cut = [&](int rows) { return streams * ((T + rows - 1) / rows); };
+  auto cut = [&](int rows) { return T < rows ? streams : streams * ((T + rows - 1) / rows); };
   s.tiles1 = T >= 64;
-  s.tiles2 = T >= 64 && rank <= kTileRankMax;
-  s.n1 = s.tiles1 ? cut(kAdaptTile) : tiles(kAdaptRows);
-  s.n2 = s.tiles2 ? cut(kAdaptTile) : tiles(kAdaptRows);
+  s.tiles2 = T >= 64 && rank <= kTileRankMax && aligned;
+  s.n1 = s.tiles1 ? streams * ((T + kAdaptTile - 1) / kAdaptTile) : cut(kAdaptRows);
   auto busy = [&](int n, bool tiled) {                   // tiles that lead rows
     const long long most = adapters + (long long)streams * T / kAdaptRows + 1;
     return !tiled && T < kAdaptRows && most < n ? most : (long long)n;
@@ -478,12 +606,20 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   const long long ctas = busy(s.n1, s.tiles1) * nmat * ((rank + per_cta - 1) / per_cta);
   s.splits = 1;
   while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
-  const int unit = s.tiles2 ? kAdaptTile : kExpandWarps * (w_pieces < 3 ? 64 : 32);
+  s.chunks = 0;
+  if (s.tiles2) {                                        // steps of all matrices for a tile, and CTAs
+    s.chunk_cols = kAdaptTile;
+    for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + kAdaptTile - 1) / kAdaptTile;
+    const long long steps = (long long)streams * ((T + kAdaptTile - 1) / kAdaptTile) * s.chunks;
+    s.n2 = int(steps < sms ? steps : sms);
+    return s;
+  }
+  s.n2 = cut(kAdaptRows);
+  const int unit = kExpandWarps * (w_pieces < 3 ? 64 : 32);
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  long long per = units * busy(s.n2, s.tiles2) / ((s.tiles2 ? 4LL : 3LL) * sms);
+  const long long per = units * busy(s.n2, false) / (3LL * sms);
   s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
-  s.chunks = 0;
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
   return s;
 }

@@ -785,16 +785,31 @@ static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape
                         size_t(warps) + expand_h_bytes<TY>(P.rank, KC), stream, P);
 }
 
+// [rows][n] elements of `size` bytes, boxes of kExpandBox rows x kAdaptTile columns; n * size a multiple of 16.
+static bool encode_rows_map(CUtensorMap* map, const void* p, int size, int n, int rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {cuuint64_t(n), cuuint64_t(rows)}, strides[1] = {cuuint64_t(n) * size};
+  const cuuint32_t box[2] = {kAdaptTile, kExpandBox}, step[2] = {1, 1};
+  return enc(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p), dims, strides, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename TY, typename TW>
 static cudaError_t launch_adapt_expand(AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   if (sh.tiles2) {
-    using S = ExpandTile<TY, TW>;
+    using E = ExpandTile<TY, TW>;
     static bool configured[64];
     const int halves = (P.rank + 63) / 64;
-    const cudaError_t e = allow_smem(adapt_expand_tile_kernel<TY, TW>, S::smem(1) > S::smem(2) ? S::smem(1) : S::smem(2), configured);
+    const cudaError_t e = allow_smem(adapt_expand_tile_kernel<TY, TW>, E::smem(1) > E::smem(2) ? E::smem(1) : E::smem(2), configured);
     if (e != cudaSuccess) return e;
-    P.stages = S::stages(halves);
-    return launch_chained(adapt_expand_tile_kernel<TY, TW>, dim3(sh.n2, sh.chunks), dim3(kExpandTileThreads), S::smem(halves), stream, P);
+    P.stages = E::stages(halves); P.ring = E::ring(halves);
+    AdaptMaps M;
+    memset(&M, 0, sizeof(M));
+    for (int i = 0; i < P.nmat; ++i)
+      if (!encode_rows_map(&M.y[i], P.y[i], int(sizeof(TY)), P.n_out[i], P.R) || !encode_rows_map(&M.out[i], P.out[i], int(sizeof(TY)), P.n_out[i], P.R))
+        return cudaErrorInvalidValue;
+    return launch_chained(adapt_expand_tile_kernel<TY, TW>, dim3(sh.n2), dim3(kExpandTileThreads), E::smem(halves), stream, P, M);
   }
   if (sh.kc == 16) return vec ? launch_adapt_expand_as<TY, TW, 16, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 16, false>(P, sh, stream);
   return vec ? launch_adapt_expand_as<TY, TW, 32, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 32, false>(P, sh, stream);
@@ -2002,6 +2017,13 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
 // ---- many requests: adapters, verification of drafted tokens, the state after the accepted ones
 static int adapt_weight_pieces(int dtype) { return dtype == B200RWKV_F32 ? 3 : dtype == B200RWKV_F16 ? 2 : 1; }
 
+static bool adapt_tile_fits(int dtype, int row_dtype, int rank) {
+  const int halves = (rank + 63) / 64;
+  if (dtype == B200RWKV_F32) return ExpandTile<float, float>::stages(halves) > 0;
+  if (dtype == B200RWKV_BF16) return (row_dtype == B200RWKV_F32 ? ExpandTile<float, __nv_bfloat16>::stages(halves) : ExpandTile<__nv_bfloat16, __nv_bfloat16>::stages(halves)) > 0;
+  return (row_dtype == B200RWKV_F32 ? ExpandTile<float, __half>::stages(halves) : ExpandTile<__half, __half>::stages(halves)) > 0;
+}
+
 static const char* adapt_problem(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int streams, int tokens_per_stream) {
   if (nmat < 1 || nmat > kAdaptMaxMats || !banks) return "1..3 banks";
   if (n_adapters < 1 || rank < 4 || rank > kAdaptMaxRank || rank % 4) return "at least one adapter, rank a multiple of 4 up to 256";
@@ -2034,7 +2056,7 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
   const size_t eb = size_t(dense_elem_bytes(row_dtype));
   AdaptParams P;
   memset(&P, 0, sizeof(P));
-  bool vec = true;               // rows of y and out start on boundaries of four elements
+  bool vec = true, aligned = true;         // rows of y and out start on boundaries of four elements, of 16 bytes
   for (int i = 0; i < nmat; ++i) {
     const b200rwkv_adapters& m = banks[i];
     if (!m.a || !m.b || !x[i] || !y[i] || !out[i] || !aligned16(m.a) || !aligned16(m.b) || !aligned16(x[i]))
@@ -2042,8 +2064,11 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
     P.a[i] = m.a; P.b[i] = m.b; P.scale[i] = m.scale; P.x[i] = x[i]; P.y[i] = y[i]; P.out[i] = out[i]; P.n_out[i] = m.n_out;
     P.h[i] = reinterpret_cast<float*>(static_cast<char*>(workspace) + size_t(i) * (need / nmat));
     vec = vec && m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
+    aligned = aligned && m.n_out * eb % 16 == 0 && aligned16(y[i]) && aligned16(out[i]);
   }
-  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), device_sms());
+  // the form for tiles keeps h and 64 or 128 ranks of B in shared memory
+  aligned = aligned && adapt_tile_fits(dtype, row_dtype, rank);
+  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), aligned, device_sms());
   for (int i = 0; i < nmat; ++i) P.chunk_end[i] = (i ? P.chunk_end[i - 1] : 0) + (P.n_out[i] + sh.chunk_cols - 1) / sh.chunk_cols;
   P.ids = reinterpret_cast<const long long*>(ids);
   P.nmat = nmat; P.adapters = n_adapters; P.rank = rank; P.K = k_in; P.R = streams * tokens_per_stream; P.T = tokens_per_stream;

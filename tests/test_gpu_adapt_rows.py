@@ -82,6 +82,11 @@ SHAPES = [
     (2, 333, 1024, [260, 64], 64, 5),
     (2, 70, 8, [5], 256, 2),                 # the shortest K, the largest rank
     (9, 2, 520, [1], 200, 4),
+    (3, 129, 64, [1024, 392, 8], 20, 2),     # tiles of 128 rows, several matrices and columns that end inside a step
+    (5, 200, 456, [640, 2048], 64, 4),
+    (2, 701, 2048, [256], 128, 2),
+    (40, 64, 128, [776], 48, 3),             # more tiles than SMs have steps for at once
+    (1, 2000, 96, [1160, 16], 12, 1),
 ]
 
 
