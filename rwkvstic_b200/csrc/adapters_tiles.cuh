@@ -249,15 +249,15 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
 // a TMEM lane each).  One persistent CTA per SM takes an equal share of all steps of all tiles and matrices, in order; a
 // segment is what it has of one tile and matrix, whose pieces of h it lays out once.
 //   warps 0..3   bring B and cut it into pieces, a step at a time
-//   warps 4..11  add: a warp has 32 columns (lanes) and every second 16 rows of a half step
-//   warp 12      issues the MMAs; two accumulators
-//   warp 13      requests y, 64 rows x 128 columns a half step, in TMA boxes of 16 rows, up to four half steps ahead
+//   warps 4..19  add: a warp has 32 columns (lanes) and 16 rows of a half step
+//   warp 20      issues the MMAs; two accumulators
+//   warp 21      requests y, 64 rows x 128 columns a half step, in TMA boxes of 16 rows, up to four half steps ahead
 // Sums are added in place in shared memory, with the lanes along a row, and leave in the same boxes (as bulk copies of single
 // rows, 512 bytes each, both ways took 215 us for 8192 rows of a 3B ffn).  What bounds it is memory: 128
 // bytes per 16 values pass the SM.  The same tiles with y through registers were bound by the L1 lines that loads in flight
 // occupy beside 226 KB of shared memory (3B ffn, 8192 rows: 190 us for 839 MB), mma.sync by its own rate under the power cap.
 // A tile without an adapter goes through unchanged, or is left out where out is y.
-constexpr int kExpandTileLoaders = 128, kExpandTileAdders = 256, kExpandTileThreads = kExpandTileLoaders + kExpandTileAdders + 64;
+constexpr int kExpandTileLoaders = 128, kExpandTileAdders = 512, kExpandTileThreads = kExpandTileLoaders + kExpandTileAdders + 64;
 constexpr int kExpandTileRing = 4, kExpandHalf = 64;       // half steps of y in shared memory, at most; rows of one
 
 struct ExpandTileControl {
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
       }
     }
   } else if (warp < kMmaWarp) {
-    const int w = warp - kAdd0, q = warp & 3, part = w >> 2;                  // TMEM lanes 32 q ..; 16-row groups part, part + 2 of a half step
+    const int w = warp - kAdd0, q = warp & 3, part = w >> 2;                  // TMEM lanes 32 q ..; rows 16 part .. of a half step
     griddep_wait();
     bool ok = true;
     int slot = 0, uses = 0, last_slot = -1;                // uses: accumulators taken so far
@@ -457,10 +457,8 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
           ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(y_full + 8 * slot, phase, abort_flag));
           char* half = ring + slot * E::kHalfBytes;
           const int rows = min(kExpandHalf, G.count - hf * kExpandHalf);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r0 = (part + 2 * e) * 16;
-            if (r0 >= rows) break;
+          const int r0 = part * 16;
+          if (r0 < rows) {
             if (G.id >= 0) {
               float d[16];
               if (ok) {
@@ -472,7 +470,9 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
               }
               TY* mine = reinterpret_cast<TY*>(half + r0 * E::kRow) + q * 32 + lane;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) adapt_store(mine + i * kAdaptTile, adapt_float(mine[i * kAdaptTile]) + d[i]);
+              for (int i = 0; i < 16; ++i) d[i] += adapt_float(mine[i * kAdaptTile]);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) adapt_store(mine + i * kAdaptTile, d[i]);
               fence_smem_to_mma();
             }
             named_bar_sync(1 + part, 128);                 // the four warps of these 16 rows
