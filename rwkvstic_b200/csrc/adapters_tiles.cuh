@@ -40,7 +40,7 @@ __device__ __forceinline__ int tile_unit(int row, int u) { return row * 128 + ((
 
 // Barriers and flags at the front of dynamic shared memory (1024 bytes, so that the tiles behind are aligned).
 struct TileControl {
-  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], h_full;
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   int abort;
   uint32_t tmem;
 };
@@ -48,9 +48,11 @@ __device__ __forceinline__ TileControl* tile_control(char* shared) { return rein
 
 // ---------------------------------------------------------------------------------------------- the first launch
 // h[row][j] = sum_k x[row][k] A[id][j][k] for 128 rows (the MMAs' M, a TMEM lane each) and up to 64 ranks (their N).  Eight warps
-// bring 64 k of x and A at a time, requested one stage ahead, cut them into pieces and store them; one warp issues the MMAs.
-// Two stages make a sum: its 24 additions are cut off by the tensor cores (rank 64, fp32 x, bf16 A: 12 MMAs each), so the eight
-// warps add it up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
+// bring 64 k of x and A at a time; one warp issues the MMAs.  x comes by asynchronous copies some stages ahead: into the MMAs'
+// own tiles where both operands are of one 16-bit type, else into slots of the thread that asked, which cuts it into pieces.
+// (Loads into registers were bound by the few L1 lines that are left beside this much shared memory: 3B ffn, 8192 rows 62 us.)
+// Two stages make a sum: its additions (rank 64, fp32 x, bf16 A: 24) are cut off by the tensor cores, so the eight warps add it
+// up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
 constexpr int kShrinkTileWorkers = 256, kShrinkTileThreads = kShrinkTileWorkers + 32, kShrinkTileRanks = 64;
 
 template <typename TX, typename TW>
@@ -58,9 +60,10 @@ struct ShrinkTile {
   static constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   static constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
   static constexpr int kBytesX = PX * kTileBytes, kStage = kBytesX + PW * kTileBytes / 2;
-  static constexpr int kStages = kStage <= 28 * 1024 ? 4 : kStage <= 56 * 1024 ? 2 : kStage <= 64 * 1024 ? 3 : 2;
+  static constexpr int kStages = kSame ? 8 : 2, kRaw = kSame ? 0 : 64 * kAdaptTile * int(sizeof(TX)), kFit = kSame ? 0 : (226 * 1024 - 1024 - 2 * kStage) / kRaw;
+  static constexpr int kRing = kFit > 4 ? 4 : kFit;        // stages of x as it comes
   static constexpr int kPitch = kShrinkTileRanks + 1, kTable = kAdaptTile * kPitch * 4;
-  static constexpr int kSmem = 1024 + (kStages * kStage > kTable ? kStages * kStage : kTable);
+  static constexpr int kSmem = 1024 + (kStages * kStage + kRing * kRaw > kTable ? kStages * kStage + kRing * kRaw : kTable);
   // loads of a thread: 16 bytes each
   static constexpr int kUnitX = 16 / int(sizeof(TX)), kRowX = 64 / kUnitX, kHopX = kShrinkTileWorkers / kRowX, kLoadX = kAdaptTile / kHopX;
   static constexpr int kUnitW = 16 / int(sizeof(TW)), kRowW = 64 / kUnitW, kHopW = kShrinkTileWorkers / kRowW, kLoadW = kShrinkTileRanks / kHopW;
@@ -91,7 +94,7 @@ __device__ __forceinline__ void tile_put(char* tile, int hop, int row, int load,
 }
 
 template <typename TX, typename TW>
-__global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem <= 113 * 1024 ? 2 : 1) adapt_shrink_tile_kernel(const AdaptParams P) {
+__global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kernel(const AdaptParams P) {
   using S = ShrinkTile<TX, TW>;
   extern __shared__ __align__(1024) char shared[];
   TileControl& C = *tile_control(shared);
@@ -126,29 +129,40 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
     const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
     const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
     const int ux = tid % S::kRowX, rx = tid / S::kRowX, uw = tid % S::kRowW, rw = tid / S::kRowW;
-    uint4 vx[S::kLoadX], vw[S::kLoadW];
+    uint4 vw[S::kLoadW];
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    auto load = [&](int c) {
-      const int kx = c * 64 + ux * S::kUnitX, kw = c * 64 + uw * S::kUnitW;
-#pragma unroll
-      for (int i = 0; i < S::kLoadX; ++i) {
-        const int r = rx + i * S::kHopX;
-        vx[i] = r < count && kx < K ? __ldg(reinterpret_cast<const uint4*>(x + size_t(r) * K + kx)) : zero;
-      }
+    auto load_w = [&](int c) {
+      const int k = c * 64 + uw * S::kUnitW;
 #pragma unroll
       for (int i = 0; i < S::kLoadW; ++i) {
         const int r = rw + i * S::kHopW;
-        vw[i] = r < ranks && kw < K ? __ldg(reinterpret_cast<const uint4*>(a + size_t(r) * K + kw)) : zero;
+        vw[i] = r < ranks && k < K ? __ldg(reinterpret_cast<const uint4*>(a + size_t(r) * K + k)) : zero;
       }
     };
-    // ask L2 for the lines of x some stages further on: registers hold one stage, which is too little to keep HBM busy
-    constexpr int kLines = 64 * int(sizeof(TX)) / 128, kAhead = 4;
-    auto ask = [&](int c) {
-      const int r = tid / kLines, k = c * 64 + tid % kLines * (128 / int(sizeof(TX)));
-      if (c < c1 && r < count && k < K) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + size_t(r) * K + k));
-    };
+    // 16-byte units of x (and of A where nothing is cut) to `at(i)`; past the end of rows, ranks or k zeros
+    char* raw = stages + S::kStages * S::kStage + tid * 16;
+    auto request = [&](int c, int slot) {
+      if (c < c1) {
+        const int k = c * 64 + ux * S::kUnitX;
+        char* to = stages + slot * S::kStage;
 #pragma unroll
-    for (int i = 1; i < kAhead; ++i) ask(c0 + i);
+        for (int i = 0; i < S::kLoadX; ++i) {
+          const int r = rx + i * S::kHopX;
+          const bool in = r < count && k < K;
+          cp_async16(smem_u32(S::kSame ? to + tile_unit(r, ux) : raw + slot * S::kRaw + i * kShrinkTileWorkers * 16), in ? x + size_t(r) * K + k : x, in);
+        }
+        if constexpr (S::kSame) {
+          const int kw = c * 64 + uw * S::kUnitW;
+#pragma unroll
+          for (int i = 0; i < S::kLoadW; ++i) {
+            const int r = rw + i * S::kHopW;
+            const bool in = r < ranks && kw < K;
+            cp_async16(smem_u32(to + S::kBytesX + tile_unit(r, uw)), in ? a + size_t(r) * K + kw : a, in);
+          }
+        }
+      }
+      cp_async_commit();                                   // a group per stage, also an empty one
+    };
     bool ok = true;
     auto flush = [&](int g) {                              // the sum of stages 2 g and 2 g + 1
       ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * (g & 1), uint32_t(g >> 1) & 1u, abort_flag));
@@ -169,19 +183,37 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
       tc_fence_before();
       if (lane == 0) mbar_arrive(acc_empty + 8 * (g & 1));
     };
-    load(c0);
-    int slot = 0;
+    int slot = 0;                                          // of the MMAs' stages
     uint32_t phase = 0;
+    // stages ahead: the tiles' own are free again two MMAs later, the slots of x at once
+    constexpr int kAhead = S::kSame ? S::kStages - 2 : S::kRing;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) request(c0 + i, i);
+    int ask = S::kSame ? kAhead : 0;                       // slot of the next request
+    if constexpr (!S::kSame) load_w(c0);
     for (int c = c0; c < c1 && ok; ++c) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag));
-      if (!ok) break;
-      char* to = stages + slot * S::kStage;
+      const int n0 = c - c0;
+      if constexpr (S::kSame) {
+        if (c + kAhead < c1 && n0 + kAhead >= S::kStages)  // chunk n0 + kAhead takes the stage of n0 + kAhead - kStages = n0 - 2
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * ask, uint32_t((n0 + kAhead) / S::kStages - 1) & 1u, abort_flag));
+        if (!ok) break;
+        request(c + kAhead, ask);
+        if (++ask == S::kStages) ask = 0;
+        cp_async_wait<kAhead>();
+      } else {
+        cp_async_wait<kAhead - 1>();
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * slot, phase ^ 1u, abort_flag));
+        if (!ok) break;
+        char* to = stages + slot * S::kStage;
 #pragma unroll
-      for (int i = 0; i < S::kLoadX; ++i) tile_put<TX, S::PX>(to, kTileBytes, rx + i * S::kHopX, ux, vx[i]);
+        for (int i = 0; i < S::kLoadX; ++i)
+          tile_put<TX, S::PX>(to, kTileBytes, rx + i * S::kHopX, ux, *reinterpret_cast<const uint4*>(raw + ask * S::kRaw + i * kShrinkTileWorkers * 16));
 #pragma unroll
-      for (int i = 0; i < S::kLoadW; ++i) tile_put<TW, S::PW>(to + S::kBytesX, kTileBytes / 2, rw + i * S::kHopW, uw, vw[i]);
-      if (c + 1 < c1) load(c + 1);
-      ask(c + kAhead);
+        for (int i = 0; i < S::kLoadW; ++i) tile_put<TW, S::PW>(to + S::kBytesX, kTileBytes / 2, rw + i * S::kHopW, uw, vw[i]);
+        if (c + 1 < c1) load_w(c + 1);
+        request(c + kAhead, ask);                          // over what this thread has just read
+        if (++ask == S::kRing) ask = 0;
+      }
       fence_smem_to_mma();
       mbar_arrive(full + 8 * slot);
       if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
@@ -189,6 +221,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
       if (n >= 2 && (n & 1) == 0) flush(n / 2 - 1);
     }
     if (ok) flush((c1 - c0 + 1) / 2 - 1);                  // the others have been
+    cp_async_wait<0>();
     if (!ok)
 #pragma unroll
       for (int i = 0; i < 32; ++i) sum[i] = NAN;
@@ -224,7 +257,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, ShrinkTile<TX, TW>::kSmem 
       if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
     }
   }
-  // every MMA is over (the workers saw the last sum): the stages become the table of sums
+  // every MMA is over (the workers saw the last sum) and no copy on its way: the stages become the table of sums
   float* table = reinterpret_cast<float*>(stages);
   if (warp < kShrinkTileWorkers / 32) {
     float* mine = table + (q * 32 + lane) * S::kPitch + half * 32;
@@ -587,7 +620,7 @@ struct AdaptShape {
 
 // Streams of 64 rows or more are cut into tiles of 128; shorter ones are gathered.  The second launch has its form for tiles for
 // ranks up to 128 and rows that start on 16 bytes (`aligned`; y passes as bulk copies), one CTA per SM.
-// Splits of K: a power of two that leaves the launch one wave of two CTAs per SM, with 256 or more k each.
+// Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
 // Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves three CTAs per SM (each starts with
 // a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40).
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool aligned, int sms) {
@@ -605,7 +638,7 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   const int per_cta = s.tiles1 ? kShrinkTileRanks : 16 * s.mt;
   const long long ctas = busy(s.n1, s.tiles1) * nmat * ((rank + per_cta - 1) / per_cta);
   s.splits = 1;
-  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= 2LL * sms && K >= 512 * s.splits) s.splits *= 2;
+  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= (s.tiles1 ? 1LL : 2LL) * sms && K >= 512 * s.splits) s.splits *= 2;
   s.chunks = 0;
   if (s.tiles2) {                                        // steps of all matrices for a tile, and CTAs
     s.chunk_cols = kAdaptTile;
