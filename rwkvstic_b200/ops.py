@@ -29,8 +29,11 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_HERE = nullcontext()
+
+
 def _on(index: int):
-    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def _cmatrix(m: QuantMatrix) -> _lib.Matrix:
@@ -260,6 +263,7 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     if ids.dtype != torch.int64 or ids.get_device() != index or not ids.is_contiguous() or (rows % streams if streams else rows):
         raise ValueError("ids must be contiguous int64 on the banks' device, one per stream, and the rows a multiple of them")
     packed, px, py, po, n_out = [], [], [], [], []
+    x_want = (rows, k_in)
     for (a, b, s), x, y, o in zip(banks, xs, ys, outs):
         b_shape = b.shape
         if a.shape != bank_shape or len(b_shape) != 3 or b_shape[0] != count or b_shape[2] != rank:
@@ -269,25 +273,34 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
             raise ValueError("adapt_rows banks must be contiguous, of one type, on one device")
         if s is not None and (s.dtype != torch.float32 or s.get_device() != index or s.shape != (count,) or not s.is_contiguous()):
             raise ValueError("an adapter bank's scale must be contiguous fp32 [n] on its device")
-        y_shape = (rows, b_shape[1])
-        if (x.shape != (rows, k_in) or y.shape != y_shape or x.dtype != row_dt or y.dtype != row_dt or x.get_device() != index
+        n_o = b_shape[1]
+        y_want = (rows, n_o)
+        if (x.shape != x_want or y.shape != y_want or x.dtype != row_dt or y.dtype != row_dt or x.get_device() != index
                 or y.get_device() != index or not x.is_contiguous() or not y.is_contiguous()):
             raise ValueError("adapt_rows rows must be contiguous, of one type, on the banks' device, and match their bank")
-        if o is not y and (o.shape != y_shape or o.dtype != row_dt or o.get_device() != index or not o.is_contiguous()):
+        if o is not y and (o.shape != y_want or o.dtype != row_dt or o.get_device() != index or not o.is_contiguous()):
             raise ValueError("adapt_rows outputs must be contiguous, of the rows' type and shape, on the banks' device")
-        packed += (a.data_ptr(), b.data_ptr(), 0 if s is None else s.data_ptr(), b_shape[1])
-        px.append(x.data_ptr()); py.append(y.data_ptr()); po.append(o.data_ptr()); n_out.append(b_shape[1])
+        packed += (a.data_ptr(), b.data_ptr(), 0 if s is None else s.data_ptr(), n_o)
+        px.append(x.data_ptr())
+        py.append(y.data_ptr())
+        po.append(o.data_ptr())
+        n_out.append(n_o)
     if rows == 0:
         return list(outs)
-    # the C side's arrays as bytes: b200rwkv_adapters (three pointers, an int32 and its padding) and pointers
-    banks_c, pointers = struct.pack("=" + "QQQi4x" * n, *packed), "=%dQ" % n
-    shape = (count, rank, k_in, _DENSE_DTYPES[dt])
+    # the C side's arrays as one buffer: n b200rwkv_adapters (three pointers, an int32 and its padding), three times n pointers
+    arrays = C.create_string_buffer(_ADAPT_PACK[n].pack(*packed, *px, *py, *po), 56 * n)
+    at = C.addressof(arrays)
+    code = _DENSE_DTYPES[dt]
+    tokens = rows // streams
+    nbytes = _adapt_workspace(tuple(n_out), count, rank, k_in, code, streams, tokens)
     with _on(index):
-        ws = torch.empty(_adapt_workspace(tuple(n_out), *shape, streams, rows // streams), dtype=torch.uint8, device=a0.device)
-        _lib.check(_lib.lib().b200rwkv_adapt_rows(n, banks_c, *shape, struct.pack(pointers, *px), struct.pack(pointers, *py),
-                                                  struct.pack(pointers, *po), _DENSE_DTYPES[row_dt], ids.data_ptr(), streams,
-                                                  rows // streams, ws.data_ptr(), ws.numel(), _raw_stream(index)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a0.device)
+        _lib.check(_lib.lib().b200rwkv_adapt_rows(n, at, count, rank, k_in, code, at + 32 * n, at + 40 * n, at + 48 * n, _DENSE_DTYPES[row_dt],
+                                                  ids.data_ptr(), streams, tokens, ws.data_ptr(), nbytes, _raw_stream(index)))
     return list(outs)
+
+
+_ADAPT_PACK = {n: struct.Struct("=" + "QQQi4x" * n + "%dQ" % (3 * n)) for n in (1, 2, 3)}
 
 
 @lru_cache(maxsize=1024)
