@@ -217,9 +217,10 @@ struct ShrinkRing {
   static_assert(kStages >= 2, "a block ahead of the one in use");
 };
 
+// The split's sums of a tile as a table [count][16 * MT] in shared memory, to be read after a barrier.
 template <typename TX, typename TW, int MT, int NT>
-__device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int mat, int split, int chunk, const int* rows,
-                                            int count, char* shared) {
+__device__ __forceinline__ float* shrink_sums(const AdaptParams& P, const TX* x, const TW* a, int split, int chunk, const int* rows, int count,
+                                              char* shared) {
   using Ring = ShrinkRing<TX, TW, MT>;
   constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
@@ -346,10 +347,7 @@ __device__ __forceinline__ void shrink_sums(const AdaptParams& P, const TX* x, c
     for (int w = 0; w < kShrinkWarps; ++w) s += red[(w * 16 + r) * kStride + j];
     part_sums[i] = s;
   }
-  shrink_join(P, part_sums, count * RC, [](int i) { return i; }, [&](int i, float s) {
-    const int r = i / RC, j = chunk * RC + i - r * RC;
-    if (j < rank) P.h[mat][size_t(rows[r]) * rank + j] = s;
-  });
+  return part_sums;
 }
 
 template <typename TX, typename TW, int MT>
@@ -364,8 +362,14 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_kernel(const A
   if (count == 0 || id < 0) return;        // the whole cluster
   const TX* x = static_cast<const TX*>(P.x[mat]);
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * P.rank * P.K;
-  if (count <= 8) shrink_sums<TX, TW, MT, 1>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
-  else shrink_sums<TX, TW, MT, 2>(P, x, a, mat, split, blockIdx.y, rows, count, shared);
+  constexpr int RC = 16 * MT;
+  const int chunk = blockIdx.y;
+  float* sums = count <= 8 ? shrink_sums<TX, TW, MT, 1>(P, x, a, split, chunk, rows, count, shared)
+                           : shrink_sums<TX, TW, MT, 2>(P, x, a, split, chunk, rows, count, shared);
+  shrink_join(P, sums, count * RC, [](int i) { return i; }, [&](int i, float s) {
+    const int r = i / RC, j = chunk * RC + i - r * RC;
+    if (j < P.rank) P.h[mat][size_t(rows[r]) * P.rank + j] = s;
+  });
 }
 
 template <typename TY>
@@ -461,6 +465,20 @@ struct ExpandRing {
 };
 template <typename TY>
 __host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * ((rank + kc - 1) / kc * (kc / 16)) * (sizeof(TY) == 2 ? 2 : 3) * 256; }
+
+// Four ranks of a row of h into their fragments: 16 step + 4 t .. + 3 of a step and lane, or with 32 ranks a stage
+// 32 (step / 2) + 8 t + 4 (step % 2) .. + 3.
+template <typename TY, int KC>
+__device__ __forceinline__ void expand_put_h(char* shared, int ksteps, int r, int j4, float4 s) {
+  constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
+  uint32_t lo[PH], hi[PH];
+  split_pair<PH>(s.x, s.y, lo);
+  split_pair<PH>(s.z, s.w, hi);
+  const int ks = KC == 16 ? j4 >> 2 : (j4 >> 3) * 2 + (j4 & 1), t = KC == 16 ? j4 & 3 : (j4 >> 1) & 3;
+  uint2* f = reinterpret_cast<uint2*>(shared) + ((r >> 3) * ksteps + ks) * PH * 32 + (r & 7) * 4 + t;
+#pragma unroll
+  for (int p = 0; p < PH; ++p) f[p * 32] = make_uint2(lo[p], hi[p]);
+}
 
 // NT: products of 8 rows; stage_h() puts the tile's h into shared memory.
 template <typename TY, typename TW, int KC, bool VEC, int NT, typename StageH>
@@ -623,7 +641,6 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
 template <typename TY, typename TW, int KC, bool VEC>
 __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const AdaptParams P) {
   using Ring = ExpandRing<TY, TW, KC>;
-  constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
   extern __shared__ __align__(16) char shared[];
   __shared__ int rows[kAdaptRows];
   __shared__ size_t row_at[16];                            // where they start in y and out
@@ -652,14 +669,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
       const int r = i / r4, j4 = i - r * r4, j = j4 * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < count && j < rank) s = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(rows[r]) * rank + j));
-      uint32_t lo[PH], hi[PH];
-      split_pair<PH>(s.x * scale, s.y * scale, lo);
-      split_pair<PH>(s.z * scale, s.w * scale, hi);
-      // ranks of a step and lane: 16 step + 4 t .. + 3, or with 32 ranks a stage 32 (step / 2) + 8 t + 4 (step % 2) .. + 3
-      const int ks = KC == 16 ? j4 >> 2 : (j4 >> 3) * 2 + (j4 & 1), t = KC == 16 ? j4 & 3 : (j4 >> 1) & 3;
-      uint2* f = reinterpret_cast<uint2*>(shared) + ((r >> 3) * ksteps + ks) * PH * 32 + (r & 7) * 4 + t;
-#pragma unroll
-      for (int p = 0; p < PH; ++p) f[p * 32] = make_uint2(lo[p], hi[p]);
+      expand_put_h<TY, KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
     }
     __syncthreads();
   };
@@ -668,6 +678,70 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   const int c0 = c_begin + warp * Ring::kCols;
   if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
   else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
+}
+
+// Both in one launch, for calls of a few tiles, where a launch and the hand-over of h through memory are most of the time: a
+// cluster of eight CTAs per tile and matrix, each with an eighth of K, then of the columns; h meets in shared memory.
+constexpr int kFusedCtas = 8;
+static_assert(kFusedCtas <= kAdaptMaxSplits, "");
+
+template <typename T, typename TW, int MT>
+struct FusedShape {
+  static constexpr int KC = MT == 1 ? 16 : 32, kH = expand_h_bytes<T>(16 * MT, KC), kRing = kExpandWarps * ExpandRing<T, TW, KC>::kWarp;
+  static constexpr int kSmem = kH + kRing + ShrinkRing<T, TW, MT>::kSmem;
+  static_assert(kSmem <= 226 * 1024, "");
+};
+
+template <typename T, typename TW, int MT, bool VEC>
+__global__ void __launch_bounds__(kExpandThreads, 1) adapt_fused_kernel(const AdaptParams P) {
+  using F = FusedShape<T, TW, MT>;
+  constexpr int KC = F::KC, RC = 16 * MT, kCols = ExpandRing<T, TW, KC>::kCols;
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ __align__(16) char shared[];
+  __shared__ int rows[kAdaptRows];
+  __shared__ size_t row_at[16];
+  __shared__ uint32_t mask[kAdaptWindow / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, tile = blockIdx.x / kFusedCtas, part = blockIdx.x - tile * kFusedCtas, mat = blockIdx.y;
+  int id = -1;
+  const int count = adapt_tile(P, tile, rows, mask, &id), N = P.n_out[mat], rank = P.rank;
+  const int per = (N + kFusedCtas * kCols - 1) / (kFusedCtas * kCols) * kCols, c_begin = part * per, c_end = min(N, c_begin + per);
+  const T* y = static_cast<const T*>(P.y[mat]);
+  T* out = static_cast<T*>(P.out[mat]);
+  if (count == 0) return;                                  // the whole cluster, here and below
+  if (id < 0) {
+    if (y != out && c_begin < c_end) adapt_copy<T, VEC>(y, out, rows, count, N, c_begin, c_end);
+    return;
+  }
+  if (tid < 16) row_at[tid] = size_t(rows[tid < count ? tid : 0]) * N;
+  const int ksteps = (rank + KC - 1) / KC * (KC / 16);
+  char *slots = shared + F::kH + warp * ExpandRing<T, TW, KC>::kWarp, *work = shared + F::kH + F::kRing;
+  const T* x = static_cast<const T*>(P.x[mat]);
+  const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * rank * P.K;
+  auto stage_h = [&] {
+    float* sums = count <= 8 ? shrink_sums<T, TW, MT, 1>(P, x, a, part, 0, rows, count, work) : shrink_sums<T, TW, MT, 2>(P, x, a, part, 0, rows, count, work);
+    cluster.sync();
+    const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
+    const int r4 = ksteps * 4, padded = (count + 7) / 8 * 8;         // groups of four ranks; rows
+    for (int i = tid; i < padded * r4; i += kExpandThreads) {
+      const int r = i / r4, j4 = i - r * r4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < count && j4 * 4 < rank) {
+        float4 v[kFusedCtas];
+#pragma unroll
+        for (int c = 0; c < kFusedCtas; ++c) v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + r * RC + j4 * 4, c));
+        s = v[0];
+#pragma unroll
+        for (int c = 1; c < kFusedCtas; ++c) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
+      }
+      expand_put_h<T, KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
+    }
+    cluster.sync();                                        // the tables are read before their CTAs go on or leave
+  };
+  const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
+  const int c0 = c_begin + warp * kCols;
+  if (count <= 8) expand_columns<T, TW, KC, VEC, 1>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
+  else expand_columns<T, TW, KC, VEC, 2>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
 }
 
 }  // namespace b200

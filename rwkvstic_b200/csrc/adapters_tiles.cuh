@@ -612,12 +612,14 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
 }
 
 struct AdaptShape {
+  bool fused;                              // one launch
   bool tiles1, tiles2;                     // the forms for 128 rows of a stream, else for gathered tiles of 16
   int n1, n2;                              // tiles that a launch has at most; CTAs of the second launch's form for tiles
   int splits, mt;                          // first launch: CTAs that share K; gathered: ranks of a CTA in 16
   int kc, chunk_cols, chunks;              // second launch: ranks per stage (gathered), columns of a CTA or step, those of all matrices
 };
 
+// Calls whose tiles' clusters of eight all run at once, with at most 64 KB of B per CTA, take one launch.
 // Streams of 64 rows or more are cut into tiles of 128; shorter ones are gathered.  The second launch has its form for tiles for
 // ranks up to 128 and rows that start on 16 bytes (`aligned`; y passes as bulk copies), one CTA per SM.
 // Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
@@ -635,6 +637,8 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   };
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.kc = rank <= 16 ? 16 : 32;
+  s.fused = !s.tiles1 && rank <= 16 * s.mt && (long long)s.n1 * nmat * kFusedCtas <= sms;
+  for (int i = 0; i < nmat; ++i) s.fused = s.fused && (long long)n_out[i] * rank * (w_pieces == 3 ? 4 : 2) <= kFusedCtas * 64 * 1024;
   const int per_cta = s.tiles1 ? kShrinkTileRanks : 16 * s.mt;
   const long long ctas = busy(s.n1, s.tiles1) * nmat * ((rank + per_cta - 1) / per_cta);
   s.splits = 1;

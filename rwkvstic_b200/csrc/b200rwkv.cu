@@ -815,9 +815,29 @@ static cudaError_t launch_adapt_expand(AdaptParams& P, const AdaptShape& sh, boo
   return vec ? launch_adapt_expand_as<TY, TW, 32, true>(P, sh, stream) : launch_adapt_expand_as<TY, TW, 32, false>(P, sh, stream);
 }
 
+template <typename T, typename TW, int MT>
+static cudaError_t launch_adapt_fused(const AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
+  static bool configured[2][64];
+  constexpr int smem = FusedShape<T, TW, MT>::kSmem;
+  const dim3 grid(sh.n1 * kFusedCtas, P.nmat);
+  cudaError_t e;
+  if (vec) {
+    e = allow_smem(adapt_fused_kernel<T, TW, MT, true>, smem, configured[1]);
+    return e == cudaSuccess ? launch_clustered(kFusedCtas, adapt_fused_kernel<T, TW, MT, true>, grid, dim3(kExpandThreads), smem, stream, P) : e;
+  }
+  e = allow_smem(adapt_fused_kernel<T, TW, MT, false>, smem, configured[0]);
+  return e == cudaSuccess ? launch_clustered(kFusedCtas, adapt_fused_kernel<T, TW, MT, false>, grid, dim3(kExpandThreads), smem, stream, P) : e;
+}
+
 template <typename TY, typename TW>
 static cudaError_t launch_adapt(AdaptParams& P, const AdaptShape& sh, bool vec, cudaStream_t stream) {
   g_chain_launch = false;        // the first launch waits for the work in front of the call, which may still write its inputs
+  if (sh.fused) {
+    P.splits = kFusedCtas;
+    if (sh.mt == 1) return launch_adapt_fused<TY, TW, 1>(P, sh, vec, stream);
+    if (sh.mt == 2) return launch_adapt_fused<TY, TW, 2>(P, sh, vec, stream);
+    if constexpr (AdaptType<TW>::kPieces == 1) return launch_adapt_fused<TY, TW, 4>(P, sh, vec, stream);
+  }
   cudaError_t e = launch_adapt_shrink<TY, TW>(P, sh, stream);
   return e == cudaSuccess ? launch_adapt_expand<TY, TW>(P, sh, vec, stream) : e;
 }
