@@ -1,21 +1,26 @@
 // Low-rank adapters of many requests beside shared projections: out[row] = y[row] + scale[id] * (x[row] A[id]^T) B[id]^T
 // for rows whose stream has adapter id, out[row] = y[row] for the others.  A [rank][K], B [N][rank] per adapter.
 //
-// Two launches.  The first forms h = x A^T (K long, rank short), the second adds h B^T onto y (rank short, N long).
-// Rows of one adapter share its weights: a CTA takes a tile of up to `rt` rows that all have the same adapter.  Streams of
-// rt rows or more are cut into tiles; shorter ones are gathered: CTA s looks through the ids of its window of kAdaptWindow
-// streams, in the order of the streams, and leads a tile where a multiple of rt rows of its adapter ends in front of one of
-// its rows.  So no pass sorts the rows and no count travels to the host; CTAs that lead nothing leave.
+// h = x A^T has a long sum (K) and few columns (the rank), y + h B^T a short sum and many columns.  Three forms:
+//   a cluster of eight CTAs per tile and matrix does both, for calls of a few tiles (adapt_fused_kernel);
+//   two launches, the second started before the first ends, over gathered tiles of up to 16 rows (adapt_shrink_kernel and
+//   adapt_expand_kernel below, mma.sync);
+//   the same over tiles of 128 rows of one stream on tcgen05, where products are many (adapters_tiles.cuh, which has the rules).
+// Rows of one adapter share its weights, so a tile is of one adapter.  Streams of 16 rows or more are cut into tiles; shorter
+// ones are gathered: CTA s looks through the ids of its window of kAdaptWindow streams, in the order of the streams, and leads
+// a tile where a multiple of 16 rows of its adapter ends in front of one of its rows.  So no pass sorts the rows and no count
+// travels to the host; CTAs that lead nothing leave.
 //
-// Products run on the tensor cores (mma.sync m16n8k16) with fp32 sums.  Operands that are not of one 16-bit type are cut
-// into bfloat16 pieces: a float is exactly three (the upper 8 bits of its significand, the next 8, the last 8), a half
-// exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21 of the whole together and left out.  The tensor cores
-// cut their sums off, so no chain is longer than 64 k of a lane before its part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity
-// or a NaN comes out as NaN, where it has an adapter.
-// What bounds both is memory: h takes rank multiplications per value of x, y takes rank per value.  At rank 64 with fp32 rows
-// that is 48 products of pieces a byte, below what mma.sync sustains beside the loads, so nothing is gained by staging
-// operands for tcgen05; fragments go from global memory to registers directly.  The index along a product is free to permute,
-// and is, so that a lane's elements are consecutive: 16 bytes of A, 8 of B.
+// Operands that are not of one 16-bit type are cut into bfloat16 pieces: a float is exactly three (the upper 8 bits of its
+// significand, the next 8, the last 8), a half exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21
+// of the whole together and left out.  The tensor cores cut their sums off, so no chain is longer than 64 k of a lane before its
+// part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
+// where it has an adapter.
+// What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces: 7B key, value and receptance for
+// 256 streams of 64 adapters (338 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (117 MB)
+// 41; 7B ffn for 64 streams of 16 adapters (57 MB) 25.5.  Fragments go from global memory to a lane's own slots of shared memory
+// and from there to its registers, without a barrier between warps.  The index along a product is free to permute, and is, so
+// that a lane's elements are consecutive: 16 bytes of A, 8 of B.
 #pragma once
 
 #include <cooperative_groups.h>

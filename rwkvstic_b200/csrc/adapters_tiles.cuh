@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
           const int rows = min(kExpandHalf, G.count - hf * kExpandHalf);
           const int r0 = part * 16;
           if (r0 < rows) {
-            if (G.id >= 0) {
+            if (G.id >= 0 || !ok) {
               float d[16];
               if (ok) {
                 tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * kAdaptTile + hf * kExpandHalf + r0), d);
@@ -619,17 +619,42 @@ struct AdaptShape {
   int kc, chunk_cols, chunks;              // second launch: ranks per stage (gathered), columns of a CTA or step, those of all matrices
 };
 
-// Calls whose tiles' clusters of eight all run at once, with at most 64 KB of B per CTA, take one launch.
-// Streams of 64 rows or more are cut into tiles of 128; shorter ones are gathered.  The second launch has its form for tiles for
-// ranks up to 128 and rows that start on 16 bytes (`aligned`; y passes as bulk copies), one CTA per SM.
+// SMs that clusters of one CTA per SM can take at once.  A cluster stays inside a GPC and GPCs have SMs over: 15 clusters of eight
+// run together on 148 SMs, not 18 (a 16th costs a second pass: rank 16, 10240 -> 2560, 240 rows 7.3 us, 256 rows 12.8), 32 of four.
+inline int cluster_room(int ctas, int sms) { return ctas >= 8 ? sms * 13 / 16 : ctas >= 4 ? sms * 7 / 8 : sms; }
+
+// Products of pieces i and j with i + j < limit.
+inline int piece_products(int a, int b, int limit) {
+  int n = 0;
+  for (int i = 0; i < a; ++i)
+    for (int j = 0; j < b; ++j) n += i + j < limit;
+  return n;
+}
+
+// Which form.  Calls whose tiles' clusters of eight all run at once, with at most 64 KB of B per CTA, take one launch (1.5B key,
+// value and receptance, one row: 5.1 us against 6.2 in two; rank 16, 10240 -> 2560, 240 rows 7.3 against 10.9).
+// Tiles of 128 rows are for streams of 64 rows or more, where the products are many: each launch by itself, since gathered tiles
+// start sooner and tcgen05 takes products faster.  Time of gathered tiles beside that of these, 64 to 8192 rows in 1 to 8 streams,
+// 768 to 10240 wide, ranks 8 to 128, all types (least, median, most):
+//   first launch, by products of 16 ranks x rows x K
+//     about 8M -29, -16, -4 %;  16M -18, -8, +22;  32M -7, +4, +25;  64M 0, +16, +108;  256M and more +14, +106, +148
+//   second launch, by products of 16 ranks x rows x N x bytes of y
+//     about 32M -23, -11, +3 %;  64M -14, -2, +15;  128M -7, +16, +41;  512M +6, +29, +84;  2000M +40, +76, +110
+// Ranks up to 128 and rows that start on 16 bytes for the second (`aligned`; y passes as bulk copies), one CTA per SM.
 // Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
 // Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves three CTAs per SM (each starts with
 // a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40).
-inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, bool aligned, int sms) {
+inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int row_bytes, bool same16,
+                              bool aligned, int sms) {
   AdaptShape s;
   auto cut = [&](int rows) { return T < rows ? streams : streams * ((T + rows - 1) / rows); };
-  s.tiles1 = T >= 64;
-  s.tiles2 = T >= 64 && rank <= kTileRankMax && aligned;
+  long long columns = 0;
+  for (int i = 0; i < nmat; ++i) columns += n_out[i];
+  const long long work = (long long)streams * T * ((rank + 15) / 16);
+  const int shrink_products = same16 ? 1 : piece_products(row_bytes == 4 ? 3 : w_pieces, w_pieces, 3);
+  const int expand_products = piece_products(row_bytes == 4 ? 3 : 2, w_pieces, row_bytes == 4 ? 3 : 2);
+  s.tiles1 = T >= 64 && work * shrink_products * K * nmat >= 24000000;
+  s.tiles2 = T >= 64 && work * expand_products * columns * row_bytes >= 60000000 && rank <= kTileRankMax && aligned;
   s.n1 = s.tiles1 ? streams * ((T + kAdaptTile - 1) / kAdaptTile) : cut(kAdaptRows);
   auto busy = [&](int n, bool tiled) {                   // tiles that lead rows
     const long long most = adapters + (long long)streams * T / kAdaptRows + 1;
@@ -637,12 +662,12 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   };
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.kc = rank <= 16 ? 16 : 32;
-  s.fused = !s.tiles1 && rank <= 16 * s.mt && (long long)s.n1 * nmat * kFusedCtas <= sms;
+  s.fused = !s.tiles1 && rank <= 16 * s.mt && (long long)s.n1 * nmat * kFusedCtas <= cluster_room(kFusedCtas, sms);
   for (int i = 0; i < nmat; ++i) s.fused = s.fused && (long long)n_out[i] * rank * (w_pieces == 3 ? 4 : 2) <= kFusedCtas * 64 * 1024;
   const int per_cta = s.tiles1 ? kShrinkTileRanks : 16 * s.mt;
   const long long ctas = busy(s.n1, s.tiles1) * nmat * ((rank + per_cta - 1) / per_cta);
   s.splits = 1;
-  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= (s.tiles1 ? 1LL : 2LL) * sms && K >= 512 * s.splits) s.splits *= 2;
+  while (s.splits < kAdaptMaxSplits && ctas * 2 * s.splits <= (s.tiles1 ? 1LL : 2LL) * cluster_room(2 * s.splits, sms) && K >= 512 * s.splits) s.splits *= 2;
   s.chunks = 0;
   if (s.tiles2) {                                        // steps of all matrices for a tile, and CTAs
     s.chunk_cols = kAdaptTile;

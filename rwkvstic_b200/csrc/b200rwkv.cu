@@ -2035,6 +2035,11 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
 }
 
 // ---- many requests: adapters, verification of drafted tokens, the state after the accepted ones
+static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
+
 static int adapt_weight_pieces(int dtype) { return dtype == B200RWKV_F32 ? 3 : dtype == B200RWKV_F16 ? 2 : 1; }
 
 static bool adapt_tile_fits(int dtype, int row_dtype, int rank) {
@@ -2086,9 +2091,18 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
     vec = vec && m.n_out % 4 == 0 && reinterpret_cast<uintptr_t>(y[i]) % (4 * eb) == 0 && reinterpret_cast<uintptr_t>(out[i]) % (4 * eb) == 0;
     aligned = aligned && m.n_out * eb % 16 == 0 && aligned16(y[i]) && aligned16(out[i]);
   }
+  // rows are read ahead of what other CTAs write: a y is its own out or apart from every out, an x apart from every out
+  const size_t row_bytes = size_t(streams) * tokens_per_stream * eb;
+  auto meet = [&](const void* p, int np, const void* q, int nq) { return overlap(p, row_bytes * np, q, row_bytes * nq); };
+  for (int i = 0; i < nmat; ++i)
+    for (int j = 0; j < nmat; ++j)
+      if (meet(out[i], P.n_out[i], x[j], k_in) || (i != j && meet(out[i], P.n_out[i], out[j], P.n_out[j])) ||
+          (!(i == j && out[i] == y[j]) && meet(out[i], P.n_out[i], y[j], P.n_out[j])))
+        return fail(B200RWKV_EINVAL, "adapt_rows: out %d overlaps another out, an x, or a y that is not its own", i);
   // the form for tiles keeps h and 64 or 128 ranks of B in shared memory
   aligned = aligned && adapt_tile_fits(dtype, row_dtype, rank);
-  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype), aligned, device_sms());
+  const AdaptShape sh = adapt_shape(nmat, P.n_out, n_adapters, rank, k_in, streams, tokens_per_stream, adapt_weight_pieces(dtype),
+                                    int(eb), row_dtype == dtype && eb == 2, aligned, device_sms());
   for (int i = 0; i < nmat; ++i) P.chunk_end[i] = (i ? P.chunk_end[i - 1] : 0) + (P.n_out[i] + sh.chunk_cols - 1) / sh.chunk_cols;
   P.ids = reinterpret_cast<const long long*>(ids);
   P.nmat = nmat; P.adapters = n_adapters; P.rank = rank; P.K = k_in; P.R = streams * tokens_per_stream; P.T = tokens_per_stream;
@@ -2137,6 +2151,10 @@ int b200rwkv_advance_state(const float* state, float* out, const int64_t* counts
     return fail(B200RWKV_EINVAL, "advance_state: streams=%d layers=%d tokens=%d channels=%d (channels a multiple of 4)", streams, layers, tokens, channels);
   if (!aligned16(state) || !aligned16(out) || !aligned16(trace) || !aligned16(params))
     return fail(B200RWKV_EINVAL, "advance_state: state, out, trace and params must be 16-byte aligned");
+  const size_t state_bytes = size_t(streams) * layers * 5 * channels * 4;
+  if ((out != state && overlap(out, state_bytes, state, state_bytes)) ||
+      overlap(out, state_bytes, trace, size_t(layers) * 4 * streams * tokens * channels * 4) || overlap(out, state_bytes, params, size_t(layers) * 5 * channels * 4))
+    return fail(B200RWKV_EINVAL, "advance_state: out is state itself or apart from state, trace and params");
   AdvanceParams P;
   P.state = state; P.out = out; P.trace = trace; P.params = params; P.counts = reinterpret_cast<const long long*>(counts);
   P.B = streams; P.L = layers; P.T = tokens; P.C = channels;

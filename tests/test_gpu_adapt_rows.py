@@ -98,6 +98,29 @@ def test_against_formula(shape, w, t):
     check(banks, xs, ids, ys)
 
 
+# Streams of 64 rows and more whose products are many enough for the tiles of 128 rows, in every type.
+TILES = [
+    (3, 1029, 1016, [1024, 392, 8], 100, 2),     # several matrices, a last tile of 5 rows, columns that end inside a step
+    (40, 64, 3208, [2000], 48, 3),               # half a tile per stream, more tiles than SMs
+    (1, 2000, 12008, [7520], 12, 1),
+    (2, 701, 2400, [5400], 128, 2),
+    (3, 129, 8200, [10000], 128, 3),             # K cut over CTAs, a tile of one row
+    (6, 200, 2056, [1000, 136, 4096], 68, 4),
+    (64, 300, 1304, [808], 4, 2),
+    (9, 1000, 272, [64], 256, 2),                # only the first launch
+    (2, 700, 8, [8192], 64, 2),                  # only the second
+    (4, 500, 2048, [2049], 32, 2),               # rows that start anywhere
+]
+
+
+@pytest.mark.parametrize("w,t", COMBOS)
+@pytest.mark.parametrize("shape", TILES, ids=[f"{s[0]}x{s[1]}_k{s[2]}_r{s[4]}" for s in TILES])
+def test_tiles_against_formula(shape, w, t):
+    banks, xs, ids, ys = make(*shape, TYPES[w], TYPES[t], seed=len(str(shape)))
+    check(banks, xs, ids, ys, [torch.full_like(y, 7.0) for y in ys])
+    check(banks, xs, ids, ys)
+
+
 @pytest.mark.parametrize("w,t", COMBOS)
 def test_rows_without_adapter_are_not_read(w, t):
     """Their x may hold anything, and ids outside the bank mean none."""
@@ -185,6 +208,41 @@ def test_two_streams_at_once():
                 ops.adapt_rows(b, x, i, y, o)
     torch.cuda.synchronize()
     assert all(torch.equal(o[0], w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 512, [256, 256], 16, 3), (70, 1, 512, [256, 256], 16, 3), (3, 300, 2048, [2048, 512], 64, 3)],
+                         ids=["one launch", "gathered", "tiles"])
+def test_every_form_captured_beside_other_calls(shape):
+    """A captured call replayed on one stream while eager calls of the same shape run on another."""
+    cases = [make(*shape, torch.bfloat16, torch.float32, seed=s) for s in range(2)]
+    want = [[o.clone() for o in ops.adapt_rows(b, x, i, y, [torch.empty_like(v) for v in y])] for b, x, i, y in cases]
+    outs = [[torch.empty_like(v) for v in c[3]] for c in cases]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.adapt_rows(*cases[0], outs[0])
+    other = torch.cuda.Stream()
+    for _ in range(10):
+        graph.replay()
+        with torch.cuda.stream(other):
+            ops.adapt_rows(*cases[1], outs[1])
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+def test_outputs_that_overlap_are_refused():
+    banks, xs, ids, ys = make(4, 2, 64, [32, 32], 8, 2, torch.bfloat16, torch.float32)
+    flat = torch.zeros(4096, device=DEV)
+    near = [flat[:256].view(8, 32), flat[128:384].view(8, 32)]
+    for y, out in (([ys[0], ys[0]], [ys[0], ys[0]]), (ys, [ys[1], ys[0]]), (ys, near), ([near[0], ys[1]], [near[1], ys[1]])):
+        with pytest.raises(_lib.B200RWKVError, match="overlaps"):
+            ops.adapt_rows(banks, xs, ids, y, out)
+    square, xs, ids, ys = make(4, 2, 64, [64], 8, 2, torch.bfloat16, torch.float32)
+    with pytest.raises(_lib.B200RWKVError, match="overlaps"):
+        ops.adapt_rows(square, xs, ids, ys, xs)
+    side = [flat[:512].view(8, 64), flat[512:1024].view(8, 64)]        # next to each other is fine
+    ops.adapt_rows(square * 2, xs * 2, ids, side)
 
 
 def test_pack_adapters_of_different_ranks():

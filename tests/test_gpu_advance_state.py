@@ -135,3 +135,14 @@ def test_refusals():
     same = state.clone()
     assert torch.equal(ops.advance_state(state, counts, trace[:, :, :, :0].contiguous(), params), same)
     assert ops.advance_state(state[:0], counts[:0], trace[:, :, :0].contiguous(), params).shape[0] == 0
+
+
+def test_outputs_that_overlap_are_refused():
+    state, counts, trace, params = make(3, 2, 4, 64)
+    room = torch.zeros(4, 2, 5, 64, device=DEV)
+    for bad in [(room[:3], counts, trace, params, room[1:]), (state, counts, trace, params, trace.view(-1)[:state.numel()].view_as(state))]:
+        with pytest.raises(_lib.B200RWKVError, match="apart"):
+            ops.advance_state(*bad)
+    room[:3] = state
+    again = ops.advance_state(room[:3], counts, trace, params, room[:3])       # the same memory under another name
+    assert torch.equal(again, ops.advance_state(state, counts, trace, params, torch.empty_like(state)))
