@@ -17,8 +17,8 @@
 // part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
 // where it has an adapter.
 // What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces: 7B key, value and receptance for
-// 256 streams of 64 adapters (338 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (117 MB)
-// 41; 7B ffn for 64 streams of 16 adapters (57 MB) 25.5.  Fragments go from global memory to a lane's own slots of shared memory
+// 256 streams of 200 adapters (332 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (115 MB)
+// 33; 7B ffn for 64 streams of 48 adapters (56 MB) 27.  Fragments go from global memory to a lane's own slots of shared memory
 // and from there to its registers, without a barrier between warps.  The index along a product is free to permute, and is, so
 // that a lane's elements are consecutive: 16 bytes of A, 8 of B.
 #pragma once
@@ -390,42 +390,36 @@ __device__ __forceinline__ void adapt_store(TY* p, float v) {
   else *p = __float2bfloat16_rn(v);
 }
 
-// Four consecutive elements of a row, held as loaded.
-template <typename TY>
-struct AdaptFour {
-  uint32_t w[sizeof(TY)];
-  __device__ __forceinline__ void load(const TY* p) {
-    if constexpr (sizeof(TY) == 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+// W consecutive elements of a row (1, 2 or 4), held as loaded.
+template <typename TY, int W>
+struct AdaptFew {
+  using Word = std::conditional_t<W * sizeof(TY) == 16, uint4, std::conditional_t<W * sizeof(TY) == 8, uint2, std::conditional_t<W * sizeof(TY) == 4, uint32_t, unsigned short>>>;
+  Word w;
+  __device__ __forceinline__ void load(const TY* p) { w = *reinterpret_cast<const Word*>(p); }
+  __device__ __forceinline__ void store(TY* p) const { *reinterpret_cast<Word*>(p) = w; }
+  // + f[0 .. W), rounded once; W 2 only of fp32
+  __device__ __forceinline__ void add_store(TY* p, const float* f) const {
+    if constexpr (W == 1) {
+      adapt_store(p, adapt_float(*reinterpret_cast<const TY*>(&w)) + f[0]);
+    } else if constexpr (W == 2 && sizeof(TY) == 4) {
+      const float2 d = *reinterpret_cast<const float2*>(f);
+      *reinterpret_cast<float2*>(p) = make_float2(__uint_as_float(w.x) + d.x, __uint_as_float(w.y) + d.y);
     } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x; w[1] = v.y;
+      const float4 d = *reinterpret_cast<const float4*>(f);
+      if constexpr (sizeof(TY) == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(__uint_as_float(w.x) + d.x, __uint_as_float(w.y) + d.y, __uint_as_float(w.z) + d.z, __uint_as_float(w.w) + d.w);
+      else
+        *reinterpret_cast<uint2*>(p) = make_uint2(add_pair(w.x, d.x, d.y), add_pair(w.y, d.z, d.w));
     }
   }
-  __device__ __forceinline__ void store(TY* p) const {
-    if constexpr (sizeof(TY) == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  }
-  // + f, rounded once
-  __device__ __forceinline__ void add_store(TY* p, const float (&f)[4]) const {
-    if constexpr (std::is_same<TY, float>::value) {
-      *reinterpret_cast<float4*>(p) = make_float4(__uint_as_float(w[0]) + f[0], __uint_as_float(w[1]) + f[1], __uint_as_float(w[2]) + f[2],
-                                                  __uint_as_float(w[3]) + f[3]);
+  static __device__ __forceinline__ uint32_t add_pair(uint32_t a, float x, float y) {
+    if constexpr (std::is_same<TY, __half>::value) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
+      const __half2 r = __floats2half2_rn(v.x + x, v.y + y);
+      return *reinterpret_cast<const uint32_t*>(&r);
     } else {
-      uint32_t o[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (std::is_same<TY, __half>::value) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          const __half2 r = __floats2half2_rn(a.x + f[2 * i], a.y + f[2 * i + 1]);
-          o[i] = *reinterpret_cast<const uint32_t*>(&r);
-        } else {
-          const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) + f[2 * i], __uint_as_float(w[i] & 0xffff0000u) + f[2 * i + 1]);
-          o[i] = *reinterpret_cast<const uint32_t*>(&r);
-        }
-      }
-      *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
+      const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(a << 16) + x, __uint_as_float(a & 0xffff0000u) + y);
+      return *reinterpret_cast<const uint32_t*>(&r);
     }
   }
 };
@@ -440,33 +434,27 @@ __device__ __forceinline__ void adapt_copy(const TY* y, TY* out, const int* rows
     const TY* from = y + at;
     TY* to = out + at;
     for (int c = lane * W; c < n; c += U * 32 * W) {
-      AdaptFour<TY> four[VEC ? U : 1];
-      TY one[VEC ? 1 : U];
+      AdaptFew<TY, W> few[U];
 #pragma unroll
       for (int k = 0; k < U; ++k)
-        if (c + k * 32 * W < n) {
-          if constexpr (VEC) four[k].load(from + c + k * 32 * W);
-          else one[k] = from[c + k * 32];
-        }
+        if (c + k * 32 * W < n) few[k].load(from + c + k * 32 * W);
 #pragma unroll
       for (int k = 0; k < U; ++k)
-        if (c + k * 32 * W < n) {
-          if constexpr (VEC) four[k].store(to + c + k * 32 * W);
-          else to[c + k * 32] = one[k];
-        }
+        if (c + k * 32 * W < n) few[k].store(to + c + k * 32 * W);
     }
   }
 }
 
 // The second launch, for tiles of up to 16 rows.  Shared memory: h in the fragments' own order, [8 rows][step of 16 ranks][piece]
 // [lane] of 8 bytes; then per warp the stages of B and the table in which its sums are turned.
-// KC: ranks of B per stage.
+// KC: ranks of B per stage.  Stages leave shared memory to L1, which holds the lines of y that are on their way: 3B head for
+// 48 x 5 rows 40 us with 4 stages of 16 ranks, 33 with 3 or 2.
 template <typename TY, typename TW, int KC>
 struct ExpandRing {
   static constexpr int MT = sizeof(TW) == 2 ? 4 : 2, kCols = 16 * MT;        // products of 16 columns that a warp forms at a time
   static constexpr int kLane = KC / 4 * int(sizeof(TW)), kUnit = kLane < 16 ? kLane : 16, kParts = kLane / kUnit;
   static constexpr int kStage = MT * 2 * 32 * kLane, kPitch = kCols + 4, kTurn = 16 * kPitch * 4;
-  static constexpr int kStages = KC == 16 ? 4 : sizeof(TW) == 2 ? 2 : 3, kWarp = kStages * kStage + kTurn;
+  static constexpr int kStages = KC == 16 ? 3 : sizeof(TW) == 2 ? 2 : 3, kWarp = kStages * kStage + kTurn;
 };
 template <typename TY>
 __host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * ((rank + kc - 1) / kc * (kc / 16)) * (sizeof(TY) == 2 ? 2 : 3) * 256; }
@@ -534,28 +522,37 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
     cp_async_commit();                                     // a group per stage, also an empty one
     to = to == (kStages - 1) * Ring::kStage ? 0 : to + Ring::kStage;
   };
+  // VEC: two or four columns per lane; four of fp32 rows cost the loop of 64 columns registers for the addresses of two rows, and
+  // it spilled (3B head with rows of 50280: 48 us, 32 with two)
+  constexpr int W = !VEC ? 1 : COLS == 64 && sizeof(TY) == 4 ? 2 : 4, kLanes = COLS / W < 32 ? COLS / W : 32, kAtOnce = 32 / kLanes;
+  constexpr int kPasses = 8 * NT / kAtOnce, kQ = COLS / (kLanes * W);
+  // y of the next columns is requested as this one's sums go out, where a stage is 16 ranks (3B head 42 -> 40 us, with 3 stages of B
+  // 33); with 32 ranks its registers are wanted for B (7B key, value and receptance, 256 streams 66 us so, 71 ahead)
+  constexpr bool kAhead = KC == 16;
+  const int my_row = lane / kLanes, my_col = lane % kLanes * W;
+  AdaptFew<TY, W> line[kPasses][kQ];
+  auto load_y = [&](int i, int c) {                        // pass i of the columns from c
+    const int r = i * kAtOnce + my_row;
+    const TY* p = y + row_at[r] + c + my_col;
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) request();         // weights: no part of what the first launch writes
+    for (int q = 0; q < kQ; ++q)
+      if (r < count && c + q * 32 + my_col < c_end) line[i][q].load(p + q * 32);
+  };
+  // weights and y: no part of what the first launch writes
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) request();
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (i * kAtOnce < count) load_y(i, c0);
+  }
   stage_h();
-  // sums go out row by row: VEC, half a warp per row, four columns per lane; else a warp per row, a column per lane
-  constexpr int kPass = VEC ? 4 * NT : 8 * NT, kLanes = COLS / 4, kRowsAtOnce = VEC ? 32 / kLanes : 1, kPasses = VEC ? (8 * NT + kRowsAtOnce - 1) / kRowsAtOnce : kPass;
-  const int my_row = VEC ? lane / kLanes : 0, my_col = VEC ? lane % kLanes * 4 : lane;
   const char* from = slots;
   for (; c0 < c_end; c0 += kStep) {
-    AdaptFour<TY> four[VEC ? kPasses : 1];
-    TY line[VEC ? 1 : kPasses][VEC ? 1 : COLS / 32];
+    if constexpr (!kAhead) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (i * kRowsAtOnce >= count) break;
-      const int r = i * kRowsAtOnce + my_row;
-      const TY* p = y + row_at[r] + c0 + my_col;
-      if constexpr (VEC) {
-        if (r < count && c0 + my_col < c_end) four[i].load(p);
-      } else {
-#pragma unroll
-        for (int q = 0; q < COLS / 32; ++q)
-          if (c0 + q * 32 + my_col < c_end) line[i][q] = p[q * 32];
-      }
+      for (int i = 0; i < kPasses; ++i)
+        if (i * kAtOnce < count) load_y(i, c0);
     }
     float acc[MT][NT][4];
 #pragma unroll
@@ -619,20 +616,13 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      if (i * kRowsAtOnce >= count) break;
-      const int r = i * kRowsAtOnce + my_row;
+      if (i * kAtOnce >= count) break;
+      const int r = i * kAtOnce + my_row;
       TY* p = out + row_at[r] + c0 + my_col;
-      if constexpr (VEC) {
-        if (r < count && c0 + my_col < c_end) {
-          const float4 v = *reinterpret_cast<const float4*>(turn + r * Ring::kPitch + my_col);
-          const float d[4] = {v.x, v.y, v.z, v.w};
-          four[i].add_store(p, d);
-        }
-      } else {
 #pragma unroll
-        for (int q = 0; q < COLS / 32; ++q)
-          if (c0 + q * 32 + my_col < c_end) adapt_store(p + q * 32, adapt_float(line[i][q]) + turn[r * Ring::kPitch + q * 32 + my_col]);
-      }
+      for (int q = 0; q < kQ; ++q)
+        if (r < count && c0 + q * 32 + my_col < c_end) line[i][q].add_store(p + q * 32, turn + r * Ring::kPitch + q * 32 + my_col);
+      if constexpr (kAhead) load_y(i, c0 + kStep);         // in flight until the next columns' sums are there
     }
   }
   cp_async_wait<0>();
@@ -666,6 +656,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   }
   const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);
   if (tid < 16) row_at[tid] = size_t(rows[tid < count ? tid : 0]) * N;
+  __syncthreads();
   auto stage_h = [&] {
     griddep_wait();
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
@@ -719,6 +710,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) adapt_fused_kernel(const Ad
     return;
   }
   if (tid < 16) row_at[tid] = size_t(rows[tid < count ? tid : 0]) * N;
+  __syncthreads();
   const int ksteps = (rank + KC - 1) / KC * (KC / 16);
   char *slots = shared + F::kH + warp * ExpandRing<T, TW, KC>::kWarp, *work = shared + F::kH + F::kRing;
   const T* x = static_cast<const T*>(P.x[mat]);

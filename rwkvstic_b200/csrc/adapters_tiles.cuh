@@ -642,8 +642,9 @@ inline int piece_products(int a, int b, int limit) {
 //     about 32M -23, -11, +3 %;  64M -14, -2, +15;  128M -7, +16, +41;  512M +6, +29, +84;  2000M +40, +76, +110
 // Ranks up to 128 and rows that start on 16 bytes for the second (`aligned`; y passes as bulk copies), one CTA per SM.
 // Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
-// Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves three CTAs per SM (each starts with
-// a search; 7B ffn for 64 streams 24, 26, 29 us with 2, 3, 6, 3B head for 240 rows 52, 41, 40).
+// Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves the two CTAs that an SM holds at
+// once, by the number of tiles where streams spread evenly over the adapters (7B ffn for 64 streams of 48 adapters 19, 20, 26 us
+// with two, three, six CTAs per SM; 16384 columns for 200 streams of 6 adapters 48, 58, 58).
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int row_bytes, bool same16,
                               bool aligned, int sms) {
   AdaptShape s;
@@ -678,9 +679,11 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   }
   s.n2 = cut(kAdaptRows);
   const int unit = kExpandWarps * (w_pieces < 3 ? 64 : 32);
+  const long long shared_by = adapters < streams ? adapters : streams, filled = (long long)streams * T / kAdaptRows + shared_by / 2;
+  const long long tiles = T >= kAdaptRows ? s.n2 : filled > shared_by ? filled : shared_by;        // about as many as lead rows
   long long units = 0;
   for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  const long long per = units * busy(s.n2, false) / (3LL * sms);
+  const long long per = (units * tiles + sms) / (2LL * sms);
   s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
   return s;
