@@ -178,6 +178,9 @@ class B200RWKV:
         self.emptyState = torch.zeros(self.n_layer, 5, self.n_embd, dtype=torch.float32, device=self.device)
         self.emptyState[:, 4] = -1e30
         self._build_descriptor()
+        # for accept; laid out here because accept may be captured
+        names = ("ln1.weight", "ln1.bias", "ln2.weight", "ln2.bias", "att.time_decay")
+        self._advance_params = torch.stack([torch.stack([ly.vec[k].reshape(-1) for k in names]) for ly in weights.layers]) if weights.layers else None
         self.stage_stream_rows = 2     # forward_rows_stage: up to this many rows go through the one-row step
         nbytes = int(self._L.b200rwkv_decode_workspace_bytes(C.byref(self._cmodel)))
         self._ws = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
@@ -445,9 +448,6 @@ class B200RWKV:
         """Move ``state [B,L,5,D]`` on, in place, by the first ``counts[b]`` (int64, device) of the tokens that
         ``forward_draft`` was given: the sure one and the accepted ones (``ops.verify_drafts``'s count plus one)."""
         from . import ops
-        if getattr(self, "_advance_params", None) is None:
-            names = ("ln1.weight", "ln1.bias", "ln2.weight", "ln2.bias", "att.time_decay")
-            self._advance_params = torch.stack([torch.stack([ly.vec[k].reshape(-1) for k in names]) for ly in self.w.layers])
         self.launch_count += 1
         return ops.advance_state(state, counts, trace, self._advance_params)
 

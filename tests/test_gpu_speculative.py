@@ -68,6 +68,26 @@ def test_streams_accept_different_numbers(model):
     close_states(state, want)
 
 
+def test_the_first_accept_may_be_a_captured_one():
+    """What accept needs of the weights is there before it is called, so an eager call behind a capture has it too."""
+    model = B200RWKV.from_checkpoint(synth_checkpoint(L, D, vocab=V, seed=13), device=DEV)
+    state, g = start(model, 4)
+    tokens, counts = torch.randint(0, V, (4, 3), generator=g).to(DEV), torch.tensor([1, 3, 0, 2], device=DEV)
+    _, trace = model.forward_draft(tokens, state)
+    captured = state.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        model.accept(captured, trace, counts)
+    eager = model.accept(state.clone(), trace, counts)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(captured, eager) and not torch.equal(eager[1], state[1])
+    want = state[1:2].clone()
+    model.forward_rows(tokens[1:2], want)
+    close_states(eager[1:2], want)
+
+
 def test_a_text_decoded_with_drafts_is_the_text_fed_plainly(model):
     """Draft, verify, accept, several times; then the tokens that came out are fed one after another from the first state."""
     B, K, rounds = 6, 3, 5
