@@ -367,8 +367,10 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
  *   workspace b200rwkv_adapt_rows_workspace_bytes(...) (0: a size that is not taken), 256-byte aligned; nothing
  *             is kept in it between calls
  * Sums are f32 over exact products of 16-bit pieces, h = x A^T stays f32, and out is rounded once.  Sums go over fixed parts
- * in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
- * adapter.  Two launches on `stream`, no allocation, capturable.  No counterpart in the reference.
+ * in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row
+ * of x that holds an infinity or a NaN comes out as NaN where it has an adapter.  One or two launches on `stream`, no
+ * allocation, capturable; device-side waits are bounded (1 s), and rows whose wait runs out come out as NaN.  Outputs that
+ * overlap more than their own y are refused.  No counterpart in the reference.
  */
 typedef struct b200rwkv_adapters {
   const void *a, *b;
@@ -413,7 +415,7 @@ int b200rwkv_verify_drafts(const float* target, int64_t target_stream_stride, in
  * [layers][4][streams][tokens][channels]: the residual stream in front of ln1 and of ln2, key and value of every token; params
  * device f32 [layers][5][channels]: ln1 weight and bias, ln2 weight and bias, w = -exp(time_decay).  Row 0 / 1 become the layer
  * norm of the last accepted token's rows, rows 2..4 take counts[s] WKV steps (agnosticRwkv.py:68-103).  channels a multiple of 4;
- * all buffers 16-byte aligned.  One launch, no allocation, capturable.
+ * all buffers 16-byte aligned, out state itself or apart from the other buffers.  One launch, no allocation, capturable.
  */
 int b200rwkv_advance_state(const float* state, float* out, const int64_t* counts, const float* trace, const float* params, int streams,
                            int layers, int tokens, int channels, void* stream);
