@@ -47,26 +47,31 @@ struct TileControl {
 __device__ __forceinline__ TileControl* tile_control(char* shared) { return reinterpret_cast<TileControl*>(shared); }
 
 // ---------------------------------------------------------------------------------------------- the first launch
-// h[row][j] = sum_k x[row][k] A[id][j][k] for 128 rows (the MMAs' M, a TMEM lane each) and up to 64 ranks (their N).  Eight warps
-// bring 64 k of x and A at a time; one warp issues the MMAs.  x comes by asynchronous copies some stages ahead: into the MMAs'
-// own tiles where both operands are of one 16-bit type, else into slots of the thread that asked, which cuts it into pieces.
-// (Loads into registers were bound by the few L1 lines that are left beside this much shared memory: 3B ffn, 8192 rows 62 us.)
-// Two stages make a sum: its additions (rank 64, fp32 x, bf16 A: 24) are cut off by the tensor cores, so the eight warps add it
-// up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
-constexpr int kShrinkTileWorkers = 256, kShrinkTileThreads = kShrinkTileWorkers + 32, kShrinkTileRanks = 64;
+// h[row][j] = sum_k x[row][k] A[id][j][k] for 128 rows (the MMAs' M, a TMEM lane each) and up to 64 ranks (their N).  Eight
+// warps, or sixteen where they cut pieces (3B ffn, 8192 rows of fp32 50 us with eight, 47 with sixteen; 3B value, 1402 rows of
+// fp16 14 and 15), bring 64 k of x and A at a time; one warp issues the MMAs.  x comes by asynchronous copies some stages ahead:
+// into the MMAs' own tiles where both operands are of one 16-bit type, else into slots of the thread that asked, which cuts it
+// into pieces.  (Loads into registers were bound by the few L1 lines that are left beside this much shared memory: 3B ffn, 8192
+// rows 62 us.)  Two stages make a sum: its additions (rank 64, fp32 x, bf16 A: 24) are cut off by the tensor cores, so those
+// warps add it up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
+// What bounds it: with pieces, shared memory (a stage's 32 KB of x pass it five times), 3.4 TB/s from memory.
+constexpr int kShrinkTileRanks = 64;
 
 template <typename TX, typename TW>
 struct ShrinkTile {
   static constexpr bool kSame = std::is_same<TX, TW>::value && sizeof(TX) == 2;
   static constexpr int PX = kSame ? 1 : AdaptType<TX>::kPieces, PW = kSame ? 1 : AdaptType<TW>::kPieces;
+  static constexpr int kWorkers = kSame ? 256 : 512, kThreads = kWorkers + 32;
+  static constexpr int kSums = kShrinkTileRanks / (kWorkers / 128);        // ranks whose sums a thread has, of one row
+  static_assert(kSums % 16 == 0, "");
   static constexpr int kBytesX = PX * kTileBytes, kStage = kBytesX + PW * kTileBytes / 2;
   static constexpr int kStages = kSame ? 8 : 2, kRaw = kSame ? 0 : 64 * kAdaptTile * int(sizeof(TX)), kFit = kSame ? 0 : (226 * 1024 - 1024 - 2 * kStage) / kRaw;
   static constexpr int kRing = kFit > 4 ? 4 : kFit;        // stages of x as it comes
   static constexpr int kPitch = kShrinkTileRanks + 1, kTable = kAdaptTile * kPitch * 4;
   static constexpr int kSmem = 1024 + (kStages * kStage + kRing * kRaw > kTable ? kStages * kStage + kRing * kRaw : kTable);
   // loads of a thread: 16 bytes each
-  static constexpr int kUnitX = 16 / int(sizeof(TX)), kRowX = 64 / kUnitX, kHopX = kShrinkTileWorkers / kRowX, kLoadX = kAdaptTile / kHopX;
-  static constexpr int kUnitW = 16 / int(sizeof(TW)), kRowW = 64 / kUnitW, kHopW = kShrinkTileWorkers / kRowW, kLoadW = kShrinkTileRanks / kHopW;
+  static constexpr int kUnitX = 16 / int(sizeof(TX)), kRowX = 64 / kUnitX, kHopX = kWorkers / kRowX, kLoadX = kAdaptTile / kHopX;
+  static constexpr int kUnitW = 16 / int(sizeof(TW)), kRowW = 64 / kUnitW, kHopW = kWorkers / kRowW, kLoadW = kShrinkTileRanks / kHopW;
 };
 
 // One 16-byte load of T as P pieces into tiles `hop` bytes apart: eight elements are a unit, four (fp32) half of one.
@@ -94,7 +99,7 @@ __device__ __forceinline__ void tile_put(char* tile, int hop, int row, int load,
 }
 
 template <typename TX, typename TW>
-__global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kernel(const AdaptParams P) {
+__global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_tile_kernel(const AdaptParams P) {
   using S = ShrinkTile<TX, TW>;
   extern __shared__ __align__(1024) char shared[];
   TileControl& C = *tile_control(shared);
@@ -110,22 +115,23 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
   const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty);
   volatile int* abort_flag = &C.abort;
   if (tid == 0) {
-    for (int i = 0; i < S::kStages; ++i) { mbar_init(full + 8 * i, kShrinkTileWorkers); mbar_init(empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kShrinkTileWorkers / 32); }
+    for (int i = 0; i < S::kStages; ++i) { mbar_init(full + 8 * i, S::kWorkers); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, S::kWorkers / 32); }
     C.abort = 0;
     fence_mbar_init();
   }
-  if (warp == kShrinkTileWorkers / 32) tmem_alloc_cols<128>(smem_u32(&C.tmem));
+  if (warp == S::kWorkers / 32) tmem_alloc_cols<128>(smem_u32(&C.tmem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
   griddep_launch_dependents();                             // only now: the second launch takes tensor memory too
-  float sum[32];
+  constexpr int kSums = S::kSums;
+  float sum[kSums];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) sum[i] = 0.f;
-  const int q = warp & 3, half = warp >> 2;                // workers: TMEM lanes 32 q .., ranks 32 half ..
-  if (warp < kShrinkTileWorkers / 32) {
+  for (int i = 0; i < kSums; ++i) sum[i] = 0.f;
+  const int q = warp & 3, r0 = (warp >> 2) * kSums;        // workers: TMEM lanes 32 q .., ranks r0 ..
+  if (warp < S::kWorkers / 32) {
     const TX* x = static_cast<const TX*>(P.x[mat]) + size_t(row0) * K;
     const TW* a = static_cast<const TW*>(P.a[mat]) + (size_t(asked) * rank + j0) * K;
     const int ux = tid % S::kRowX, rx = tid / S::kRowX, uw = tid % S::kRowW, rw = tid / S::kRowW;
@@ -149,7 +155,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
         for (int i = 0; i < S::kLoadX; ++i) {
           const int r = rx + i * S::kHopX;
           const bool in = r < count && k < K;
-          cp_async16(smem_u32(S::kSame ? to + tile_unit(r, ux) : raw + slot * S::kRaw + i * kShrinkTileWorkers * 16), in ? x + size_t(r) * K + k : x, in);
+          cp_async16(smem_u32(S::kSame ? to + tile_unit(r, ux) : raw + slot * S::kRaw + i * S::kWorkers * 16), in ? x + size_t(r) * K + k : x, in);
         }
         if constexpr (S::kSame) {
           const int kw = c * 64 + uw * S::kUnitW;
@@ -168,18 +174,14 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
       ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * (g & 1), uint32_t(g >> 1) & 1u, abort_flag));
       if (!ok) return;
       tc_fence_after();
-      if (half * 32 < n16) {
-        float v[2][16];
-        const uint32_t at = tmem + (uint32_t(q * 32) << 16) + uint32_t((g & 1) * 64 + half * 32);
-        tmem_ld16(at, v[0]);
-        if (half * 32 + 16 < n16) tmem_ld16(at + 16, v[1]);
-        tmem_ld_wait();
+      float v[kSums / 16][16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i] += v[0][i];
-        if (half * 32 + 16 < n16)
+      for (int i = 0; i < kSums / 16; ++i)
+        if (r0 + 16 * i < n16) tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t((g & 1) * 64 + r0 + 16 * i), v[i]);
+      tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum[16 + i] += v[1][i];
-      }
+      for (int i = 0; i < kSums; ++i)
+        if (r0 + (i & ~15) < n16) sum[i] += v[i >> 4][i & 15];
       tc_fence_before();
       if (lane == 0) mbar_arrive(acc_empty + 8 * (g & 1));
     };
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
         char* to = stages + slot * S::kStage;
 #pragma unroll
         for (int i = 0; i < S::kLoadX; ++i)
-          tile_put<TX, S::PX>(to, kTileBytes, rx + i * S::kHopX, ux, *reinterpret_cast<const uint4*>(raw + ask * S::kRaw + i * kShrinkTileWorkers * 16));
+          tile_put<TX, S::PX>(to, kTileBytes, rx + i * S::kHopX, ux, *reinterpret_cast<const uint4*>(raw + ask * S::kRaw + i * S::kWorkers * 16));
 #pragma unroll
         for (int i = 0; i < S::kLoadW; ++i) tile_put<TW, S::PW>(to + S::kBytesX, kTileBytes / 2, rw + i * S::kHopW, uw, vw[i]);
         if (c + 1 < c1) load_w(c + 1);
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
     cp_async_wait<0>();
     if (!ok)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sum[i] = NAN;
+      for (int i = 0; i < kSums; ++i) sum[i] = NAN;
   } else {
     const uint32_t idesc = umma_idesc_f16(kAdaptTile, n16, !(S::kSame && std::is_same<TX, __half>::value));
     const uint32_t base = smem_u32(stages);
@@ -259,10 +261,10 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
   }
   // every MMA is over (the workers saw the last sum) and no copy on its way: the stages become the table of sums
   float* table = reinterpret_cast<float*>(stages);
-  if (warp < kShrinkTileWorkers / 32) {
-    float* mine = table + (q * 32 + lane) * S::kPitch + half * 32;
+  if (warp < S::kWorkers / 32) {
+    float* mine = table + (q * 32 + lane) * S::kPitch + r0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) mine[i] = sum[i];
+    for (int i = 0; i < kSums; ++i) mine[i] = sum[i];
   }
   tc_fence_before();
   float* h = P.h[mat] + size_t(row0) * rank + j0;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(kShrinkTileThreads, 1) adapt_shrink_tile_kerne
                 const int r = i / kShrinkTileRanks, j = i % kShrinkTileRanks;
                 if (j < ranks) h[size_t(r) * rank + j] = v;
               });
-  if (warp == kShrinkTileWorkers / 32) {
+  if (warp == S::kWorkers / 32) {
     tc_fence_after();
     tmem_free_cols<128>(tmem);
   }

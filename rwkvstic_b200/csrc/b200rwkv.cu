@@ -767,7 +767,7 @@ static cudaError_t launch_adapt_shrink(const AdaptParams& P, const AdaptShape& s
     const cudaError_t e = allow_smem(adapt_shrink_tile_kernel<TX, TW>, smem, configured);
     if (e != cudaSuccess) return e;
     return launch_clustered(P.splits, adapt_shrink_tile_kernel<TX, TW>, dim3(sh.n1 * P.splits, (P.rank + kShrinkTileRanks - 1) / kShrinkTileRanks, P.nmat),
-                            dim3(kShrinkTileThreads), smem, stream, P);
+                            dim3(ShrinkTile<TX, TW>::kThreads), smem, stream, P);
   }
   if (sh.mt == 1) return launch_adapt_shrink_as<TX, TW, 1>(P, sh, stream);
   if (sh.mt == 2) return launch_adapt_shrink_as<TX, TW, 2>(P, sh, stream);
