@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   R.Ps = S.p_sum[n]; R.Qs = kind == VERIFY_LEFT ? S.q_sum[n] : 1.0; R.V = V;
   const long long d = kind == VERIFY_OTHERS ? __ldg(tokens + n) : -1;
   R.refused = d >= 0 && d < V ? int(d) : -1;
-  VerifyShared* S0 = cluster.map_shared_rank(&S, 0);
   cluster.barrier_wait(std::move(started));                        // all CTAs run, so their shared memory exists, and S.any is set
+  VerifyShared* S0 = cluster.map_shared_rank(&S, 0);
   for (;;) {                                                       // a second time where the first distribution is empty
     for (int s = rank * kVerifyWarps + warp; s < segs; s += C * kVerifyWarps) {
       const double v = kind == VERIFY_TARGET ? __ldcg(sums + (long long)n * segs + s)     // the first launch has these
