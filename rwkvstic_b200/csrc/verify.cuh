@@ -10,8 +10,8 @@
 // to the segment, then the token, that holds the uniform number.  The segments depend on the vocabulary alone, so a stream's
 // result does not depend on the other streams of the call.
 // Bounds: the first launch by memory and by turning weights into fp64, 16 a clock and SM (256 streams, vocabulary 50277, 1150
-// rows looked at, 231 MB: 41 us), the second by instructions and latency (the same 256 streams, no draft distribution: 19 to 23
-// us, part of it beside the first; 1 stream of 4 drafted tokens: 10 us for both).  All in one launch of a cluster per stream
+// rows looked at, 231 MB: 41 us), the second by latency (the same 256 streams, no draft distribution: 12 us, part of it
+// beside the first, 19 where it formed all segments anew; 1 stream of 4 drafted tokens: 9.5 us for both).  All in one launch of a cluster per stream
 // was slower where a stream is alone, 13.9 us against 9.4, since eight CTAs then sum what 50 times more warps do here.
 #pragma once
 
@@ -210,11 +210,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   R.Ps = S.p_sum[n]; R.Qs = kind == VERIFY_LEFT ? S.q_sum[n] : 1.0; R.V = V;
   const long long d = kind == VERIFY_OTHERS ? __ldg(tokens + n) : -1;
   R.refused = d >= 0 && d < V ? int(d) : -1;
+  const int refused_seg = R.refused >= 0 ? R.refused / kVerifySeg : -1;
   cluster.barrier_wait(std::move(started));                        // all CTAs run, so their shared memory exists, and S.any is set
   VerifyShared* S0 = cluster.map_shared_rank(&S, 0);
   for (;;) {                                                       // a second time where the first distribution is empty
     for (int s = rank * kVerifyWarps + warp; s < segs; s += C * kVerifyWarps) {
-      const double v = kind == VERIFY_TARGET ? __ldcg(sums + (long long)n * segs + s)     // the first launch has these
+      // the first launch has the target's own, also where a refused token is elsewhere
+      const double v = kind == VERIFY_TARGET || (kind == VERIFY_OTHERS && s != refused_seg) ? __ldcg(sums + (long long)n * segs + s)
                        : kind == VERIFY_LEFT ? verify_segment_sum<VERIFY_LEFT>(R, s) : verify_segment_sum<VERIFY_OTHERS>(R, s);
       if (lane == 0) {
         S0->seg[s] = v;
