@@ -18,7 +18,7 @@
 // where it has an adapter.
 // What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces: 7B key, value and receptance for
 // 256 streams of 200 adapters (332 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (115 MB)
-// 33; 7B ffn for 64 streams of 48 adapters (56 MB) 27.  Fragments go from global memory to a lane's own slots of shared memory
+// 33; 7B ffn for 64 streams of 48 adapters (56 MB) 23.  Fragments go from global memory to a lane's own slots of shared memory
 // and from there to its registers, without a barrier between warps.  The index along a product is free to permute, and is, so
 // that a lane's elements are consecutive: 16 bytes of A, 8 of B.
 #pragma once

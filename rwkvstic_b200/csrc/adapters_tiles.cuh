@@ -644,9 +644,10 @@ inline int piece_products(int a, int b, int limit) {
 //     about 32M -23, -11, +3 %;  64M -14, -2, +15;  128M -7, +16, +41;  512M +6, +29, +84;  2000M +40, +76, +110
 // Ranks up to 128 and rows that start on 16 bytes for the second (`aligned`; y passes as bulk copies), one CTA per SM.
 // Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
-// Columns of a CTA of the second launch, gathered: what it takes at a time, times what leaves the two CTAs that an SM holds at
-// once, by the number of tiles where streams spread evenly over the adapters (7B ffn for 64 streams of 48 adapters 19, 20, 26 us
-// with two, three, six CTAs per SM; 16384 columns for 200 streams of 6 adapters 48, 58, 58).
+// Columns of a CTA of the second launch, gathered: the number of steps for which the rounds of the two CTAs that an SM holds take
+// the least, a start being worth a step, by the number of tiles where streams spread evenly over the adapters.  Time follows
+// the rounds: 3B head for 48 x 5 rows of 20 adapters, 4 6 7 8 10 12 16 steps (2 2 2 1 1 1 1 rounds) 33.5 37.9 38.1 32.4 34.8 38.4 47
+// us; 7B ffn for 64 streams of 48 adapters, 4 6 8 12 16 steps 24.6 26.6 23.1 26.9 32.
 inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank, int K, int streams, int T, int w_pieces, int row_bytes, bool same16,
                               bool aligned, int sms) {
   AdaptShape s;
@@ -683,10 +684,15 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
   const int unit = kExpandWarps * (w_pieces < 3 ? 64 : 32);
   const long long shared_by = adapters < streams ? adapters : streams, filled = (long long)streams * T / kAdaptRows + shared_by / 2;
   const long long tiles = T >= kAdaptRows ? s.n2 : filled > shared_by ? filled : shared_by;        // about as many as lead rows
-  long long units = 0;
-  for (int i = 0; i < nmat; ++i) units += (n_out[i] + unit - 1) / unit;
-  const long long per = (units * tiles + sms) / (2LL * sms);
-  s.chunk_cols = unit * int(per < 1 ? 1 : per > 64 ? 64 : per);
+  long long least = 0;
+  for (int per = 64; per >= 1; --per) {                  // rounds of two CTAs per SM, times units of a CTA and one for its start
+    long long chunks = 0;
+    for (int i = 0; i < nmat; ++i) chunks += (n_out[i] + per * unit - 1) / (per * unit);
+    const long long cost = (chunks * tiles + 2 * sms - 1) / (2 * sms) * (per + 1);
+    if (least && cost >= least) continue;
+    least = cost;
+    s.chunk_cols = per * unit;
+  }
   for (int i = 0; i < nmat; ++i) s.chunks += (n_out[i] + s.chunk_cols - 1) / s.chunk_cols;
   return s;
 }
