@@ -242,7 +242,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
 
     ``banks[i] = (a [n,rank,k_in], b [n,n_out_i,rank], scale f32 [n] or None)`` of bf16, fp16 or fp32 (see
     ``pack_adapters``), ``xs[i] [rows,k_in]`` and ``ys[i] [rows,n_out_i]`` of fp32 or the banks' type, ``ids`` int64
-    ``[streams]``; all contiguous on one CUDA device.  In place on ``ys`` when ``outs`` is omitted.  ``h = x A^T`` stays
+    ``[streams]``; all contiguous on one CUDA device.  Rank a multiple of 4 up to 256, k_in of 8, up to 65535 rows.  In
+    place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T`` stays
     fp32 and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
     adapter; rows without one are left as they are."""
     n = len(banks)
@@ -294,7 +295,7 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     tokens = rows // streams
     nbytes = _adapt_workspace(tuple(n_out), count, rank, k_in, code, streams, tokens)
     with _on(index):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=a0.device)
+        ws = ids.new_empty(nbytes // 8)
         _lib.check(_lib.lib().b200rwkv_adapt_rows(n, at, count, rank, k_in, code, at + 32 * n, at + 40 * n, at + 48 * n, _DENSE_DTYPES[row_dt],
                                                   ids.data_ptr(), streams, tokens, ws.data_ptr(), nbytes, _raw_stream(index)))
     return list(outs)
@@ -340,16 +341,17 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         raise ValueError(f"u must be contiguous fp32 [{B},{K + 1}] on the target's device")
     if lengths is not None and (lengths.dtype != torch.int64 or lengths.get_device() != index or lengths.shape != (B,) or not lengths.is_contiguous()):
         raise ValueError(f"lengths must be contiguous int64 [{B}] on the target's device")
-    device = target.device
-    out = torch.empty((B, K + 1), dtype=torch.int64, device=device)
-    accepted = torch.empty(B, dtype=torch.int64, device=device)
+    # (sizes one by one, and new_empty, parse faster than a tuple with a type and a device)
+    out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)
+    accepted = tokens.new_empty(B)
     if B == 0:
         return out, accepted
     with _on(index):
-        ws = torch.empty(_verify_workspace(B, K, V), dtype=torch.uint8, device=device)
+        nbytes = _verify_workspace(B, K, V)
+        ws = tokens.new_empty(nbytes // 8)
         _lib.check(_lib.lib().b200rwkv_verify_drafts(target.data_ptr(), t_stream, t_row, d_ptr, d_stream, d_row, tokens.data_ptr(),
                                                      u.data_ptr(), None if lengths is None else lengths.data_ptr(), B, K, V, out.data_ptr(),
-                                                     accepted.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(index)))
+                                                     accepted.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(index)))
     return out, accepted
 
 

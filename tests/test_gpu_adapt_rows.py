@@ -73,6 +73,7 @@ SHAPES = [
     (40, 1, 264, [130], 20, 1),              # one adapter for more rows than a tile
     (150, 1, 136, [64], 12, 40),
     (1100, 1, 64, [36], 8, 3),               # more streams than a window
+    (1300, 3, 64, [36], 8, 5),               # the same with tiles that begin and end inside a stream
     (48, 5, 256, [1029], 8, 20),             # tiles that begin and end inside a stream
     (33, 31, 72, [65, 1], 4, 2),
     (3, 33, 128, [100], 36, 2),
