@@ -80,7 +80,7 @@ __device__ __forceinline__ void mma_to(bool first, float (&d)[4], const uint32_t
   }
 }
 
-// Elements 2i and 2i + 1 of a lane's, as loaded (16-bit types) or as floats.
+// bfloat16 pieces that hold a value exactly.
 template <typename T>
 struct AdaptType;
 template <> struct AdaptType<__nv_bfloat16> { static constexpr int kPieces = 1; };
@@ -100,26 +100,11 @@ __device__ __forceinline__ void split_pair(float lo, float hi, uint32_t (&p)[P])
   for (int i = 0; i < P; ++i) p[i] = take_piece(lo, hi);
 }
 
-// N consecutive elements of T (N * sizeof(T) a multiple of 8), zero where !ok.
+// N consecutive elements of T, held as loaded.
 template <typename T, int N>
 struct AdaptRaw {
   static constexpr int kWords = N * int(sizeof(T)) / 4;
   uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* p, bool ok) {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = 0u;
-    if (!ok) return;
-    if constexpr (kWords % 4 == 0) {
-#pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-      }
-    } else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-      w[0] = v.x; w[1] = v.y;
-    }
-  }
   // pieces of the pair of elements 2i, 2i + 1
   template <int P>
   __device__ __forceinline__ void pair(int i, uint32_t (&p)[P]) const {
@@ -182,11 +167,7 @@ __device__ __forceinline__ int adapt_tile(const AdaptParams& P, int tile, int* r
   return n;
 }
 
-// h[row][j] = sum_k x[row][k] A[id][j][k].  Grid (tiles * splits of K, rank chunks of 16 * MT, matrices); the CTAs of a tile's
-// splits are a cluster, whose sums meet in shared memory, in the order of the splits.
-// For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter.  A warp takes every eighth
-// block of 32 k of the split; a lane copies its own 16-byte fragments of A and x into slots of its own, several blocks ahead, so
-// that nothing but the end of the sums needs the other warps.
+// The splits of a tile are a cluster, whose sums meet in shared memory, in the order of the splits:
 // put(i, sum over the cluster's CTAs of part_sums[place(i)]) for i < n
 template <typename Place, typename Put>
 __device__ __forceinline__ void shrink_join(const AdaptParams& P, float* part_sums, int n, Place place, Put put) {
@@ -355,6 +336,10 @@ __device__ __forceinline__ float* shrink_sums(const AdaptParams& P, const TX* x,
   return part_sums;
 }
 
+// h[row][j] = sum_k x[row][k] A[id][j][k].  Grid (tiles * splits of K, rank chunks of 16 * MT, matrices).
+// For tiles of 16 rows (as columns of the products, 8 at a time), which read little but their adapter.  A warp takes every eighth
+// block of 32 k of the split; a lane copies its own 16-byte fragments of A and x into slots of its own, several blocks ahead, so
+// that nothing but the end of the sums needs the other warps.
 template <typename TX, typename TW, int MT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) adapt_shrink_kernel(const AdaptParams P) {
   extern __shared__ __align__(16) char shared[];
@@ -393,7 +378,8 @@ __device__ __forceinline__ void adapt_store(TY* p, float v) {
 // W consecutive elements of a row (1, 2 or 4), held as loaded.
 template <typename TY, int W>
 struct AdaptFew {
-  using Word = std::conditional_t<W * sizeof(TY) == 16, uint4, std::conditional_t<W * sizeof(TY) == 8, uint2, std::conditional_t<W * sizeof(TY) == 4, uint32_t, unsigned short>>>;
+  static constexpr int kBytes = W * int(sizeof(TY));
+  using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, uint32_t, unsigned short>>>;
   Word w;
   __device__ __forceinline__ void load(const TY* p) { w = *reinterpret_cast<const Word*>(p); }
   __device__ __forceinline__ void store(TY* p) const { *reinterpret_cast<Word*>(p) = w; }
@@ -407,7 +393,8 @@ struct AdaptFew {
     } else {
       const float4 d = *reinterpret_cast<const float4*>(f);
       if constexpr (sizeof(TY) == 4)
-        *reinterpret_cast<float4*>(p) = make_float4(__uint_as_float(w.x) + d.x, __uint_as_float(w.y) + d.y, __uint_as_float(w.z) + d.z, __uint_as_float(w.w) + d.w);
+        *reinterpret_cast<float4*>(p) = make_float4(__uint_as_float(w.x) + d.x, __uint_as_float(w.y) + d.y, __uint_as_float(w.z) + d.z,
+                                                    __uint_as_float(w.w) + d.w);
       else
         *reinterpret_cast<uint2*>(p) = make_uint2(add_pair(w.x, d.x, d.y), add_pair(w.y, d.z, d.w));
     }
@@ -716,7 +703,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) adapt_fused_kernel(const Ad
   const T* x = static_cast<const T*>(P.x[mat]);
   const TW* a = static_cast<const TW*>(P.a[mat]) + size_t(id) * rank * P.K;
   auto stage_h = [&] {
-    float* sums = count <= 8 ? shrink_sums<T, TW, MT, 1>(P, x, a, part, 0, rows, count, work) : shrink_sums<T, TW, MT, 2>(P, x, a, part, 0, rows, count, work);
+    float* sums = count <= 8 ? shrink_sums<T, TW, MT, 1>(P, x, a, part, 0, rows, count, work)
+                             : shrink_sums<T, TW, MT, 2>(P, x, a, part, 0, rows, count, work);
     cluster.sync();
     const float scale = P.scale[mat] ? __ldg(P.scale[mat] + id) : 1.f;
     const int r4 = ksteps * 4, padded = (count + 7) / 8 * 8;         // groups of four ranks; rows

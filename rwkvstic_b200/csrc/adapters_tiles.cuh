@@ -44,7 +44,6 @@ struct TileControl {
   int abort;
   uint32_t tmem;
 };
-__device__ __forceinline__ TileControl* tile_control(char* shared) { return reinterpret_cast<TileControl*>(shared); }
 
 // ---------------------------------------------------------------------------------------------- the first launch
 // h[row][j] = sum_k x[row][k] A[id][j][k] for 128 rows (the MMAs' M, a TMEM lane each) and up to 64 ranks (their N).  Eight
@@ -65,7 +64,8 @@ struct ShrinkTile {
   static constexpr int kSums = kShrinkTileRanks / (kWorkers / 128);        // ranks whose sums a thread has, of one row
   static_assert(kSums % 16 == 0, "");
   static constexpr int kBytesX = PX * kTileBytes, kStage = kBytesX + PW * kTileBytes / 2;
-  static constexpr int kStages = kSame ? 8 : 2, kRaw = kSame ? 0 : 64 * kAdaptTile * int(sizeof(TX)), kFit = kSame ? 0 : (226 * 1024 - 1024 - 2 * kStage) / kRaw;
+  static constexpr int kStages = kSame ? 8 : 2, kRaw = kSame ? 0 : 64 * kAdaptTile * int(sizeof(TX));
+  static constexpr int kFit = kSame ? 0 : (226 * 1024 - 1024 - 2 * kStage) / kRaw;
   static constexpr int kRing = kFit > 4 ? 4 : kFit;        // stages of x as it comes
   static constexpr int kPitch = kShrinkTileRanks + 1, kTable = kAdaptTile * kPitch * 4;
   static constexpr int kSmem = 1024 + (kStages * kStage + kRing * kRaw > kTable ? kStages * kStage + kRing * kRaw : kTable);
@@ -102,7 +102,7 @@ template <typename TX, typename TW>
 __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_tile_kernel(const AdaptParams P) {
   using S = ShrinkTile<TX, TW>;
   extern __shared__ __align__(1024) char shared[];
-  TileControl& C = *tile_control(shared);
+  TileControl& C = *reinterpret_cast<TileControl*>(shared);
   char* stages = shared + 1024;
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
   const int tile = blockIdx.x / P.splits, split = blockIdx.x - tile * P.splits, mat = blockIdx.z;
@@ -376,16 +376,18 @@ __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.w
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 template <typename TY, typename TW>
-__global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kernel(const __grid_constant__ AdaptParams P, const __grid_constant__ AdaptMaps M) {
+__global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kernel(const __grid_constant__ AdaptParams P,
+                                                                                const __grid_constant__ AdaptMaps M) {
   using E = ExpandTile<TY, TW>;
   constexpr int PH = E::PH, PW = E::PW;
   extern __shared__ __align__(1024) char shared[];
   ExpandTileControl& C = *reinterpret_cast<ExpandTileControl*>(shared);
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-  const int rank = P.rank, ksteps = (rank + 15) / 16, halves = (rank + 63) / 64, NS = P.stages, NR = P.ring, h_piece = halves * kTileBytes, stage_bytes = PW * h_piece;
+  const int rank = P.rank, ksteps = (rank + 15) / 16, halves = (rank + 63) / 64, NS = P.stages, NR = P.ring;
+  const int h_piece = halves * kTileBytes, stage_bytes = PW * h_piece;
   char *ring = shared + 1024, *h_tiles = ring + NR * E::kHalfBytes, *stages = h_tiles + PH * h_piece;
-  const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty), h_full = smem_u32(&C.h_full);
-  const uint32_t y_full = smem_u32(C.y_full), y_empty = smem_u32(C.y_empty);
+  const uint32_t full = smem_u32(C.full), empty = smem_u32(C.empty), acc_full = smem_u32(C.acc_full), acc_empty = smem_u32(C.acc_empty);
+  const uint32_t h_full = smem_u32(&C.h_full), y_full = smem_u32(C.y_full), y_empty = smem_u32(C.y_empty);
   volatile int* abort_flag = &C.abort;
   constexpr int kAddWarps = kExpandTileAdders / 32, kAdd0 = kExpandTileLoaders / 32, kMmaWarp = kAdd0 + kAddWarps;
   if (tid == 0) {
