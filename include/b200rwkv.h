@@ -366,8 +366,9 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
  *   ids       device int64 [streams], read on the device (a captured call follows them)
  *   workspace b200rwkv_adapt_rows_workspace_bytes(...) (0: a size that is not taken), 256-byte aligned; nothing
  *             is kept in it between calls
- * Sums are f32 over exact products of 16-bit pieces, h = x A^T stays f32, and out is rounded once.  Sums go over fixed parts
- * in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row
+ * Sums are f32 and out is rounded once.  Operands of one 16-bit type are multiplied as they are; others, and h = x A^T, which is
+ * f32 whatever the types, in bf16 pieces that hold them exactly (f32 three, f16 two), without the products of pieces that are below
+ * 2^-21 of the whole product together.  Sums go over fixed parts in a fixed order: a call repeats its bits, and in calls of one shape a row's do not depend on the other rows and ids.  A row
  * of x that holds an infinity or a NaN comes out as NaN where it has an adapter.  One or two launches on `stream`, no
  * allocation, capturable; device-side waits are bounded (1 s), and rows whose wait runs out come out as NaN.  Outputs that
  * overlap more than their own y are refused.  No counterpart in the reference.

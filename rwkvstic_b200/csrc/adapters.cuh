@@ -443,14 +443,16 @@ struct ExpandRing {
   static constexpr int kStage = MT * 2 * 32 * kLane, kPitch = kCols + 4, kTurn = 16 * kPitch * 4;
   static constexpr int kStages = KC == 16 ? 3 : sizeof(TW) == 2 ? 2 : 3, kWarp = kStages * kStage + kTurn;
 };
-template <typename TY>
-__host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * ((rank + kc - 1) / kc * (kc / 16)) * (sizeof(TY) == 2 ? 2 : 3) * 256; }
+// h has all its 24 bits whatever the rows' type: two pieces (16 bits, cut) beside rows of 16 bits put 2.8 % of fp16 and 0.3 % of bf16
+// results on a neighbouring value, and saved 2 us of 68 (7B key, value and receptance, 256 streams).
+constexpr int kPiecesH = 3;
+__host__ __device__ constexpr int expand_h_bytes(int rank, int kc) { return 2 * ((rank + kc - 1) / kc * (kc / 16)) * kPiecesH * 256; }
 
 // Four ranks of a row of h into their fragments: 16 step + 4 t .. + 3 of a step and lane, or with 32 ranks a stage
 // 32 (step / 2) + 8 t + 4 (step % 2) .. + 3.
-template <typename TY, int KC>
+template <int KC>
 __device__ __forceinline__ void expand_put_h(char* shared, int ksteps, int r, int j4, float4 s) {
-  constexpr int PH = sizeof(TY) == 2 ? 2 : 3;
+  constexpr int PH = kPiecesH;
   uint32_t lo[PH], hi[PH];
   split_pair<PH>(s.x, s.y, lo);
   split_pair<PH>(s.z, s.w, hi);
@@ -465,7 +467,7 @@ template <typename TY, typename TW, int KC, bool VEC, int NT, typename StageH>
 __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b, const TY* y, TY* out, int c0, int c_end, const size_t* row_at,
                                                int count, const char* shared, char* slots, StageH stage_h) {
   using Ring = ExpandRing<TY, TW, KC>;
-  constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  constexpr int PH = kPiecesH, PW = AdaptType<TW>::kPieces;
   constexpr int MT = Ring::MT, COLS = Ring::kCols, kStages = Ring::kStages, kStep = kExpandWarps * COLS;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);
@@ -618,8 +620,8 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
 // out[row][c] = y[row][c] + scale * sum_j h[row][j] B[id][c][j].  Grid (tiles of up to 16 rows, column chunks of all matrices).
 // Columns are the rows of the products and rows, 8 at a time, their columns, so that a tile of one row, the common one of a
 // decoding step, wastes little.  A lane's fragments of B come by asynchronous copies into slots of its own, some stages ahead;
-// sums are turned in the warp's table and leave in lines of a row.  h is scaled, and the sum with y rounded once to TY; two
-// pieces of h carry 16 bits, enough for a 16-bit y.  VEC: all rows of y and out start on boundaries of four elements.
+// sums are turned in the warp's table and leave in lines of a row.  h is scaled, and the sum with y rounded once to TY.
+// VEC: all rows of y and out start on boundaries of four elements.
 template <typename TY, typename TW, int KC, bool VEC>
 __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const AdaptParams P) {
   using Ring = ExpandRing<TY, TW, KC>;
@@ -652,12 +654,12 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
       const int r = i / r4, j4 = i - r * r4, j = j4 * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < count && j < rank) s = __ldcg(reinterpret_cast<const float4*>(P.h[mat] + size_t(rows[r]) * rank + j));
-      expand_put_h<TY, KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
+      expand_put_h<KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
     }
     __syncthreads();
   };
   const TW* b = static_cast<const TW*>(P.b[mat]) + size_t(id) * N * rank;
-  char* slots = shared + expand_h_bytes<TY>(rank, KC) + warp * Ring::kWarp;
+  char* slots = shared + expand_h_bytes(rank, KC) + warp * Ring::kWarp;
   const int c0 = c_begin + warp * Ring::kCols;
   if (count <= 8) expand_columns<TY, TW, KC, VEC, 1>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
   else expand_columns<TY, TW, KC, VEC, 2>(P, b, y, out, c0, c_end, row_at, count, shared, slots, stage_h);
@@ -670,7 +672,7 @@ static_assert(kFusedCtas <= kAdaptMaxSplits, "");
 
 template <typename T, typename TW, int MT>
 struct FusedShape {
-  static constexpr int KC = MT == 1 ? 16 : 32, kH = expand_h_bytes<T>(16 * MT, KC), kRing = kExpandWarps * ExpandRing<T, TW, KC>::kWarp;
+  static constexpr int KC = MT == 1 ? 16 : 32, kH = expand_h_bytes(16 * MT, KC), kRing = kExpandWarps * ExpandRing<T, TW, KC>::kWarp;
   static constexpr int kSmem = kH + kRing + ShrinkRing<T, TW, MT>::kSmem;
   static_assert(kSmem <= 226 * 1024, "");
 };
@@ -719,7 +721,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) adapt_fused_kernel(const Ad
 #pragma unroll
         for (int c = 1; c < kFusedCtas; ++c) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
       }
-      expand_put_h<T, KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
+      expand_put_h<KC>(shared, ksteps, r, j4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale));
     }
     cluster.sync();                                        // the tables are read before their CTAs go on or leave
   };

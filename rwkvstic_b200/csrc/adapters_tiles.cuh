@@ -303,7 +303,7 @@ struct ExpandTileControl {
 
 template <typename TY, typename TW>
 struct ExpandTile {
-  static constexpr int PH = sizeof(TY) == 2 ? 2 : 3, PW = AdaptType<TW>::kPieces;
+  static constexpr int PH = kPiecesH, PW = AdaptType<TW>::kPieces;
   static constexpr int kRow = kAdaptTile * int(sizeof(TY)), kHalfBytes = kExpandHalf * kRow;
   // for `halves` times 64 ranks: half steps of y (2 to 4) that leave room for a stage of B beside h, 0 where none do; then stages
   // of B, at most 4
@@ -644,6 +644,8 @@ inline int piece_products(int a, int b, int limit) {
 //     about 8M -29, -16, -4 %;  16M -18, -8, +22;  32M -7, +4, +25;  64M 0, +16, +108;  256M and more +14, +106, +148
 //   second launch, by products of 16 ranks x rows x N x bytes of y
 //     about 32M -23, -11, +3 %;  64M -14, -2, +15;  128M -7, +16, +41;  512M +6, +29, +84;  2000M +40, +76, +110
+//     (rows of 16 bits: without the third piece of h, which costs gathered tiles less than a product: 10240 -> 2560 for 2 x 701 rows,
+//     fp16, rank 32, 43M so and 72M with it: 22.6 us, 24.8 as tiles; bf16, rank 64, 57M and 86M: 27.1 and 25.5)
 // Ranks up to 128 and rows that start on 16 bytes for the second (`aligned`; y passes as bulk copies), one CTA per SM.
 // Splits of K: a power of two that leaves the launch one wave (of one CTA per SM for tiles, else of two), 256 or more k each.
 // Columns of a CTA of the second launch, gathered: the number of steps for which the rounds of the two CTAs that an SM holds take

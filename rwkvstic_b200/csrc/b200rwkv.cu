@@ -779,10 +779,10 @@ template <typename TY, typename TW, int KC, bool VEC>
 static cudaError_t launch_adapt_expand_as(const AdaptParams& P, const AdaptShape& sh, cudaStream_t stream) {
   constexpr int warps = kExpandWarps * ExpandRing<TY, TW, KC>::kWarp;
   static bool configured[64];
-  const cudaError_t e = allow_smem(adapt_expand_kernel<TY, TW, KC, VEC>, warps + expand_h_bytes<TY>(kAdaptMaxRank, KC), configured);
+  const cudaError_t e = allow_smem(adapt_expand_kernel<TY, TW, KC, VEC>, warps + expand_h_bytes(kAdaptMaxRank, KC), configured);
   if (e != cudaSuccess) return e;
   return launch_chained(adapt_expand_kernel<TY, TW, KC, VEC>, dim3(sh.n2, sh.chunks), dim3(kExpandThreads),
-                        size_t(warps) + expand_h_bytes<TY>(P.rank, KC), stream, P);
+                        size_t(warps) + expand_h_bytes(P.rank, KC), stream, P);
 }
 
 // [rows][n] elements of `size` bytes, boxes of kExpandBox rows x kAdaptTile columns; n * size a multiple of 16.

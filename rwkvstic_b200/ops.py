@@ -243,8 +243,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     ``banks[i] = (a [n,rank,k_in], b [n,n_out_i,rank], scale f32 [n] or None)`` of bf16, fp16 or fp32 (see
     ``pack_adapters``), ``xs[i] [rows,k_in]`` and ``ys[i] [rows,n_out_i]`` of fp32 or the banks' type, ``ids`` int64
     ``[streams]``; all contiguous on one CUDA device.  Rank a multiple of 4 up to 256, k_in of 8, up to 65535 rows.  In
-    place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T`` stays
-    fp32 and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
+    place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T`` is
+    fp32 whatever the types, products leave out less than 2^-21 of themselves, and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
     adapter; rows without one are left as they are."""
     n = len(banks)
     outs = ys if outs is None else outs

@@ -285,3 +285,32 @@ def test_refusals():
     empty = torch.zeros(0, 64, device=DEV)
     assert ops.adapt_rows(banks, [empty], ids, [torch.zeros(0, 32, device=DEV)])[0].shape == (0, 32)
     assert ops.adapt_rows(banks, [empty], ids[:0], [torch.zeros(0, 32, device=DEV)])[0].shape == (0, 32)
+
+
+# (streams, rows of a stream, k, outputs, rank) that take each form
+FORMS = {"one launch": (3, 1, 64, 64, 8), "gathered": (70, 2, 64, 264, 16), "gathered, 32 ranks a stage": (70, 2, 64, 264, 100),
+         "tiles": (2, 701, 4288, 4096, 64), "tiles, second launch of two times 64 ranks": (1, 300, 64, 8192, 128)}
+
+
+@pytest.mark.parametrize("w", ["bf16", "f16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_h_keeps_24_bits_beside_rows_of_16(form, w):
+    """Pairs of 2^20 + a and -2^20 + b, which cancel in the second product: every number on the way is a whole one below 2^24
+    and the result below 2^8, so it is exact.  (h in 16 bits would lose all of a and b.)"""
+    streams, T, k, n_out, rank = FORMS[form]
+    g = torch.Generator().manual_seed(rank)
+    whole = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g).double()
+    a, b = torch.zeros(2, rank, k, dtype=torch.float64), torch.zeros(2, n_out, rank // 2, 2, dtype=torch.float64)
+    a[:, 0::2, 0], a[:, 1::2, 0], a[:, :, k - 1] = 512.0, -512.0, whole(-7, 7, 2, rank)
+    b.scatter_(2, torch.rand(2, n_out, rank // 2, generator=g).topk(4).indices.unsqueeze(-1).expand(-1, -1, -1, 2), 1.0)     # four pairs a column
+    b = b.reshape(2, n_out, rank) * (2 * whole(0, 1, 2, n_out, 1) - 1)
+    x, y = torch.zeros(streams * T, k, dtype=torch.float64), whole(-60, 60, streams * T, n_out)
+    x[:, 0], x[:, k - 1] = 2048.0, whole(1, 3, streams * T)
+    ids = torch.arange(streams) % 2
+    want = y.clone()
+    for i, j in enumerate(ids.tolist()):
+        want[i * T:(i + 1) * T] += x[i * T:(i + 1) * T] @ a[j].T @ b[j].T
+    assert float(want.abs().max()) <= 256
+    d = lambda v: v.to(TYPES[w]).to(DEV)
+    got = ops.adapt_rows([(d(a), d(b), None)], [d(x)], ids.to(DEV), [d(y)])[0]
+    assert torch.equal(got.double().cpu(), want)
