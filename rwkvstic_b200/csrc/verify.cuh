@@ -121,7 +121,8 @@ template <int KIND>
 __device__ __forceinline__ double verify_value(float p, float q, const VerifyRow& R) {
   const double pd = verify_weight(p);
   if (KIND != VERIFY_LEFT) return pd;
-  const double v = pd * R.Qs - verify_weight(q) * R.Ps;
+  // each product rounded: as one fused operation equal rows would leave the rounding errors of one of them
+  const double v = __dsub_rn(__dmul_rn(pd, R.Qs), __dmul_rn(verify_weight(q), R.Ps));
   const int hi = __double2hiint(v), keep = ~(hi >> 31);    // zero where negative
   return __hiloint2double(hi & keep, __double2loint(v) & keep);
 }

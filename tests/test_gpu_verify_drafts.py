@@ -187,3 +187,18 @@ def test_refusals():
         ops.verify_drafts(torch.zeros(1, 66, 4, device=DEV), None, torch.zeros(1, 65, dtype=torch.int64, device=DEV), torch.zeros(1, 66, device=DEV))
     out, accepted = ops.verify_drafts(target[:0], draft[:0], tokens[:0], u[:0])
     assert out.shape == (0, 3) and accepted.shape == (0,)
+
+
+@pytest.mark.parametrize("V", [50, 1025, 50277])
+def test_nothing_is_left_where_the_draft_equals_the_target(V):
+    """Weights alike bit for bit: p Q - q P is zero for every token, so a refused one is replaced by a draw from the target's own row."""
+    B, K = 12, 2
+    target, _, _, u, _ = make(B, K, V, seed=V, cut=0.0)
+    target *= 0.25 + torch.rand(B, K + 1, 1, generator=torch.Generator().manual_seed(V))      # any sum, the draft's the same
+    tokens = target[:, :K].argmax(-1)
+    tokens[0::3, 0] = -1                                      # refused since they are no tokens
+    tokens[1::3, 1] = V
+    for b in range(2, B, 3):                                  # refused since neither gives them any weight
+        target[b, 0, tokens[b, 0]] = 0.0
+    out, accepted = check(target, target[:, :K].clone(), tokens, u)
+    assert accepted.tolist() == [0, 1, 0] * (B // 3)
