@@ -638,9 +638,12 @@ __global__ void __launch_bounds__(kExpandThreads, 2) adapt_expand_kernel(const A
   const int c_begin = chunk * P.chunk_cols, c_end = min(N, c_begin + P.chunk_cols);
   const TY* y = static_cast<const TY*>(P.y[mat]);
   TY* out = static_cast<TY*>(P.out[mat]);
-  if (count == 0) return;
-  if (id < 0) {                                            // no adapter: only a copy, where out is not y
-    if (y != out) adapt_copy<TY, VEC>(y, out, rows, count, N, c_begin, c_end);
+  if (count == 0 || id < 0) {
+    // no adapter: only a copy, where out is not y
+    if (count > 0 && y != out) adapt_copy<TY, VEC>(y, out, rows, count, N, c_begin, c_end);
+    // A launch in which nobody waits may end before the first one has read its ids, and what follows the call on the stream may
+    // overwrite those, or the workspace.  The first CTA always leads rows: it waits, here or for h.
+    if (blockIdx.x == 0 && blockIdx.y == 0) griddep_wait();
     return;
   }
   const int rank = P.rank, ksteps = (rank + KC - 1) / KC * (KC / 16);

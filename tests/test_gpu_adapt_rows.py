@@ -5,6 +5,8 @@ at most 3 K / 16 + 32 additions that may each lose a unit in the last place (2^-
 magnitudes bounds); what the pieces leave out is below 2^-21 of a product; the second product the same with the rank in K's
 place; y + delta is rounded once (fp32 2^-24, bf16 2^-8, fp16 2^-11 of the value; subnormal halves half of 2^-24).  For 16-bit rows h goes in with 16 of
 its bits (2^-15), and with fp16 weights products of two second pieces are left out (2^-14)."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -314,3 +316,29 @@ def test_h_keeps_24_bits_beside_rows_of_16(form, w):
     d = lambda v: v.to(TYPES[w]).to(DEV)
     got = ops.adapt_rows([(d(a), d(b), None)], [d(x)], ids.to(DEV), [d(y)])[0]
     assert torch.equal(got.double().cpu(), want)
+
+
+@pytest.mark.parametrize("shape", [(256, 1, 4096, [256, 256, 256], 32, 8), (40, 2, 64, [8], 4, 2), (2, 701, 4288, [64], 64, 2), (3, 700, 8, [8192], 64, 2)],
+                         ids=["gathered", "small", "first launch tiles", "second launch tiles"])
+def test_a_call_without_adapters_is_over_before_what_follows_it(shape):
+    """No row has an adapter, so nobody needs the first launch; the call still ends with it: ids that the next operation on the stream
+    fills in are not followed, and nothing is written to the workspace."""
+    banks, xs, ids, ys = make(*shape, torch.bfloat16, torch.float32)
+    streams, T, k, outs, rank, n = shape
+    L, m = _lib.lib(), len(outs)
+    bank = (_lib.Adapters * m)(*[_lib.Adapters(a.data_ptr(), b.data_ptr(), s.data_ptr(), o) for (a, b, s), o in zip(banks, outs)])
+    bf16, f32 = ops._DENSE_DTYPES[torch.bfloat16], ops._DENSE_DTYPES[torch.float32]
+    nbytes = L.b200rwkv_adapt_rows_workspace_bytes(m, bank, n, rank, k, bf16, streams, T)
+    ws = torch.full((nbytes,), 0xA5, dtype=torch.uint8, device=DEV)
+    p = lambda ts: (C.c_void_p * m)(*[t.data_ptr() for t in ts])
+    px, py = p(xs), p(ys)
+    before = [y.clone() for y in ys]
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(100):
+        ids.fill_(-1)
+        _lib.check(L.b200rwkv_adapt_rows(m, C.addressof(bank), n, rank, k, bf16, C.addressof(px), C.addressof(py), C.addressof(py), f32,
+                                         ids.data_ptr(), streams, T, ws.data_ptr(), nbytes, stream))
+        ids.zero_()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, b) for y, b in zip(ys, before))
+    assert bool((ws == 0xA5).all())
