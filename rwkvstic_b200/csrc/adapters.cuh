@@ -13,8 +13,12 @@
 //
 // Operands that are not of one 16-bit type are cut into bfloat16 pieces: a float is exactly three (the upper 8 bits of its
 // significand, the next 8, the last 8), a half exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21
-// of the whole together and left out.  The tensor cores cut their sums off, so no chain is longer than 64 k of a lane before its
-// part joins a sum that rounds.  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
+// of the whole together and left out.  The tensor cores cut the terms of a sum off at the last place of the largest, and its result, so
+// chains are short before their part joins a sum that rounds: in the first launch 64 k of a lane (tiles of 128 rows: 128 k), in the
+// second 32 ranks with the small products first, while the sum is small (tiles: all of up to 128 ranks).  Lost on average where all
+// terms are positive, fp32 throughout: first launch 5 units of 2^-23 of the sum for 512 k (tiles of 128 rows 20, for 2048), second
+// 0.8 for any rank (one chain of 256 ranks in the order of k 57; joining costs rank 256 up to a tenth, 110 -> 117 us for 4 x 500 rows
+// of 2048 -> 2048, ranks up to 32 nothing).  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
 // where it has an adapter.
 // What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces: 7B key, value and receptance for
 // 256 streams of 200 adapters (332 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (115 MB)
@@ -116,6 +120,18 @@ struct AdaptRaw {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       split_pair<P>(f.x, f.y, p);
     }
+  }
+  // their first pieces alone
+  __device__ __forceinline__ uint32_t first(int i) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return w[i];
+    uint32_t p[1];
+    if constexpr (std::is_same<T, float>::value) {
+      split_pair<1>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), p);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      split_pair<1>(f.x, f.y, p);
+    }
+    return p[0];
   }
 };
 
@@ -543,13 +559,6 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
       for (int i = 0; i < kPasses; ++i)
         if (i * kAtOnce < count) load_y(i, c0);
     }
-    float acc[MT][NT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
     for (int k0 = 0; k0 < rank; k0 += KC) {
       request();
       cp_async_wait<kStages - 1>();
@@ -569,39 +578,71 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
           }
         }
       from = from == slots + (kStages - 1) * Ring::kStage ? slots : from + Ring::kStage;
+      // weights that need no cutting: 8 rows at a time, for the registers
+      constexpr int NB = PW == 1 ? 1 : NT;
 #pragma unroll
-      for (int s = 0; s < KC / 16; ++s) {
-        uint32_t fa[MT][PW][4];
+      for (int n0 = 0; n0 < NT; n0 += NB) {
+        float acc[MT][NB][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t f[PW];
-            raw[m][i & 1].template pair<PW>(2 * s + (i >> 1), f);
+          for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
-          }
+            for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+        auto h_of = [&](int n, int s, int p) { return hf[(((n0 + n) * ksteps + k0 / 16 + s) * PH + p) * 32]; };
+        // the small products of the stage first, while the sum is small (see the head of this file)
 #pragma unroll
-        for (int p = PH - 1; p >= 0; --p)
+        for (int s = 0; s < KC / 16; ++s) {
+          uint32_t fa[MT][PW][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint2 h = hf[((n * ksteps + k0 / 16 + s) * PH + p) * 32];
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int w = PW - 1; w >= 0; --w) {
-              if (p + w >= PH) continue;
+            for (int i = 0; i < 4; ++i) {
+              uint32_t f[PW];
+              raw[m][i & 1].template pair<PW>(2 * s + (i >> 1), f);
 #pragma unroll
-              for (int m = 0; m < MT; ++m) mma_bf16(acc[m][n], fa[m][w], h.x, h.y);
+              for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
             }
+#pragma unroll
+          for (int p = PH - 1; p >= 0; --p)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              if (p == 0 && PW == 1) continue;
+              const uint2 h = h_of(n, s, p);
+#pragma unroll
+              for (int w = PW - 1; w >= 0; --w) {
+                if (p + w >= PH || p + w == 0) continue;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) mma_bf16(acc[m][n], fa[m][w], h.x, h.y);
+              }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < KC / 16; ++s) {
+          uint32_t fa[MT][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa[m][i] = raw[m][i & 1].first(2 * s + (i >> 1));
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const uint2 h = h_of(n, s, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma_bf16(acc[m][n], fa[m], h.x, h.y);
           }
+        }
+        if (k0 == 0 && n0 == 0) __syncwarp();              // the table has been read
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float* at = turn + ((n0 + n) * 8 + 2 * t + (i & 1)) * Ring::kPitch + m * 16 + (i >> 1) * 8 + g;
+              *at = k0 ? *at + acc[m][n][i] : acc[m][n][i];          // stages join here, rounding
+            }
       }
     }
-    __syncwarp();                                          // the table has been read
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) turn[(n * 8 + 2 * t + (i & 1)) * Ring::kPitch + m * 16 + (i >> 1) * 8 + g] = acc[m][n][i];
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {

@@ -51,8 +51,9 @@ struct TileControl {
 // fp16 14 and 15), bring 64 k of x and A at a time; one warp issues the MMAs.  x comes by asynchronous copies some stages ahead:
 // into the MMAs' own tiles where both operands are of one 16-bit type, else into slots of the thread that asked, which cuts it
 // into pieces.  (Loads into registers were bound by the few L1 lines that are left beside this much shared memory: 3B ffn, 8192
-// rows 62 us.)  Two stages make a sum: its additions (rank 64, fp32 x, bf16 A: 24) are cut off by the tensor cores, so those
-// warps add it up in registers, rounding, while the next one is formed in the other half of the TMEM columns.
+// rows 62 us.)  Two stages make a sum of 128 k: up to 48 MMAs (fp32 throughout), whose results
+// the tensor cores cut off, so those warps add it up in registers, rounding, while the next one is formed in the other half of
+// the TMEM columns.
 // What bounds it: with pieces, shared memory (a stage's 32 KB of x pass it five times), 3.4 TB/s from memory.
 constexpr int kShrinkTileRanks = 64;
 
@@ -556,17 +557,17 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
           tc_fence_after();
           const uint32_t d = tmem + uint32_t(buf * kAdaptTile);
           uint32_t more = 0u;
-          for (int k = 0; k < ksteps; ++k) {
-            const uint32_t off = uint32_t((k >> 2) * kTileBytes + (k & 3) * 32);
 #pragma unroll
-            for (int p = PH - 1; p >= 0; --p)
+          for (int p = PH - 1; p >= 0; --p)
 #pragma unroll
-              for (int w = PW - 1; w >= 0; --w) {
-                if (p + w >= PH) continue;
+            for (int w = PW - 1; w >= 0; --w) {            // the small products first
+              if (p + w >= PH) continue;
+              for (int k = 0; k < ksteps; ++k) {
+                const uint32_t off = uint32_t((k >> 2) * kTileBytes + (k & 3) * 32);
                 umma_f16<false>(d, umma_desc(base + slot * stage_bytes + w * h_piece + off), umma_desc(h_at + p * h_piece + off), idesc, more);
                 more = 1u;
               }
-          }
+            }
           umma_commit<false>(empty + 8 * slot);
           umma_commit<false>(acc_full + 8 * buf);
         }

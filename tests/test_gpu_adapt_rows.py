@@ -342,3 +342,22 @@ def test_a_call_without_adapters_is_over_before_what_follows_it(shape):
     torch.cuda.synchronize()
     assert all(torch.equal(y, b) for y, b in zip(ys, before))
     assert bool((ws == 0xA5).all())
+
+
+def test_long_ranks_are_not_cut_off_one_after_another():
+    """fp32 adapters of rank 256, all values positive, in units of 2^-23 of the whole.  A product of tensor cores cuts its terms, the running sum
+    among them, to the last place of the largest, and its result: up to a unit each, half of one on average.  A chain is 32 ranks: ten
+    products of small pieces, of 17 terms each, at a sum below 2^-6 of the chain's (2.7, on average 1.3), then two of the first pieces, which are
+    multiples of 2^-14 below 4 and lose nothing at a sum below 128, so that running sum and result, at half and at the whole, lose 3 (1.5).
+    Chains join by seven additions that round (3.5, on average 0); what is left out is below 2^-21 (4) and on average 2^-23 / 2.25 (0.5, pieces
+    being spread evenly); the sum with y rounds (0.5).  One chain of 256 ranks lost 57 on average."""
+    g = torch.Generator().manual_seed(3)
+    rank, n_out = 256, 4096
+    h, b = 1 + torch.rand(3, rank, generator=g), 1 + torch.rand(3, n_out, rank, generator=g)
+    a, x = torch.zeros(3, rank, 8), torch.zeros(6, 8)
+    a[:, :, 0], x[:, 0] = h, 1.0                              # h is exact: one product, of 1
+    ids = torch.tensor([0, 2, 1, 0, 2, 2])
+    got = ops.adapt_rows([(a.to(DEV), b.to(DEV), None)], [x.to(DEV)], ids.to(DEV), [torch.zeros(6, n_out, device=DEV)])[0].double().cpu()
+    want = torch.einsum("sr,snr->sn", h[ids].double(), b[ids].double())
+    lost = (want - got) / want * 2.0 ** 23
+    assert float(lost.abs().max()) <= 14.0 and abs(float(lost.mean())) <= 4.0, (float(lost.abs().max()), float(lost.mean()))
