@@ -372,6 +372,10 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
  * of x that holds an infinity or a NaN comes out as NaN where it has an adapter.  One or two launches on `stream`, no
  * allocation, capturable; device-side waits are bounded (1 s), and rows whose wait runs out come out as NaN.  Outputs that
  * overlap more than their own y are refused.  No counterpart in the reference.
+ * b200rwkv_adapt_rows_status waits for `stream` and returns B200RWKV_ETIMEOUT if a wait of a call that has ended on the current
+ * device expired since it was last asked, and B200RWKV_OK otherwise; refused while `stream` is captured.  The word it reads and
+ * clears, for hosts that look without waiting, is a device int32 whose address b200rwkv_adapt_rows_status_word returns (NULL
+ * without a device).
  */
 typedef struct b200rwkv_adapters {
   const void *a, *b;
@@ -383,6 +387,8 @@ size_t b200rwkv_adapt_rows_workspace_bytes(int nmat, const b200rwkv_adapters* ba
 int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int dtype, const void* const* x,
                         const void* const* y, void* const* out, int row_dtype, const int64_t* ids, int streams, int tokens_per_stream,
                         void* workspace, size_t workspace_bytes, void* stream);
+int b200rwkv_adapt_rows_status(void* stream);
+int32_t* b200rwkv_adapt_rows_status_word(void);
 
 /*
  * Verification of drafted tokens.  Per stream, step t = 0, 1, ... (up to its number of drafted tokens): token d is accepted

@@ -22,7 +22,8 @@ EXPORTS = (
     "b200rwkv_decode_workspace_bytes", "b200rwkv_decode_step", "b200rwkv_decode_step_traced", "b200rwkv_decode_step_stage",
     "b200rwkv_gemm_plan", "b200rwkv_gemm_workspace_bytes", "b200rwkv_gemm_u8", "b200rwkv_rows_workspace_bytes", "b200rwkv_forward_rows", "b200rwkv_forward_rows_stage", "b200rwkv_argmax",
     "b200rwkv_sample_typical", "b200rwkv_gemv_dense",
-    "b200rwkv_adapt_rows_workspace_bytes", "b200rwkv_adapt_rows", "b200rwkv_verify_drafts_workspace_bytes", "b200rwkv_verify_drafts",
+    "b200rwkv_adapt_rows_workspace_bytes", "b200rwkv_adapt_rows", "b200rwkv_adapt_rows_status", "b200rwkv_adapt_rows_status_word",
+    "b200rwkv_verify_drafts_workspace_bytes", "b200rwkv_verify_drafts",
     "b200rwkv_advance_state", "b200rwkv_forward_rows_draft",
     "b200rwkv_dense_workspace_bytes", "b200rwkv_dense_step", "b200rwkv_dense_rows_workspace_bytes", "b200rwkv_dense_forward_rows",
     "b200rwkv_dense_step_layers", "b200rwkv_dense_forward_rows_layers", "b200rwkv_wait_selftest", "b200rwkv_debug_expire_waits",
@@ -151,6 +152,10 @@ def lib() -> C.CDLL:
     L.b200rwkv_adapt_rows.restype = C.c_int
     L.b200rwkv_adapt_rows.argtypes = ([C.c_int, C.c_void_p] + [C.c_int] * 4 + [C.c_void_p] * 3 +      # arrays, or their bytes
                                       [C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p])
+    L.b200rwkv_adapt_rows_status.restype = C.c_int
+    L.b200rwkv_adapt_rows_status.argtypes = [C.c_void_p]
+    L.b200rwkv_adapt_rows_status_word.restype = C.c_void_p
+    L.b200rwkv_adapt_rows_status_word.argtypes = []
     L.b200rwkv_verify_drafts_workspace_bytes.restype = C.c_size_t
     L.b200rwkv_verify_drafts_workspace_bytes.argtypes = [C.c_int] * 3
     L.b200rwkv_verify_drafts.restype = C.c_int

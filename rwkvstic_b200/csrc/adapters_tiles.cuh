@@ -4,7 +4,7 @@
 // The operands are the same bfloat16 pieces (or values of one 16-bit type), cut by the threads that bring them and laid out
 // in shared memory as the MMAs want them: rows of 64 elements, 128-byte swizzle.  At rank 64 and fp32 rows the pieces are
 // 26 multiplications a byte, which mma.sync just about kept up with (and less under the power cap); tcgen05 leaves the
-// memory as the bound.  Every wait is bounded; where one runs out the rows concerned come out as NaN.
+// memory as the bound.  Every wait is bounded; where one runs out the rows concerned come out as NaN and g_adapt_status says so.
 #pragma once
 
 #include "adapters.cuh"
@@ -15,6 +15,9 @@ namespace b200 {
 constexpr int kAdaptTile = 128;            // rows of a tile; columns of a step of the second launch
 constexpr int kTileBytes = kAdaptTile * 128;         // 128 rows of 64 elements
 constexpr int kTileRankMax = 128;          // of the second launch: two times 64 ranks
+
+// Status bits of expired waits, kept per GPU: a call's workspace is the caller's and holds nothing between calls.
+static __device__ int g_adapt_status;
 
 __device__ __forceinline__ void fence_smem_to_mma() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int COLS>
@@ -274,6 +277,7 @@ __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_
                 const int r = i / kShrinkTileRanks, j = i % kShrinkTileRanks;
                 if (j < ranks) h[size_t(r) * rank + j] = v;
               });
+  if (tid == 0 && *abort_flag) atomicOr(&g_adapt_status, B200RWKV_STATUS_WAIT_FULL);
   if (warp == S::kWorkers / 32) {
     tc_fence_after();
     tmem_free_cols<128>(tmem);
@@ -610,6 +614,7 @@ __global__ void __launch_bounds__(kExpandTileThreads, 1) adapt_expand_tile_kerne
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(&g_adapt_status, B200RWKV_STATUS_WAIT_FULL);
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_free_cols<256>(tmem);

@@ -2116,6 +2116,32 @@ int b200rwkv_adapt_rows(int nmat, const b200rwkv_adapters* banks, int n_adapters
   return B200RWKV_OK;
 }
 
+int32_t* b200rwkv_adapt_rows_status_word(void) {
+  void* p = nullptr;
+  if (device_sms() < 1 || cudaGetSymbolAddress(&p, g_adapt_status) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  return static_cast<int32_t*>(p);
+}
+
+int b200rwkv_adapt_rows_status(void* stream) {
+  int32_t* word = b200rwkv_adapt_rows_status_word();
+  if (!word) return fail(B200RWKV_ECUDA, "adapt_rows_status: no CUDA device");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(s, &capturing);
+  if (e == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
+    return fail(B200RWKV_EINVAL, "adapt_rows_status: the stream is being captured, and this call waits for it");
+  int32_t bits = 0;
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&bits, word, 4, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && bits) e = cudaMemsetAsync(word, 0, 4, s);
+  if (e != cudaSuccess) return fail(B200RWKV_ECUDA, "adapt_rows_status: %s", cudaGetErrorString(e));
+  if (bits) return fail(B200RWKV_ETIMEOUT, "adapt_rows: a bounded device-side wait expired (status bits %d)", bits);
+  return B200RWKV_OK;
+}
+
 size_t b200rwkv_verify_drafts_workspace_bytes(int streams, int drafts, int n) {
   if (streams < 1 || streams > 65535 || drafts < 0 || drafts > kVerifyMaxDrafts || n < 1 || n > kVerifySeg * kVerifyMaxSegs) return 0;
   return size_t(streams) * (2 * drafts + 1) * verify_segs(n) * 8;

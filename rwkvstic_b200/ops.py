@@ -245,7 +245,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     ``[streams]``; all contiguous on one CUDA device.  Rank a multiple of 4 up to 256, k_in of 8, up to 65535 rows.  In
     place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T`` is
     fp32 whatever the types, products leave out less than 2^-21 of themselves, and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
-    adapter; rows without one are left as they are."""
+    adapter; rows without one are left as they are.  Should a bounded device-side wait of the forms for many rows expire,
+    its rows come out as NaN and ``check_status`` raises."""
     n = len(banks)
     outs = ys if outs is None else outs
     if n < 1 or n > 3 or len(xs) != n or len(ys) != n or len(outs) != n:
@@ -299,6 +300,13 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
         _lib.check(_lib.lib().b200rwkv_adapt_rows(n, at, count, rank, k_in, code, at + 32 * n, at + 40 * n, at + 48 * n, _DENSE_DTYPES[row_dt],
                                                   ids.data_ptr(), streams, tokens, ws.data_ptr(), nbytes, _raw_stream(index)))
     return list(outs)
+
+
+def check_status(device=None) -> None:
+    """Raise if a device-side wait of an ``adapt_rows`` call that has ended on ``device`` (the current one when omitted)
+    expired since the last check.  Waits for the device's current stream."""
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().b200rwkv_adapt_rows_status(_stream(device)))
 
 
 _ADAPT_PACK = {n: struct.Struct("=" + "QQQi4x" * n + "%dQ" % (3 * n)) for n in (1, 2, 3)}

@@ -6,7 +6,7 @@ import time
 import pytest
 import torch
 
-from rwkvstic_b200 import _lib
+from rwkvstic_b200 import _lib, ops
 from rwkvstic_b200.dense_model import B200DenseRWKV
 from rwkvstic_b200.synth import synth_tokens
 
@@ -61,3 +61,34 @@ def test_rows_kernel_gives_up_when_its_copies_are_withheld_and_recovers():
     torch.cuda.synchronize()
     assert torch.equal(m._logits, good) and torch.equal(again, good_state)
     m.check_status()
+
+
+def test_an_expired_wait_of_adapt_rows_is_reported_once():
+    """The word that its tile kernels set, and what reads it; the wait that runs out here is the self-test's."""
+    L = _lib.lib()
+    rows = lambda *s: torch.randn(*s, device=DEV)
+    bank, x, y, ids = (rows(2, 64, 4288).bfloat16(), rows(2, 4096, 64).bfloat16(), None), rows(1402, 4288), rows(1402, 4096), torch.tensor([0, 1], device=DEV)
+    ops.adapt_rows([bank], [x], ids, [y])                     # tiles of 128 rows
+    ops.check_status()
+    assert not torch.isnan(y).any()
+    word = L.b200rwkv_adapt_rows_status_word()
+    assert word
+    _lib.check(L.b200rwkv_wait_selftest(2_000_000, word, torch.cuda.current_stream().cuda_stream))
+    with pytest.raises(_lib.B200RWKVError, match="adapt_rows") as err:
+        ops.check_status(DEV)
+    assert err.value.code == _lib.ETIMEOUT
+    ops.check_status(DEV)                                     # cleared by the check that raised
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.check_status()
+    graph = torch.cuda.CUDAGraph()
+    refused = None
+    with torch.cuda.graph(graph):
+        y.add_(1.0)
+        try:
+            ops.check_status()
+        except _lib.B200RWKVError as e:
+            refused = e.code
+    assert refused == _lib.EINVAL
+    graph.replay()
+    torch.cuda.synchronize()

@@ -77,3 +77,10 @@ def test_pack_adapters():
     for bad in ([], [(torch.ones(3, 16), torch.ones(5, 4), 1.0)], [(torch.ones(3, 16), torch.ones(5, 3), 1.0), (torch.ones(3, 15), torch.ones(5, 3), 1.0)]):
         with pytest.raises(ValueError):
             ops.pack_adapters(bad)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what a host without a device gets")
+def test_adapt_rows_status_without_a_device():
+    L = _lib.lib()
+    assert L.b200rwkv_adapt_rows_status_word() is None
+    assert L.b200rwkv_adapt_rows_status(None) == _lib.ECUDA and b"no CUDA device" in L.b200rwkv_last_error()
