@@ -360,7 +360,8 @@ int b200rwkv_sample_typical(const float* x, int rows, int n, int64_t ldx, float 
  *   out_i[r][:] = y_i[r][:] + scale_i[id] * (x_i[r][:] A_i[id]^T) B_i[id]^T,   id = ids[r / tokens_per_stream]
  * for rows r of streams with an adapter; an id outside [0, n_adapters) means none, and out_i[r] = y_i[r].
  *   banks     a device [n_adapters][rank][k_in], b device [n_adapters][n_out][rank] of `dtype` (B200RWKV_F32 / _BF16 / _F16),
- *             16-byte aligned; scale device f32 [n_adapters], NULL for 1.  rank a multiple of 4 up to 256, k_in of 8
+ *             16-byte aligned; scale device f32 [n_adapters], NULL for 1.  rank a multiple of 4 up to 256, k_in of 8 up to
+ *             2^30, n_out up to 2^22
  *   x, y, out device [streams * tokens_per_stream][k_in] and [...][n_out_i] of row_dtype (f32, or the weights' type), x
  *             16-byte aligned; out_i may be y_i and overlaps nothing else.  Rows <= 65535
  *   ids       device int64 [streams], read on the device (a captured call follows them)

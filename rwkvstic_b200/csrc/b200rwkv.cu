@@ -2052,7 +2052,7 @@ static bool adapt_tile_fits(int dtype, int row_dtype, int rank) {
 static const char* adapt_problem(int nmat, const b200rwkv_adapters* banks, int n_adapters, int rank, int k_in, int streams, int tokens_per_stream) {
   if (nmat < 1 || nmat > kAdaptMaxMats || !banks) return "1..3 banks";
   if (n_adapters < 1 || rank < 4 || rank > kAdaptMaxRank || rank % 4) return "at least one adapter, rank a multiple of 4 up to 256";
-  if (k_in < 8 || k_in % 8) return "k_in a positive multiple of 8";
+  if (k_in < 8 || k_in % 8 || k_in > (1 << 30)) return "k_in a positive multiple of 8 up to 2^30";
   if (streams < 1 || tokens_per_stream < 1 || (long long)streams * tokens_per_stream > 65535) return "1..65535 rows";
   for (int i = 0; i < nmat; ++i)
     if (banks[i].n_out < 1 || banks[i].n_out > (1 << 22)) return "n_out 1..4194304";

@@ -242,11 +242,11 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
 
     ``banks[i] = (a [n,rank,k_in], b [n,n_out_i,rank], scale f32 [n] or None)`` of bf16, fp16 or fp32 (see
     ``pack_adapters``), ``xs[i] [rows,k_in]`` and ``ys[i] [rows,n_out_i]`` of fp32 or the banks' type, ``ids`` int64
-    ``[streams]``; all contiguous on one CUDA device.  Rank a multiple of 4 up to 256, k_in of 8, up to 65535 rows.  In
-    place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T`` is
-    fp32 whatever the types, products leave out less than 2^-21 of themselves, and the result is rounded once.  A row of x that holds an infinity or a NaN comes out as NaN where it has an
-    adapter; rows without one are left as they are.  Should a bounded device-side wait of the forms for many rows expire,
-    its rows come out as NaN and ``check_status`` raises."""
+    ``[streams]``; all contiguous on one CUDA device.  Rank a multiple of 4 up to 256, k_in of 8 up to 2^30, up to 65535
+    rows.  In place on ``ys`` when ``outs`` is omitted; an output may be its own y and overlaps nothing else.  ``h = x A^T``
+    is fp32 whatever the types, products leave out less than 2^-21 of themselves, and the result is rounded once.  A row of
+    x that holds an infinity or a NaN comes out as NaN where it has an adapter; rows without one are left as they are.
+    Should a bounded device-side wait of the forms for many rows expire, its rows come out as NaN and ``check_status`` raises."""
     n = len(banks)
     outs = ys if outs is None else outs
     if n < 1 or n > 3 or len(xs) != n or len(ys) != n or len(outs) != n:
@@ -264,6 +264,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
     rows, streams = x_shape[0], ids.shape[0]
     if ids.dtype != torch.int64 or ids.get_device() != index or not ids.is_contiguous() or (rows % streams if streams else rows):
         raise ValueError("ids must be contiguous int64 on the banks' device, one per stream, and the rows a multiple of them")
+    if (count | k_in | rows) >> 31:
+        raise ValueError("adapt_rows takes sizes of 32 bits")
     packed, px, py, po, n_out = [], [], [], [], []
     x_want = (rows, k_in)
     for (a, b, s), x, y, o in zip(banks, xs, ys, outs):
@@ -276,6 +278,8 @@ def adapt_rows(banks: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.
         if s is not None and (s.dtype != torch.float32 or s.get_device() != index or s.shape != (count,) or not s.is_contiguous()):
             raise ValueError("an adapter bank's scale must be contiguous fp32 [n] on its device")
         n_o = b_shape[1]
+        if n_o >> 31:
+            raise ValueError("adapt_rows takes sizes of 32 bits")
         y_want = (rows, n_o)
         if (x.shape != x_want or y.shape != y_want or x.dtype != row_dt or y.dtype != row_dt or x.get_device() != index
                 or y.get_device() != index or not x.is_contiguous() or not y.is_contiguous()):
@@ -335,6 +339,8 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     if target.dim() != 3 or tokens.dim() != 2 or target.dtype != torch.float32 or index < 0:
         raise ValueError("verify_drafts needs fp32 CUDA weights [B,K+1,V] and tokens [B,K]")
     (B, K), V = tokens.shape, target.shape[2]
+    if (B | K | V) >> 31:
+        raise ValueError("verify_drafts takes sizes of 32 bits")
     t_stream, t_row, t_step = target.stride()
     if target.shape != (B, K + 1, V) or (V > 1 and t_step != 1):
         raise ValueError(f"target must be [{B},{K + 1},V] with contiguous rows, got {tuple(target.shape)}")
@@ -381,6 +387,8 @@ def advance_state(state: torch.Tensor, counts: torch.Tensor, trace: torch.Tensor
         raise ValueError("advance_state needs state [B,L,5,C] and trace [L,4,B,T,C]")
     B, L, _, Cc = shape
     T = trace.shape[3]
+    if (B | L | T | Cc) >> 31:
+        raise ValueError("advance_state takes sizes of 32 bits")
     out = state if out is None else out
     for t, want in ((state, shape), (out, shape), (trace, (L, 4, B, T, Cc)), (params, (L, 5, Cc))):
         if t.dtype != torch.float32 or index < 0 or t.get_device() != index or t.shape != want or not t.is_contiguous():

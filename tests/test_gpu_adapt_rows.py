@@ -361,3 +361,20 @@ def test_long_ranks_are_not_cut_off_one_after_another():
     want = torch.einsum("sr,snr->sn", h[ids].double(), b[ids].double())
     lost = (want - got) / want * 2.0 ** 23
     assert float(lost.abs().max()) <= 14.0 and abs(float(lost.mean())) <= 4.0, (float(lost.abs().max()), float(lost.mean()))
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """They would wrap on their way to the library and be taken for small ones (2^32 + 64 for 64).  Nothing here is ever read."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 60 << 30:
+        pytest.skip("45 GB for the tensors")
+    wide = 2 ** 32 + 64
+    a, x, ids = torch.empty(1, 4, wide, dtype=torch.bfloat16, device=DEV), torch.empty(1, wide, dtype=torch.bfloat16, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    b, y = torch.zeros(1, 8, 4, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 8, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.adapt_rows([(a, b, None)], [x], ids, [y])
+    with pytest.raises(_lib.B200RWKVError, match="k_in"):     # within 32 bits, but not in blocks of 32
+        k = 2 ** 31 - 8
+        ops.adapt_rows([(a.view(-1)[:4 * k].view(1, 4, k), b, None)], [x[:, :k].contiguous()], ids, [y])
+    del a, x
+    torch.cuda.empty_cache()

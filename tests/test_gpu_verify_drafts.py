@@ -202,3 +202,13 @@ def test_nothing_is_left_where_the_draft_equals_the_target(V):
         target[b, 0, tokens[b, 0]] = 0.0
     out, accepted = check(target, target[:, :K].clone(), tokens, u)
     assert accepted.tolist() == [0, 1, 0] * (B // 3)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """They would wrap on their way to the library (a vocabulary of 2^32 + 5 taken for 5).  Nothing here is ever read."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 20 << 30:
+        pytest.skip("17 GB for the weights")
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.verify_drafts(torch.empty(1, 1, 2 ** 32 + 5, device=DEV), None, torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.zeros(1, 1, device=DEV))
+    torch.cuda.empty_cache()

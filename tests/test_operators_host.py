@@ -84,3 +84,8 @@ def test_adapt_rows_status_without_a_device():
     L = _lib.lib()
     assert L.b200rwkv_adapt_rows_status_word() is None
     assert L.b200rwkv_adapt_rows_status(None) == _lib.ECUDA and b"no CUDA device" in L.b200rwkv_last_error()
+
+
+def test_adapt_rows_refuses_a_k_in_that_blocks_of_it_would_pass_32_bits():
+    for k in (2 ** 31 - 8, 2 ** 30 + 8):
+        assert adapt(k=k) == _lib.EINVAL and b"k_in" in _lib.lib().b200rwkv_last_error()
