@@ -212,3 +212,11 @@ def test_sizes_beyond_32_bits_are_refused():
     with pytest.raises(ValueError, match="32 bits"):
         ops.verify_drafts(torch.empty(1, 1, 2 ** 32 + 5, device=DEV), None, torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.zeros(1, 1, device=DEV))
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("B,K,V", [(2, 3, 524288), (1, 64, 524287), (3, 1, 262145)])
+@pytest.mark.parametrize("drafted", [True, False])
+def test_the_largest_sizes(B, K, V, drafted):
+    target, draft, tokens, u, lengths = make(B, K, V, seed=K)
+    check(target, draft if drafted else None, tokens, u, lengths)
+    check(target, draft if drafted else None, tokens, u)
