@@ -13,18 +13,19 @@
 //
 // Operands that are not of one 16-bit type are cut into bfloat16 pieces: a float is exactly three (the upper 8 bits of its
 // significand, the next 8, the last 8), a half exactly two.  Products of pieces i and j with i + j of 3 and more are below 2^-21
-// of the whole together and left out.  The tensor cores cut the terms of a sum off at the last place of the largest, and its result, so
-// chains are short before their part joins a sum that rounds: in the first launch 64 k of a lane (tiles of 128 rows: 128 k), in the
-// second 32 ranks with the small products first, while the sum is small (tiles: all of up to 128 ranks).  Lost on average where all
-// terms are positive, fp32 throughout: first launch 5 units of 2^-23 of the sum for 512 k (tiles of 128 rows 20, for 2048), second
-// 0.8 for any rank (one chain of 256 ranks in the order of k 57; joining costs rank 256 up to a tenth, 110 -> 117 us for 4 x 500 rows
-// of 2048 -> 2048, ranks up to 32 nothing).  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
+// of the whole together and left out.  A piece of an infinity is NaN: a row of x that holds an infinity or a NaN comes out as NaN,
 // where it has an adapter.
-// What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces: 7B key, value and receptance for
-// 256 streams of 200 adapters (332 MB) 66 us, the first launch 33, the second 39, overlapping; 3B head for 48 x 5 rows (115 MB)
-// 33; 7B ffn for 64 streams of 48 adapters (56 MB) 23.  Fragments go from global memory to a lane's own slots of shared memory
-// and from there to its registers, without a barrier between warps.  The index along a product is free to permute, and is, so
-// that a lane's elements are consecutive: 16 bytes of A, 8 of B.
+// The tensor cores cut the terms of a sum off at the last place of the largest, and its result, so chains are short before their
+// part joins a sum that rounds, with the small products first, while the sum is small: in the first launch 32 k of a lane (64 where
+// nothing is cut; tiles of 128 rows twice that), in the second 32 ranks (tiles: all of up to 128).  Lost on average where all terms
+// are positive, in units of 2^-23 of the sum, fp32 throughout: 0.2 to 0.8 for any K or rank.  In the order of k one chain of 256
+// ranks lost 57, of 128 k 20 and of 64 k 5 to 13, in the same time but for ranks of 256 (4 x 500 rows of 2048 -> 2048, fp32: 110 us
+// in one chain, 117 joined).
+// What bounds the gathered tiles is what they read and, at rank 64, the lanes that cut pieces (on the GPU alone): 7B key, value and
+// receptance for 256 streams of 200 adapters (332 MB) 68 us, the first launch 33, the second 42, overlapping; 3B head for 48 x 5
+// rows (115 MB) 33; 7B ffn for 64 streams of 48 adapters (56 MB) 23.  Fragments go from global memory to a lane's own slots of
+// shared memory and from there to its registers, without a barrier between warps.  The index along a product is free to permute,
+// and is, so that a lane's elements are consecutive: 16 bytes of A, 8 of B.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -282,6 +283,14 @@ __device__ __forceinline__ float* shrink_sums(const AdaptParams& P, const TX* x,
   };
   for (int kb = b0 + warp; kb < b1; kb += 2 * kShrinkWarps) {   // two blocks; one past the end holds zeros
     float part[MT][NT][4];                                 // the tensor cores cut their sums off; the running sum rounds
+    auto join = [&] {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
+    };
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
       request();
@@ -293,43 +302,60 @@ __device__ __forceinline__ float* shrink_sums(const AdaptParams& P, const TX* x,
 #pragma unroll
       for (int q = 0; q < NT; ++q) take(rx[q], from + (2 * MT * Ring::kA + q * Ring::kX) * 512);
       from = from == slots + (kStages - 1) * Ring::kStage ? slots : from + Ring::kStage;
+      if constexpr (PX * PW > 1) {                         // small products of the block first, while the sum is small
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {               // elements 4 step .. 4 step + 3 of every lane
-        uint32_t fx[NT][2][PX], fa[MT][PW][4];
+        for (int step = 0; step < 2; ++step) {             // elements 4 step .. 4 step + 3 of every lane
+          uint32_t fx[NT][2][PX], fa[MT][PW][4];
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) rx[q].template pair<PX>(2 * step + i, fx[q][i]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t f[PW];
+              ra[m][i & 1].template pair<PW>(2 * step + (i >> 1), f);
+#pragma unroll
+              for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
+            }
+          bool first = step == 0;
+#pragma unroll
+          for (int i = PW - 1; i >= 0; --i)
+#pragma unroll
+            for (int j = PX - 1; j >= 0; --j) {
+              if (i + j >= 3 || i + j == 0) continue;
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < NT; ++q) mma_to<false>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
+              first = false;
+            }
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        uint32_t fx[NT][2], fa[MT][4];
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) rx[q].template pair<PX>(2 * step + i, fx[q][i]);
+          for (int i = 0; i < 2; ++i) fx[q][i] = kSame ? rx[q].w[2 * step + i] : rx[q].first(2 * step + i);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t f[PW];
-            ra[m][i & 1].template pair<PW>(2 * step + (i >> 1), f);
-#pragma unroll
-            for (int w = 0; w < PW; ++w) fa[m][w][i] = f[w];
+            const int at = 2 * step + (i >> 1);
+            fa[m][i] = kSame ? ra[m][i & 1].w[at] : ra[m][i & 1].first(at);
           }
-        bool first = o == 0 && step == 0;
 #pragma unroll
-        for (int i = PW - 1; i >= 0; --i)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int j = PX - 1; j >= 0; --j) {
-            if (i + j >= 3) continue;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int q = 0; q < NT; ++q)
-                mma_to<std::is_same<TX, __half>::value && kSame>(first, part[m][q], fa[m][i], fx[q][0][j], fx[q][1][j]);
-            first = false;
-          }
+          for (int q = 0; q < NT; ++q)
+            mma_to<std::is_same<TX, __half>::value && kSame>(kSame && o == 0 && step == 0, part[m][q], fa[m], fx[q][0], fx[q][1]);
       }
+      if constexpr (PX * PW > 1) join();
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < NT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][q][i] += part[m][q][i];
+    if constexpr (PX * PW == 1) join();
   }
   cp_async_wait<0>();
   __syncthreads();                                         // the slots become the table of sums

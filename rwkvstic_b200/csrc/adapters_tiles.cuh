@@ -54,9 +54,8 @@ struct TileControl {
 // fp16 14 and 15), bring 64 k of x and A at a time; one warp issues the MMAs.  x comes by asynchronous copies some stages ahead:
 // into the MMAs' own tiles where both operands are of one 16-bit type, else into slots of the thread that asked, which cuts it
 // into pieces.  (Loads into registers were bound by the few L1 lines that are left beside this much shared memory: 3B ffn, 8192
-// rows 62 us.)  Two stages make a sum of 128 k: up to 48 MMAs (fp32 throughout), whose results
-// the tensor cores cut off, so those warps add it up in registers, rounding, while the next one is formed in the other half of
-// the TMEM columns.
+// rows 62 us.)  A stage (two, 128 k, where nothing is cut) makes a sum, which those warps add up in registers, rounding, while the
+// next one is formed in the other half of the TMEM columns.
 // What bounds it: with pieces, shared memory (a stage's 32 KB of x pass it five times), 3.4 TB/s from memory.
 constexpr int kShrinkTileRanks = 64;
 
@@ -68,6 +67,7 @@ struct ShrinkTile {
   static constexpr int kSums = kShrinkTileRanks / (kWorkers / 128);        // ranks whose sums a thread has, of one row
   static_assert(kSums % 16 == 0, "");
   static constexpr int kBytesX = PX * kTileBytes, kStage = kBytesX + PW * kTileBytes / 2;
+  static constexpr int kChain = kSame ? 2 : 1;             // stages whose sum the tensor cores form
   static constexpr int kStages = kSame ? 8 : 2, kRaw = kSame ? 0 : 64 * kAdaptTile * int(sizeof(TX));
   static constexpr int kFit = kSame ? 0 : (226 * 1024 - 1024 - 2 * kStage) / kRaw;
   static constexpr int kRing = kFit > 4 ? 4 : kFit;        // stages of x as it comes
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_
       cp_async_commit();                                   // a group per stage, also an empty one
     };
     bool ok = true;
-    auto flush = [&](int g) {                              // the sum of stages 2 g and 2 g + 1
+    auto flush = [&](int g) {                              // the sum of stages kChain g .. kChain g + kChain - 1
       ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * (g & 1), uint32_t(g >> 1) & 1u, abort_flag));
       if (!ok) return;
       tc_fence_after();
@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_
       mbar_arrive(full + 8 * slot);
       if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
       const int n = c - c0;
-      if (n >= 2 && (n & 1) == 0) flush(n / 2 - 1);
+      if (n >= S::kChain && n % S::kChain == 0) flush(n / S::kChain - 1);
     }
-    if (ok) flush((c1 - c0 + 1) / 2 - 1);                  // the others have been
+    if (ok) flush((c1 - c0 + S::kChain - 1) / S::kChain - 1);        // the others have been
     cp_async_wait<0>();
     if (!ok)
 #pragma unroll
@@ -237,13 +237,14 @@ __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_
     int slot = 0;
     uint32_t phase = 0;
     for (int c = c0; c < c1; ++c) {
-      const int n = c - c0, g = n >> 1;
-      if ((n & 1) == 0 && !warp_wait(acc_empty + 8 * (g & 1), (uint32_t(g >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0)) break;
+      const int n = c - c0, g = n / S::kChain;
+      const bool starts = n % S::kChain == 0, ends = n % S::kChain == S::kChain - 1 || c + 1 == c1;
+      if (starts && !warp_wait(acc_empty + 8 * (g & 1), (uint32_t(g >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0)) break;
       if (!warp_wait(full + 8 * slot, phase, abort_flag, nullptr, 0)) break;
       if (elect_one()) {
         tc_fence_after();
         const uint32_t at = base + slot * S::kStage, d = tmem + uint32_t((g & 1) * 64);
-        uint32_t more = (n & 1) != 0;
+        uint32_t more = !starts;
 #pragma unroll
         for (int i = S::PW - 1; i >= 0; --i)
 #pragma unroll
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(ShrinkTile<TX, TW>::kThreads, 1) adapt_shrink_
             }
           }
         umma_commit<false>(empty + 8 * slot);
-        if ((n & 1) != 0 || c + 1 == c1) umma_commit<false>(acc_full + 8 * (g & 1));
+        if (ends) umma_commit<false>(acc_full + 8 * (g & 1));
       }
       __syncwarp();
       if (++slot == S::kStages) { slot = 0; phase ^= 1u; }
@@ -674,6 +675,7 @@ inline AdaptShape adapt_shape(int nmat, const int* n_out, int adapters, int rank
     const long long most = adapters + (long long)streams * T / kAdaptRows + 1;
     return !tiled && T < kAdaptRows && most < n ? most : (long long)n;
   };
+  // fp16 and fp32: 32 ranks, for the registers of a lane that cuts them (also beside fp16 rows, where nothing is cut)
   s.mt = rank <= 16 ? 1 : rank <= 32 || w_pieces > 1 ? 2 : 4;
   s.kc = rank <= 16 ? 16 : 32;
   s.fused = !s.tiles1 && rank <= 16 * s.mt && (long long)s.n1 * nmat * kFusedCtas <= cluster_room(kFusedCtas, sms);

@@ -378,3 +378,24 @@ def test_sizes_beyond_32_bits_are_refused():
         ops.adapt_rows([(a.view(-1)[:4 * k].view(1, 4, k), b, None)], [x[:, :k].contiguous()], ids, [y])
     del a, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("w", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("streams,T,k,chain", [(6, 1, 4096, 32), (200, 1, 4096, 32), (3, 700, 16384, 64)], ids=["one launch", "gathered", "tiles"])
+def test_long_inputs_are_not_cut_off_one_after_another(streams, T, k, chain, w):
+    """The first product of rows of fp32, all values positive; units and arithmetic as above.  A chain is 32 k of a lane (tiles: 64 of a tile):
+    the products of small pieces, up to five for 16 k, come first and lose 17 terms each at 2^-6 of the chain's sum; the first pieces' lose running
+    sum and result only, twice for 16 k (32 k: 2 (1/2 + 1) = 3, 64 k: 2 (1/4 + 1/2 + 3/4 + 1) = 5).  Half of both on average, and 0.5 of what
+    is left out (4 at most).  Chains join by additions that round, 0.5 each and 0 on average.  The second product is of h and one, exact.
+    Chains of 64 and 128 k in the order of k lost 13 and 20 on average."""
+    g = torch.Generator().manual_seed(5)
+    a, x = (1 + torch.rand(3, 4, k, generator=g)).to(TYPES[w]), 1 + torch.rand(streams * T, k, generator=g)
+    b = torch.zeros(3, 8, 4, dtype=TYPES[w])
+    b[:, :, 0] = 1.0
+    ids = torch.arange(streams) % 3
+    got = ops.adapt_rows([(a.to(DEV), b.to(DEV), None)], [x.to(DEV)], ids.to(DEV), [torch.zeros(streams * T, 8, device=DEV)])[0].double().cpu()
+    want = torch.cat([x[i * T:(i + 1) * T].double() @ a[i % 3, 0].double() for i in range(streams)]).unsqueeze(1)
+    lost = (want - got) / want * 2.0 ** 23
+    chains = 17 * 5 * (chain // 16) / 64 + (3 if chain == 32 else 5)
+    joins = k // 256 + 16 if chain == 32 else k // 64 + 8
+    assert abs(float(lost.mean())) <= chains / 2 + 0.5 and float(lost.abs().max()) <= chains + 4 + joins / 2, (float(lost.mean()), float(lost.abs().max()))
