@@ -422,8 +422,8 @@ int b200rwkv_verify_drafts(const float* target, int64_t target_stream_stride, in
  * state); counts device int64 [streams], clamped to [0, tokens], 0 leaves the state as it is; trace device f32
  * [layers][4][streams][tokens][channels]: the residual stream in front of ln1 and of ln2, key and value of every token; params
  * device f32 [layers][5][channels]: ln1 weight and bias, ln2 weight and bias, w = -exp(time_decay).  Row 0 / 1 become the layer
- * norm of the last accepted token's rows, rows 2..4 take counts[s] WKV steps (agnosticRwkv.py:68-103).  channels a multiple of 4;
- * all buffers 16-byte aligned, out state itself or apart from the other buffers.  One launch, no allocation, capturable.
+ * norm of the last accepted token's rows, rows 2..4 take counts[s] WKV steps (agnosticRwkv.py:68-103).  channels a multiple of 4
+ * up to 2^20, streams * layers up to 2^24; all buffers 16-byte aligned, out state itself or apart from the other buffers.  One launch, no allocation, capturable.
  */
 int b200rwkv_advance_state(const float* state, float* out, const int64_t* counts, const float* trace, const float* params, int streams,
                            int layers, int tokens, int channels, void* stream);

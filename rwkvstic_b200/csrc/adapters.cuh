@@ -558,7 +558,7 @@ __device__ __forceinline__ void expand_columns(const AdaptParams& P, const TW* b
   constexpr int W = !VEC ? 1 : COLS == 64 && sizeof(TY) == 4 ? 2 : 4, kLanes = COLS / W < 32 ? COLS / W : 32, kAtOnce = 32 / kLanes;
   constexpr int kPasses = 8 * NT / kAtOnce, kQ = COLS / (kLanes * W);
   // y of the next columns is requested as this one's sums go out, where a stage is 16 ranks (3B head 42 -> 40 us, with 3 stages of B
-  // 33); with 32 ranks its registers are wanted for B (7B key, value and receptance, 256 streams 66 us so, 71 ahead)
+  // 33); with 32 ranks its registers are wanted for B (7B key, value and receptance, 256 streams, h in two pieces: 66 us so, 71 ahead)
   constexpr bool kAhead = KC == 16;
   const int my_row = lane / kLanes, my_col = lane % kLanes * W;
   AdaptFew<TY, W> line[kPasses][kQ];

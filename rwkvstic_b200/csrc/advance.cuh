@@ -4,7 +4,7 @@
 //   rows 0, 1   layer norms of row n - 1 of the block's inputs and of its ffn's (the token-shift carries)
 //   rows 2..4   n steps of the WKV recurrence over the kept keys and values
 // Memory-bound: keys and values of the accepted tokens, two rows and the state are read, the state is written (32 blocks of 4096
-// channels, 64 streams, 6 tokens, 573 MB: 99 us; 12 blocks of 768, one stream: 2.7).
+// channels, 64 streams, 6 tokens, 573 MB: 100 us on the GPU, 108 per call; 12 blocks of 768, one stream: 2.9 and 7.9).
 #pragma once
 
 #include "common.cuh"

@@ -9,10 +9,10 @@
 // stream) adds the segments of a row in their order, decides, forms the remaining distribution in the same segments, and walks
 // to the segment, then the token, that holds the uniform number.  The segments depend on the vocabulary alone, so a stream's
 // result does not depend on the other streams of the call.
-// Bounds: the first launch by memory and by turning weights into fp64, 16 a clock and SM (256 streams, vocabulary 50277, 1150
-// rows looked at, 231 MB: 41 us), the second by latency (the same 256 streams, no draft distribution: 12 us, part of it
-// beside the first, 19 where it formed all segments anew; 1 stream of 4 drafted tokens: 9.5 us for both).  All in one launch of
-// a cluster per stream was slower where a stream is alone, 13.9 us against 9.4, since eight CTAs then sum what 50 times more
+// Bounds (times on the GPU alone; a call costs 2 us more, one of a single stream 7): the first launch by memory and by turning
+// weights into fp64, 16 a clock and SM (256 streams, vocabulary 50277, 1150 rows looked at, 231 MB: 41 us), the second by latency (the same 256 streams, no draft distribution: 12 us, part of it
+// beside the first, 19 where it formed all segments anew; 1 stream of 4 drafted tokens: 9.8 us for both).  All in one launch of
+// a cluster per stream was slower where a stream is alone, 13.9 us against 9.8, since eight CTAs then sum what 50 times more
 // warps do here.
 #pragma once
 
